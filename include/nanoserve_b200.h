@@ -27,7 +27,8 @@ typedef enum {
     NS_ERR_CUDA = 4           /* a CUDA runtime call (launch, attribute) failed */
 } ns_status;
 
-typedef enum { NS_BF16 = 0, NS_F32 = 1 } ns_dtype;
+/* NS_INT8 and NS_E4M3 are element types of 8-bit KV pools only. */
+typedef enum { NS_BF16 = 0, NS_F32 = 1, NS_INT8 = 2, NS_E4M3 = 3 } ns_dtype;
 
 /* Library version (major*10000 + minor*100 + patch) and last error text of the calling thread. */
 int ns_version(void);
@@ -304,6 +305,70 @@ int ns_ragged_paged_attn_simple(const void* q, const void* k_pool, const void* v
                                 int32_t head_dim, int32_t block_size, int64_t table_stride, int64_t q_stride,
                                 int64_t out_stride, int64_t pool_block_stride, int64_t pool_pos_stride,
                                 int64_t pool_head_stride, float scale, int dtype, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Rotary positions in fp32 (either pair layout, part of the head, far and scaled positions) and 8-bit KV pools.
+ *
+ * An 8-bit pool holds codes, int8 or e4m3, in the layout of any pool, and one fp32 scale per block and KV head for K and
+ * one for V, [num_blocks, n_kv_heads] through scale_block_stride / scale_head_stride: value = code * scale. The reference
+ * keeps its cache in the model's dtype (nanoserve/kv_cache.py:251-288); no counterpart there.
+ * ---------------------------------------------------------------------------------------------- */
+
+/* cos_out / sin_out [n_tokens, half] fp32 = factor * cos / sin(positions[t] * inv_freq[i]); angle, reduction and function in
+ * fp64, rounded once: positions of any size are exact to fp32. Widens nanoserve/model.py:212-217 Qwen2Model.rope. */
+int ns_rope_tables(const int64_t* positions, const float* inv_freq, double factor, float* cos_out, float* sin_out,
+                   int64_t n_tokens, int32_t half, void* stream);
+
+/* Rotate n_heads query and n_kv_heads key heads of every token and store K and V into one layer's pool.
+ * q / k / v: rows of heads (head stride head_dim) with their own token strides; one merged QKV row is three pointers into it.
+ * The first rot_dim dims of a head are rotated (0: none, cos / sin may be NULL), in pairs (i, i + rot_dim/2), or (2i, 2i+1)
+ * when interleaved: (a, b) -> (a c - b s, b c + a s), each product and each sum rounded to fp32, the result rounded once.
+ * q_out / k_out / v_out: dense, each may be NULL (n_heads may be 0). k_pool / v_pool: both or none; n_slots =
+ * num_blocks * block_size; token t goes to slot slots[t], a slot outside [0, n_slots) stores nothing.
+ * pool_dtype == dtype: rows are copied (two tokens of one call must not name the same slot).
+ * pool_dtype NS_INT8 / NS_E4M3: with A the largest magnitude of the rows of a block that this call writes and Q = 127 / 448,
+ *   S = the smallest power of two >= 2^-100 with A <= Q S (NaN if A is not finite: the block then reads as NaN).
+ *   A call that writes a block's first row starts the block afresh: scale = S, the rows it does not write get code 0.
+ *   Otherwise scale' = max(scale, S), and if it grew the other rows are re-coded round(code * scale / scale').
+ *   code = x / scale' to the nearest code, ties to even. Tokens may come in any order; of two that name one slot the later
+ *   stays. block_size: a power of two up to 64.
+ * Replaces, widened: nanoserve/kernels/fused.py:156 rope_qkv and nanoserve/kv_cache.py:274-279 PagedKVCache.write. */
+int ns_rope_append(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                   const float* cos, const float* sin, int32_t rot_dim, int32_t interleaved, void* q_out, void* k_out,
+                   void* v_out, void* k_pool, void* v_pool, float* k_scale, float* v_scale, const int64_t* slots,
+                   int64_t n_tokens, int64_t n_slots, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                   int32_t block_size, int64_t pool_block_stride, int64_t pool_pos_stride, int64_t pool_head_stride,
+                   int64_t scale_block_stride, int64_t scale_head_stride, int dtype, int pool_dtype, void* stream);
+
+/* out [num_blocks, block_size, n_kv_heads, head_dim] (dense, bf16 or f32) = the values an 8-bit pool stands for. */
+int ns_kv_values(const void* pool, const float* scale, void* out, int64_t num_blocks, int32_t block_size, int32_t n_kv_heads,
+                 int32_t head_dim, int64_t pool_block_stride, int64_t pool_pos_stride, int64_t pool_head_stride,
+                 int64_t scale_block_stride, int64_t scale_head_stride, int dtype, int pool_dtype, void* stream);
+
+/* ns_ragged_paged_attn over 8-bit pools: the same batch description, q and out bf16 or fp32 (dtype). num_blocks and
+ * table_width (entries of a block-table row) bound every access: keys past a table row's width and blocks outside the pool
+ * count as absent. A query that sees no key gets zeros; rows of no sequence are left as they were.
+ * Sequences of one token need no plan; a call with cu_seqlens and n_tokens > n_seqs takes its prefill tiles from the plan in
+ * the workspace (ns_attn_plan with the same seq_lens / cu_seqlens / table_rows). workspace as in ns_ragged_paged_attn; calls
+ * that share one must not overlap. Tensor-core kernels: block_size a multiple of 16 (prefill chunks: 16), head_dim 64 / 128,
+ * 16-byte aligned pools; everything else runs ns_ragged_paged_attn_q8_simple, which needs no workspace (head_dim <= 256).
+ * Replaces, for 8-bit pools: nanoserve/model.py:262-323 _attend and nanoserve/kernels/paged_attention.py:85-105. */
+int ns_ragged_paged_attn_q8(const void* q, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,
+                            const int32_t* block_tables, const int32_t* table_rows, const int32_t* seq_lens,
+                            const int32_t* cu_seqlens, void* out, int32_t n_seqs, int64_t n_tokens, int32_t n_heads,
+                            int32_t n_kv_heads, int32_t head_dim, int32_t block_size, int32_t num_blocks, int32_t table_width,
+                            int64_t table_stride, int64_t q_stride, int64_t out_stride, int64_t pool_block_stride,
+                            int64_t pool_pos_stride, int64_t pool_head_stride, int64_t scale_block_stride,
+                            int64_t scale_head_stride, float scale, int dtype, int pool_dtype, void* workspace,
+                            int64_t workspace_bytes, int32_t ws_max_seqs, int32_t ws_max_tokens, void* stream);
+int ns_ragged_paged_attn_q8_simple(const void* q, const void* k_pool, const void* v_pool, const float* k_scale,
+                                   const float* v_scale, const int32_t* block_tables, const int32_t* table_rows,
+                                   const int32_t* seq_lens, const int32_t* cu_seqlens, void* out, int32_t n_seqs,
+                                   int64_t n_tokens, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t block_size,
+                                   int32_t num_blocks, int32_t table_width, int64_t table_stride, int64_t q_stride,
+                                   int64_t out_stride, int64_t pool_block_stride, int64_t pool_pos_stride,
+                                   int64_t pool_head_stride, int64_t scale_block_stride, int64_t scale_head_stride,
+                                   float scale, int dtype, int pool_dtype, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Step metadata and greedy sampling on the device.

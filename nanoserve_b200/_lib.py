@@ -6,7 +6,7 @@ path never routes through PyTorch ops or CPU code for work this library owns.
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
+from ctypes import c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_void_p
 from pathlib import Path
 
 import os
@@ -16,7 +16,7 @@ import os
 LIB_PATH = Path(__file__).resolve().parent / "lib" / ("libnanoserve_b200_dbg.so" if os.environ.get("NS_DEBUG_LIB") == "1"
                                                       else "libnanoserve_b200.so")
 
-NS_BF16, NS_F32 = 0, 1
+NS_BF16, NS_F32, NS_INT8, NS_E4M3 = 0, 1, 2, 3
 # ns_tuning_knob
 (TUNE_PREFILL_IMPL, TUNE_PREFILL_OVERLAP, TUNE_DECODE_SPLIT_BLOCKS, TUNE_DECODE_MIN_BLOCKS, TUNE_DECODE_SNAP_BLOCKS,
  TUNE_DECODE_BALANCE, TUNE_DECODE_CLUSTER, TUNE_DECODE_CLUSTER_BLOCKS, TUNE_PREFILL_CLUSTER) = range(9)
@@ -64,6 +64,14 @@ SIGNATURES: dict[str, tuple] = {
                                             _I64, _I64, _F, c_int, _P]),
     "ns_ragged_paged_attn_simple": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _I32, _I64,
                                             _I64, _I64, _I64, _I64, _I64, _F, c_int, _P]),
+    "ns_rope_tables": (c_int, [_P, _P, c_double, _P, _P, _I64, _I32, _P]),
+    "ns_rope_append": (c_int, [_P, _P, _P, _I64, _I64, _I64, _P, _P, _I32, _I32, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I32,
+                               _I32, _I32, _I32, _I64, _I64, _I64, _I64, _I64, c_int, c_int, _P]),
+    "ns_kv_values": (c_int, [_P, _P, _P, _I64, _I32, _I32, _I32, _I64, _I64, _I64, _I64, _I64, c_int, c_int, _P]),
+    "ns_ragged_paged_attn_q8": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _I64,
+                                        _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, c_int, c_int, _P, _I64, _I32, _I32, _P]),
+    "ns_ragged_paged_attn_q8_simple": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _I32, _I32, _I32,
+                                               _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, c_int, c_int, _P]),
     "ns_build_step_metadata": (c_int, [_P, _I32, _P, _P, _I32, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _P]),
     "ns_argmax_rows": (c_int, [_P, _I64, _I32, _I32, _P, _P, _P, c_int, _P]),
     "ns_sample_rows": (c_int, [_P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _P, c_int, _P]),
@@ -131,6 +139,12 @@ def dtype_code(dtype) -> int:
     raise NotImplementedError(f"nanoserve_b200 kernels handle bfloat16 and float32, not {dtype}")
 
 
+def kv8_code(dtype) -> int | None:
+    """The code of an 8-bit KV pool's element type, None for any other dtype."""
+    import torch
+    return {torch.int8: NS_INT8, torch.float8_e4m3fn: NS_E4M3}.get(dtype)
+
+
 def stream_ptr() -> int:
     import torch
     return torch.cuda.current_stream().cuda_stream
@@ -144,3 +158,22 @@ def require_cuda(*tensors) -> None:
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise NanoserveB200Error("nanoserve_b200 kernels run on CUDA tensors only (there is no CPU path)")
+
+
+def same_device(*tensors):
+    """The one CUDA device all of the given tensors live on; raises for CPU tensors and for tensors of several devices."""
+    require_cuda(*tensors)
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1:
+        raise NanoserveB200Error(f"tensors of one call live on several devices: {sorted(map(str, devices))}")
+    return devices.pop()
+
+
+def call_on(device, name: str, *args) -> None:
+    """call() with `device` current and its current stream as the last argument (a kernel launch needs both)."""
+    import torch
+    if device.index == torch.cuda.current_device():
+        call(name, *args, stream_ptr())
+        return
+    with torch.cuda.device(device):
+        call(name, *args, stream_ptr())

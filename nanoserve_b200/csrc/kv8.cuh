@@ -1,0 +1,45 @@
+// 8-bit KV pools: codes (int8 or e4m3) in one layer's pool [num_blocks, block_size, n_kv_heads, head_dim] and one fp32
+// scale per block and KV head (K and V apart): value = code * scale.
+#pragma once
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace ns {
+
+// Storage kinds of a pool element. kOrd: bits of the largest code's mantissa and its exponent (127 = 1.984375 * 2^6,
+// 448 = 1.75 * 2^8), from which the smallest power-of-two scale that holds a magnitude follows without a division.
+struct KvInt8 {
+    static constexpr uint32_t kMaxMant = 0x7E0000u;
+    static constexpr int kMaxExp = 6;
+    // Nearest code, ties to even; NaN gives code 0 (its block's scale is NaN then and says so).
+    static __device__ __forceinline__ uint32_t encode(float x) {
+        return x == x ? (uint32_t)__float2int_rn(fminf(fmaxf(x, -127.f), 127.f)) & 0xffu : 0u;
+    }
+    static __device__ __forceinline__ float decode(uint32_t byte) { return (float)(int8_t)byte; }
+};
+struct KvE4m3 {
+    static constexpr uint32_t kMaxMant = 0x600000u;
+    static constexpr int kMaxExp = 8;
+    static __device__ __forceinline__ uint32_t encode(float x) {
+        return x == x ? (uint32_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3) : 0u;
+    }
+    static __device__ __forceinline__ float decode(uint32_t byte) {
+        return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
+    }
+};
+
+// Smallest scale = power of two >= 2^-100 whose largest code reaches the magnitude with these bits (sign cleared); NaN for an
+// infinity or a NaN. Powers of two make x / scale exact, so a code has one rounding, and growing a scale shifts the block's
+// older codes by whole binary places: e4m3 codes survive it unchanged (down to its subnormals), int8 codes round once
+// per doubling. (A scale of exactly A / 127 would leave int8 up to one bit finer, but would round all older codes of the
+// block again for every token that sets a new maximum, 2 to 3 times in a block of 16.)
+template <typename KV> __device__ __forceinline__ float pow2_scale(uint32_t amax_bits) {
+    if (amax_bits >= 0x7f800000u) return __int_as_float(0x7fffffff);
+    int e = (int)(amax_bits >> 23) - 127 - KV::kMaxExp + ((amax_bits & 0x7fffffu) > KV::kMaxMant ? 1 : 0);
+    e = e < -100 ? -100 : e;
+    return __int_as_float((e + 127) << 23);
+}
+
+}  // namespace ns

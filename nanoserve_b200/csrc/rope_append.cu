@@ -1,0 +1,473 @@
+// Rotary position tables in fp32, and the rotation of a step's Q and K fused with the store of K and V into one layer's
+// paged pool: 16/32-bit pools (rows copied to their slots) and 8-bit pools (codes + one scale per block and KV head).
+#include "kv8.cuh"
+
+namespace ns {
+
+// ------------------------------------------------------------------------------------------------ tables
+// cos/sin[t][i] = factor * cos/sin(pos_t * f_i). The angle of a far position needs more than fp32: at position 10^6 an fp32
+// angle is off by 0.03 rad. The product and its reduction to a fraction of a turn are in fp64 (exact to 2^-53 of the
+// angle), and so are sincospi of the reduced angle and the factor: one rounding to fp32 at the end.
+__global__ void __launch_bounds__(256) rope_tables_kernel(const int64_t* __restrict__ pos, const float* __restrict__ inv_freq,
+                                                          double factor, float* __restrict__ cos_out, float* __restrict__ sin_out,
+                                                          int64_t total, int half) {
+    constexpr double kInvPi = 0.31830988618379067154;
+    pdl_launch_dependents();
+    pdl_wait();
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t t = i / half;
+        const double half_turns = (double)pos[t] * (double)inv_freq[i - t * half] * kInvPi;
+        double s, c;
+        sincospi(half_turns - 2.0 * rint(0.5 * half_turns), &s, &c);
+        cos_out[i] = (float)(c * factor);
+        sin_out[i] = (float)(s * factor);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ rotation
+struct RopeAppendParams {
+    const void *q, *k, *v;                    // rows of heads, head stride = head_dim
+    int64_t q_stride, k_stride, v_stride;     // elements between tokens
+    const float *cos, *sin;                   // [n_tokens, rot / 2]
+    int rot, interleaved;
+    void *q_out, *k_out, *v_out;              // dense, each may be null
+    void *k_pool, *v_pool;                    // may be null
+    float *k_scale, *v_scale;                 // 8-bit pools
+    const int64_t* slots;
+    int64_t n_tokens, n_slots;
+    int n_heads, n_kv_heads, head_dim, block_size, block_shift;
+    int64_t blk_stride, pos_stride, head_stride, sc_blk_stride, sc_head_stride;
+    int kv_ctas, planes, chunk;               // 8-bit pools: CTAs of the append role, (head, K or V) planes, tokens per CTA
+};
+
+template <typename T, int V> __device__ __forceinline__ void load_vec(const T* p, float (&x)[V]) {
+    if constexpr (V == 1) {
+        x[0] = to_f32<T>(p[0]);
+    } else {
+#pragma unroll
+        for (int c = 0; c < V / Vec16<T>::N; ++c) {
+            const Vec16<T> r = load16(p + c * Vec16<T>::N);
+#pragma unroll
+            for (int j = 0; j < Vec16<T>::N; ++j) x[c * Vec16<T>::N + j] = r.get(j);
+        }
+    }
+}
+template <typename T, int V> __device__ __forceinline__ void store_vec(T* p, const float (&x)[V]) {
+    if constexpr (V == 1) {
+        p[0] = from_f32<T>(x[0]);
+    } else {
+#pragma unroll
+        for (int c = 0; c < V / Vec16<T>::N; ++c) {
+            Vec16<T> r;
+#pragma unroll
+            for (int j = 0; j < Vec16<T>::N; ++j) r.set(j, x[c * Vec16<T>::N + j]);
+            store16(p + c * Vec16<T>::N, r);
+        }
+    }
+}
+
+// cos / sin of the V dims starting at d0 of a rotated head, one value per dim (a pair shares its two).
+template <int V> __device__ __forceinline__ void load_angles(const float* row, int rot, int interleaved, int d0, float (&a)[V]) {
+    const int half = rot / 2;
+    if (interleaved) {
+        if constexpr (V == 1) {
+            a[0] = row[d0 >> 1];
+        } else {
+#pragma unroll
+            for (int c = 0; c < V / 8; ++c) {
+                const float4 w = *reinterpret_cast<const float4*>(row + (d0 >> 1) + 4 * c);
+                a[8 * c] = a[8 * c + 1] = w.x;
+                a[8 * c + 2] = a[8 * c + 3] = w.y;
+                a[8 * c + 4] = a[8 * c + 5] = w.z;
+                a[8 * c + 6] = a[8 * c + 7] = w.w;
+            }
+        }
+    } else {
+        const float* p = row + (d0 < half ? d0 : d0 - half);
+        if constexpr (V == 1) {
+            a[0] = p[0];
+        } else {
+#pragma unroll
+            for (int c = 0; c < V / 4; ++c) *reinterpret_cast<float4*>(&a[4 * c]) = *reinterpret_cast<const float4*>(p + 4 * c);
+        }
+    }
+}
+
+// The V dims starting at d0 of one rotated head: (a, b) -> (a c - b s, b c + a s), every product and every sum rounded to
+// fp32 (no contraction: the codes of an 8-bit pool are then the same on every path).
+template <typename T, int V>
+__device__ __forceinline__ void rotate_vec(const T* head, int rot, int interleaved, int d0, const float (&c)[V], const float (&s)[V],
+                                           float (&x)[V]) {
+    load_vec<T, V>(head + d0, x);
+    if (interleaved) {
+        if constexpr (V == 1) {
+            const float y = to_f32<T>(head[d0 ^ 1]);
+            const float xc = __fmul_rn(x[0], c[0]), ys = __fmul_rn(y, s[0]);
+            x[0] = (d0 & 1) ? __fadd_rn(xc, ys) : __fsub_rn(xc, ys);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; j += 2) {
+                const float a = x[j], b = x[j + 1];
+                x[j] = __fsub_rn(__fmul_rn(a, c[j]), __fmul_rn(b, s[j]));
+                x[j + 1] = __fadd_rn(__fmul_rn(b, c[j]), __fmul_rn(a, s[j]));
+            }
+        }
+    } else {
+        const int half = rot / 2;
+        const bool lo = d0 < half;
+        float y[V];
+        load_vec<T, V>(head + (lo ? d0 + half : d0 - half), y);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float xc = __fmul_rn(x[j], c[j]), ys = __fmul_rn(y[j], s[j]);
+            x[j] = lo ? __fsub_rn(xc, ys) : __fadd_rn(xc, ys);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ append, 8-bit pools
+// A block's scale depends on every row of it that the call writes, so a block has ONE owner: the warp that holds the first
+// token of the call which lands in it (the leader), whatever order the tokens come in and however often a slot is named.
+// A CTA takes `chunk` tokens and one (head, K or V) plane: it finds the leaders among its tokens, scans all slots of the
+// call for the members of their blocks (the last token that names a slot wins, a block with an earlier token elsewhere
+// is left to that token's CTA), and each warp then takes one leader: largest magnitude, scale, codes.
+constexpr int kAppendChunk = 64;              // most tokens per CTA
+constexpr int kAppendMaxBlock = 64;           // largest block size
+constexpr int kAppendWarps = 8;
+
+template <typename T, typename KV, int V>
+__device__ void append_kv8(const RopeAppendParams& p, int cta) {
+    __shared__ int member[kAppendChunk * kAppendMaxBlock];
+    __shared__ int cand_block[kAppendChunk], cand_tok[kAppendChunk], cand_dead[kAppendChunk];
+    __shared__ int n_cand;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int plane = cta % p.planes, bs = p.block_size, mask = bs - 1;
+    const int64_t t0 = (int64_t)(cta / p.planes) * p.chunk;
+    const int n_here = (int)(p.n_tokens - t0 < p.chunk ? p.n_tokens - t0 : p.chunk);
+    const int n_tok = (int)p.n_tokens;
+    if (tid == 0) n_cand = 0;
+    for (int i = tid; i < p.chunk * bs; i += blockDim.x) member[i] = -1;
+    __syncthreads();
+    auto block_of = [&](int64_t slot) -> int { return (slot >= 0 && slot < p.n_slots) ? (int)(slot >> p.block_shift) : -1; };
+    if (tid < n_here) {
+        const int t = (int)t0 + tid;
+        const int b = block_of(p.slots[t]);
+        if (b >= 0 && (t == 0 || block_of(p.slots[t - 1]) != b)) {
+            const int c = atomicAdd(&n_cand, 1);
+            cand_block[c] = b;
+            cand_tok[c] = t;
+            cand_dead[c] = 0;
+        }
+    }
+    __syncthreads();
+    const int nc = n_cand;
+    for (int t = tid; t < n_tok; t += blockDim.x) {
+        const int64_t slot = p.slots[t];
+        const int b = block_of(slot);
+        if (b < 0) continue;
+        for (int c = 0; c < nc; ++c)
+            if (cand_block[c] == b) {
+                if (t < cand_tok[c]) cand_dead[c] = 1;
+                else atomicMax(&member[c * bs + ((int)slot & mask)], t);
+            }
+    }
+    __syncthreads();
+
+    const int head = plane >> 1, is_v = plane & 1, hd = p.head_dim;
+    const T* src = reinterpret_cast<const T*>(is_v ? p.v : p.k) + (int64_t)head * hd;
+    const int64_t src_stride = is_v ? p.v_stride : p.k_stride;
+    uint8_t* pool = reinterpret_cast<uint8_t*>(is_v ? p.v_pool : p.k_pool) + head * p.head_stride;
+    float* scales = (is_v ? p.v_scale : p.k_scale) + head * p.sc_head_stride;
+    const int cpr = hd / V, items = bs * cpr, half = p.rot / 2;
+    auto values = [&](int t, int d0, float (&x)[V]) {
+        const T* row = src + t * src_stride;
+        if (!is_v && d0 < p.rot) {
+            float c[V], s[V];
+            load_angles<V>(p.cos + (int64_t)t * half, p.rot, p.interleaved, d0, c);
+            load_angles<V>(p.sin + (int64_t)t * half, p.rot, p.interleaved, d0, s);
+            rotate_vec<T, V>(row, p.rot, p.interleaved, d0, c, s, x);
+        } else {
+            load_vec<T, V>(row + d0, x);
+        }
+    };
+    for (int c = warp; c < nc; c += kAppendWarps) {
+        if (cand_dead[c]) continue;
+        const int* mem = member + c * bs;
+        const int64_t blk = cand_block[c];
+        uint32_t amax = 0;
+        for (int i = lane; i < items; i += 32) {
+            const int off = i / cpr, t = mem[off];
+            if (t < 0) continue;
+            float x[V];
+            values(t, (i - off * cpr) * V, x);
+#pragma unroll
+            for (int j = 0; j < V; ++j) amax = max(amax, (uint32_t)__float_as_int(x[j]) & 0x7fffffffu);
+        }
+        amax = __reduce_max_sync(0xffffffffu, amax);
+        const float s_new = pow2_scale<KV>(amax);
+        float* sc = scales + blk * p.sc_blk_stride;
+        const float old = *sc;
+        const bool fresh = mem[0] >= 0;
+        const float now = fresh ? s_new : (old != old || s_new != s_new) ? __int_as_float(0x7fffffff) : fmaxf(old, s_new);
+        const float inv = 1.0f / now, ratio = old / now;
+        __syncwarp();
+        if (lane == 0) *sc = now;
+        for (int i = lane; i < items; i += 32) {
+            const int off = i / cpr, t = mem[off], d0 = (i - off * cpr) * V;
+            uint8_t* dst = pool + blk * p.blk_stride + (int64_t)off * p.pos_stride + d0;
+            float x[V];
+            if (t >= 0) {
+                values(t, d0, x);
+#pragma unroll
+                for (int j = 0; j < V; ++j) x[j] = __fmul_rn(x[j], inv);
+            } else if (fresh) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) x[j] = 0.f;
+            } else if (now == old) {
+                continue;
+            } else {
+                if constexpr (V == 1) {
+                    x[0] = __fmul_rn(KV::decode(dst[0]), ratio);
+                } else {
+                    const uint2 w = *reinterpret_cast<const uint2*>(dst);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(KV::decode(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 0xffu), ratio);
+                }
+            }
+            if constexpr (V == 1) {
+                dst[0] = (uint8_t)KV::encode(x[0]);
+            } else {
+                uint2 w = make_uint2(0u, 0u);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) (j < 4 ? w.x : w.y) |= KV::encode(x[j]) << (8 * (j & 3));
+                *reinterpret_cast<uint2*>(dst) = w;
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ the kernel
+struct NoKv8 {};
+
+// CTAs [0, kv_ctas): the append role (8-bit pools). The others walk (token, V dims, group of heads): the angles of the V
+// dims are loaded once for kHeadsPerItem heads.
+constexpr int kHeadsPerItem = 4;
+
+template <typename T, typename KV, int V>
+__global__ void __launch_bounds__(kAppendWarps * 32) rope_append_kernel(const RopeAppendParams p) {
+    constexpr bool kv8 = !std::is_same<KV, NoKv8>::value;
+    pdl_launch_dependents();
+    pdl_wait();
+    if constexpr (kv8) {
+        if ((int)blockIdx.x < p.kv_ctas) {
+            append_kv8<T, KV, V>(p, blockIdx.x);
+            return;
+        }
+    }
+    const int hd = p.head_dim, cpr = hd / V, half = p.rot / 2, NH = p.n_heads, NKV = p.n_kv_heads;
+    const bool dense_k = p.k_out != nullptr, dense_v = p.v_out != nullptr, pool16 = !kv8 && p.k_pool != nullptr;
+    const int h0 = p.q_out != nullptr ? 0 : NH;                                       // heads [h0, h1) of q | k | v have work here
+    const int h1 = (dense_v || pool16) ? NH + 2 * NKV : dense_k ? NH + NKV : NH;
+    const int groups = (h1 - h0 + kHeadsPerItem - 1) / kHeadsPerItem;
+    const int64_t total = p.n_tokens * groups * cpr;
+    for (int64_t i = (blockIdx.x - p.kv_ctas) * (int64_t)blockDim.x + threadIdx.x; i < total;
+         i += (int64_t)(gridDim.x - p.kv_ctas) * blockDim.x) {
+        const int64_t tg = i / cpr;
+        const int d0 = (int)(i - tg * cpr) * V;
+        const int64_t t = tg / groups;
+        const int grp = (int)(tg - t * groups);
+        float c[V], s[V];
+        const bool rotated = d0 < p.rot;
+        if (rotated) {
+            load_angles<V>(p.cos + t * half, p.rot, p.interleaved, d0, c);
+            load_angles<V>(p.sin + t * half, p.rot, p.interleaved, d0, s);
+        }
+        const int64_t slot = pool16 ? p.slots[t] : -1;
+        const bool stored = pool16 && slot >= 0 && slot < p.n_slots;
+        const int64_t row_off = stored ? (slot / p.block_size) * p.blk_stride + (slot % p.block_size) * p.pos_stride : 0;
+#pragma unroll
+        for (int e = 0; e < kHeadsPerItem; ++e) {
+            const int h = h0 + grp * kHeadsPerItem + e;
+            if (h >= h1) break;
+            const bool is_q = h < NH, is_v = h >= NH + NKV;
+            const int g = is_q ? h : is_v ? h - NH - NKV : h - NH;
+            const T* head = (is_q   ? reinterpret_cast<const T*>(p.q) + t * p.q_stride
+                             : is_v ? reinterpret_cast<const T*>(p.v) + t * p.v_stride
+                                    : reinterpret_cast<const T*>(p.k) + t * p.k_stride) + (int64_t)g * hd;
+            float x[V];
+            if (rotated && !is_v) rotate_vec<T, V>(head, p.rot, p.interleaved, d0, c, s, x);
+            else load_vec<T, V>(head + d0, x);
+            T* dense = reinterpret_cast<T*>(is_q ? p.q_out : is_v ? p.v_out : p.k_out);
+            if (dense != nullptr) store_vec<T, V>(dense + (t * (is_q ? NH : NKV) + g) * hd + d0, x);
+            if (stored && !is_q) {
+                T* pool = reinterpret_cast<T*>(is_v ? p.v_pool : p.k_pool);
+                store_vec<T, V>(pool + row_off + g * p.head_stride + d0, x);
+            }
+        }
+    }
+}
+
+template <typename T, typename KV, int V> static int launch_rope_append(RopeAppendParams p, cudaStream_t st) {
+    constexpr bool kv8 = !std::is_same<KV, NoKv8>::value;
+    const int threads = kAppendWarps * 32;
+    int sms = device_sm_count();
+    if (sms <= 0) sms = 148;
+    p.kv_ctas = 0;
+    p.planes = 2 * p.n_kv_heads;
+    // Tokens per append CTA: few where the step is small (a decode step's tokens are one leader each: more CTAs), 64 where
+    // the scan of all slots, which every CTA repeats, would otherwise dominate.
+    p.chunk = p.n_tokens <= 1024 ? 16 : kAppendChunk;
+    if (kv8) p.kv_ctas = (int)((p.n_tokens + p.chunk - 1) / p.chunk) * p.planes;
+    const int heads = (p.q_out != nullptr ? p.n_heads : 0) + ((p.v_out || (!kv8 && p.k_pool)) ? 2 * p.n_kv_heads : p.k_out ? p.n_kv_heads : 0);
+    const int64_t items = p.n_tokens * ((heads + kHeadsPerItem - 1) / kHeadsPerItem) * (p.head_dim / V);
+    int64_t ctas = (items + threads - 1) / threads;
+    if (ctas > sms * 8) ctas = sms * 8;
+    if (ctas + p.kv_ctas == 0) return NS_OK;
+    cudaError_t e = launch_pdl(rope_append_kernel<T, KV, V>, dim3((unsigned)(ctas + p.kv_ctas)), dim3(threads), 0, st, p);
+    if (e != cudaSuccess) return fail(NS_ERR_CUDA, "rope_append: launch failed: %s", cudaGetErrorString(e));
+    return NS_OK;
+}
+
+template <typename T, int V> static int dispatch_pool(const RopeAppendParams& p, int pool_dtype, cudaStream_t st) {
+    if (pool_dtype == NS_INT8) return launch_rope_append<T, KvInt8, V>(p, st);
+    if (pool_dtype == NS_E4M3) return launch_rope_append<T, KvE4m3, V>(p, st);
+    return launch_rope_append<T, NoKv8, V>(p, st);
+}
+
+// ------------------------------------------------------------------------------------------------ values of an 8-bit pool
+template <typename T, typename KV, int V>
+__global__ void __launch_bounds__(256) kv_values_kernel(const uint8_t* __restrict__ pool, const float* __restrict__ scale, T* __restrict__ out,
+                                                        int64_t rows, int block_size, int n_kv_heads, int head_dim, int64_t blk_stride,
+                                                        int64_t pos_stride, int64_t head_stride, int64_t sc_blk, int64_t sc_head) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int cpr = head_dim / V;
+    const int64_t total = rows * n_kv_heads * cpr;
+    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t rh = i / cpr, row = rh / n_kv_heads, b = row / block_size;
+        const int d0 = (int)(i - rh * cpr) * V, h = (int)(rh - row * n_kv_heads), off = (int)(row - b * block_size);
+        const uint8_t* src = pool + b * blk_stride + off * pos_stride + h * head_stride + d0;
+        const float s = scale[b * sc_blk + h * sc_head];
+        float x[V];
+        if constexpr (V == 1) {
+            x[0] = KV::decode(src[0]) * s;
+        } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(src);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = KV::decode(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 0xffu) * s;
+        }
+        store_vec<T, V>(out + i * V, x);
+    }
+}
+
+template <typename T, typename KV, int V>
+static int launch_kv_values(const void* pool, const float* scale, void* out, int64_t rows, int bs, int nkv, int hd, int64_t s0, int64_t s1,
+                            int64_t s2, int64_t c0, int64_t c1, cudaStream_t st) {
+    int sms = device_sm_count();
+    if (sms <= 0) sms = 148;
+    int64_t ctas = (rows * nkv * (hd / V) + 255) / 256;
+    if (ctas > sms * 8) ctas = sms * 8;
+    cudaError_t e = launch_pdl(kv_values_kernel<T, KV, V>, dim3((unsigned)ctas), dim3(256), 0, st, (const uint8_t*)pool, scale, (T*)out, rows, bs,
+                               nkv, hd, s0, s1, s2, c0, c1);
+    if (e != cudaSuccess) return fail(NS_ERR_CUDA, "kv_values: launch failed: %s", cudaGetErrorString(e));
+    return NS_OK;
+}
+
+}  // namespace ns
+
+using namespace ns;
+
+extern "C" int ns_rope_tables(const int64_t* positions, const float* inv_freq, double factor, float* cos_out, float* sin_out,
+                              int64_t n_tokens, int32_t half, void* stream) {
+    NS_REQUIRE(n_tokens >= 0 && half >= 0, NS_ERR_INVALID_ARG, "rope_tables: bad shape");
+    if (n_tokens == 0 || half == 0) return NS_OK;
+    NS_REQUIRE(positions && inv_freq && cos_out && sin_out, NS_ERR_INVALID_ARG, "rope_tables: null pointer");
+    int sms = device_sm_count();
+    if (sms <= 0) sms = 148;
+    int64_t ctas = (n_tokens * half + 255) / 256;
+    if (ctas > sms * 8) ctas = sms * 8;
+    cudaError_t e = launch_pdl(rope_tables_kernel, dim3((unsigned)ctas), dim3(256), 0, (cudaStream_t)stream, positions, inv_freq, factor,
+                               cos_out, sin_out, n_tokens * half, half);
+    if (e != cudaSuccess) return fail(NS_ERR_CUDA, "rope_tables: launch failed: %s", cudaGetErrorString(e));
+    return NS_OK;
+}
+
+extern "C" int ns_rope_append(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
+                              const float* cos, const float* sin, int32_t rot_dim, int32_t interleaved, void* q_out, void* k_out,
+                              void* v_out, void* k_pool, void* v_pool, float* k_scale, float* v_scale, const int64_t* slots,
+                              int64_t n_tokens, int64_t n_slots, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
+                              int32_t block_size, int64_t pool_block_stride, int64_t pool_pos_stride, int64_t pool_head_stride,
+                              int64_t scale_block_stride, int64_t scale_head_stride, int dtype, int pool_dtype, void* stream) {
+    NS_REQUIRE(n_tokens >= 0 && n_heads >= 0 && n_kv_heads > 0 && head_dim > 0, NS_ERR_INVALID_ARG, "rope_append: bad shape");
+    NS_REQUIRE(dtype == NS_BF16 || dtype == NS_F32, NS_ERR_UNSUPPORTED, "rope_append: dtype %d", dtype);
+    NS_REQUIRE(rot_dim >= 0 && rot_dim % 2 == 0 && rot_dim <= head_dim, NS_ERR_INVALID_ARG,
+               "rope_append: rotary dim %d must be even and at most head_dim %d", rot_dim, head_dim);
+    NS_REQUIRE((k_pool == nullptr) == (v_pool == nullptr), NS_ERR_INVALID_ARG, "rope_append: need both pools or none");
+    const bool kv8 = k_pool != nullptr && (pool_dtype == NS_INT8 || pool_dtype == NS_E4M3);
+    NS_REQUIRE(k_pool == nullptr || kv8 || pool_dtype == dtype, NS_ERR_UNSUPPORTED, "rope_append: pool dtype %d with activations of dtype %d",
+               pool_dtype, dtype);
+    if (n_tokens == 0) return NS_OK;
+    NS_REQUIRE(k && v && (q || n_heads == 0 || !q_out), NS_ERR_INVALID_ARG, "rope_append: null pointer");
+    NS_REQUIRE(rot_dim == 0 || (cos && sin), NS_ERR_INVALID_ARG, "rope_append: rotary dim %d without tables", rot_dim);
+    if (k_pool != nullptr) {
+        NS_REQUIRE(slots, NS_ERR_INVALID_ARG, "rope_append: pools given without slots");
+        NS_REQUIRE(block_size > 0 && n_slots >= 0, NS_ERR_INVALID_ARG, "rope_append: bad pool shape");
+    }
+    if (kv8) {
+        NS_REQUIRE(k_scale && v_scale, NS_ERR_INVALID_ARG, "rope_append: an 8-bit pool needs its scales");
+        NS_REQUIRE(block_size <= kAppendMaxBlock && (block_size & (block_size - 1)) == 0, NS_ERR_UNSUPPORTED,
+                   "rope_append: 8-bit pools take blocks of 1, 2, 4 ... %d tokens, not %d", kAppendMaxBlock, block_size);
+        NS_REQUIRE(n_tokens <= (1 << 24) && n_slots < ((int64_t)1 << 31), NS_ERR_UNSUPPORTED, "rope_append: %lld tokens / %lld slots",
+                   (long long)n_tokens, (long long)n_slots);
+    }
+    RopeAppendParams p = {};
+    p.q = q; p.k = k; p.v = v; p.q_stride = q_stride; p.k_stride = k_stride; p.v_stride = v_stride;
+    p.cos = cos; p.sin = sin; p.rot = rot_dim; p.interleaved = interleaved ? 1 : 0;
+    p.q_out = n_heads > 0 ? q_out : nullptr; p.k_out = k_out; p.v_out = v_out; p.k_pool = k_pool; p.v_pool = v_pool;
+    p.k_scale = k_scale; p.v_scale = v_scale; p.slots = slots; p.n_tokens = n_tokens; p.n_slots = n_slots;
+    p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.head_dim = head_dim; p.block_size = block_size > 0 ? block_size : 1;
+    while ((1 << p.block_shift) < p.block_size) ++p.block_shift;
+    p.blk_stride = pool_block_stride; p.pos_stride = pool_pos_stride; p.head_stride = pool_head_stride;
+    p.sc_blk_stride = scale_block_stride; p.sc_head_stride = scale_head_stride;
+    const int kind = k_pool == nullptr ? dtype : pool_dtype;
+    cudaStream_t st = (cudaStream_t)stream;
+    // 8 dims at a time where every 8-dim piece of every buffer is 16-byte aligned (8-byte for codes) and rotated pieces lie
+    // wholly on one side of a pair; one dim at a time otherwise.
+    const int64_t e = dtype == NS_F32 ? 4 : 8;            // elements per 16 bytes
+    uintptr_t a = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)k_out | (uintptr_t)v_out | (uintptr_t)cos | (uintptr_t)sin;
+    bool wide = head_dim % 8 == 0 && (a & 15) == 0 && k_stride % e == 0 && v_stride % e == 0 && (q_stride % e == 0 || n_heads == 0) &&
+                (interleaved ? rot_dim % 8 == 0 : rot_dim % 16 == 0);
+    if (k_pool != nullptr) {
+        const int64_t pe = kv8 ? 8 : e;
+        wide = wide && (((uintptr_t)k_pool | (uintptr_t)v_pool) & (kv8 ? 7 : 15)) == 0 && pool_block_stride % pe == 0 &&
+               pool_pos_stride % pe == 0 && pool_head_stride % pe == 0;
+    }
+    if (dtype == NS_BF16) return wide ? dispatch_pool<__nv_bfloat16, 8>(p, kind, st) : dispatch_pool<__nv_bfloat16, 1>(p, kind, st);
+    return wide ? dispatch_pool<float, 8>(p, kind, st) : dispatch_pool<float, 1>(p, kind, st);
+}
+
+extern "C" int ns_kv_values(const void* pool, const float* scale, void* out, int64_t num_blocks, int32_t block_size, int32_t n_kv_heads,
+                            int32_t head_dim, int64_t pool_block_stride, int64_t pool_pos_stride, int64_t pool_head_stride,
+                            int64_t scale_block_stride, int64_t scale_head_stride, int dtype, int pool_dtype, void* stream) {
+    NS_REQUIRE(num_blocks >= 0 && block_size > 0 && n_kv_heads > 0 && head_dim > 0, NS_ERR_INVALID_ARG, "kv_values: bad shape");
+    NS_REQUIRE(dtype == NS_BF16 || dtype == NS_F32, NS_ERR_UNSUPPORTED, "kv_values: output dtype %d", dtype);
+    NS_REQUIRE(pool_dtype == NS_INT8 || pool_dtype == NS_E4M3, NS_ERR_UNSUPPORTED, "kv_values: pool dtype %d is not an 8-bit one", pool_dtype);
+    if (num_blocks == 0) return NS_OK;
+    NS_REQUIRE(pool && scale && out, NS_ERR_INVALID_ARG, "kv_values: null pointer");
+    cudaStream_t st = (cudaStream_t)stream;
+    const bool wide = head_dim % 8 == 0 && ((uintptr_t)out & 15) == 0 && ((uintptr_t)pool & 7) == 0 && pool_block_stride % 8 == 0 &&
+                      pool_pos_stride % 8 == 0 && pool_head_stride % 8 == 0;
+    const int64_t rows = num_blocks * block_size;
+#define NS_GO(T, KV)                                                                                                                          \
+    return wide ? launch_kv_values<T, KV, 8>(pool, scale, out, rows, block_size, n_kv_heads, head_dim, pool_block_stride, pool_pos_stride,    \
+                                             pool_head_stride, scale_block_stride, scale_head_stride, st)                                     \
+                : launch_kv_values<T, KV, 1>(pool, scale, out, rows, block_size, n_kv_heads, head_dim, pool_block_stride, pool_pos_stride,    \
+                                             pool_head_stride, scale_block_stride, scale_head_stride, st)
+    if (dtype == NS_BF16) {
+        if (pool_dtype == NS_INT8) NS_GO(__nv_bfloat16, KvInt8);
+        NS_GO(__nv_bfloat16, KvE4m3);
+    }
+    if (pool_dtype == NS_INT8) NS_GO(float, KvInt8);
+    NS_GO(float, KvE4m3);
+#undef NS_GO
+}

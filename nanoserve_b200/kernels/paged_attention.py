@@ -44,6 +44,20 @@ class AttnWorkspace:
 
 
 _cached: dict[tuple, AttnWorkspace] = {}
+_cached_q8: dict[tuple, AttnWorkspace] = {}
+
+
+def _workspace_q8(device, n_seqs: int, n_tokens: int, n_heads: int, head_dim: int) -> AttnWorkspace:
+    """The workspace of a call over an 8-bit pool that brings none: one per device and stream, so that calls on two streams
+    never share one; inside a graph capture a new one, which belongs to the graph."""
+    cap_s, cap_t = max(256, 1 << (max(n_seqs, 1) - 1).bit_length()), max(4096, 1 << (max(n_tokens, 1) - 1).bit_length())
+    if torch.cuda.is_current_stream_capturing():
+        return AttnWorkspace(max(n_seqs, 1), max(n_tokens, 1), n_heads, head_dim, device)
+    key = (device.index, torch.cuda.current_stream(device).cuda_stream, n_heads, head_dim)
+    ws = _cached_q8.get(key)
+    if ws is None or not ws.fits(n_seqs, n_tokens, n_heads, head_dim):
+        ws = _cached_q8[key] = AttnWorkspace(cap_s, cap_t, n_heads, head_dim, device)
+    return ws
 
 
 def _workspace_for(device, n_seqs: int, n_tokens: int, n_heads: int, head_dim: int) -> AttnWorkspace:
@@ -63,11 +77,56 @@ def _check_pool(q, k_pool, v_pool):
     assert k_pool.dtype == q.dtype and v_pool.dtype == q.dtype
 
 
+def _attend_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, seq_lens, cu_seqlens, scale, n_seqs, workspace, planned, out,
+               simple) -> torch.Tensor:
+    """Ragged attention over an int8 / float8_e4m3fn pool (ns_ragged_paged_attn_q8)."""
+    from nanoserve_b200.kernels.rotary import check_kv8_scales
+    dev = _lib.same_device(q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, seq_lens, cu_seqlens, out)
+    assert k_pool.dim() == 4 and q.dim() == 3 and v_pool.shape == k_pool.shape
+    assert q.stride(-1) == 1 and k_pool.stride(-1) == 1 and v_pool.stride() == k_pool.stride() and v_pool.dtype == k_pool.dtype
+    assert q.stride(1) == q.shape[2] or q.shape[1] == 1, "query heads must be adjacent (head stride == head_dim)"
+    check_kv8_scales(k_pool, k_scale, v_scale)
+    assert block_tables.dtype == torch.int32 and block_tables.dim() == 2 and (block_tables.stride(1) == 1 or block_tables.shape[1] <= 1)
+    assert seq_lens.dtype == torch.int32 and seq_lens.is_contiguous() and seq_lens.shape[0] >= n_seqs
+    assert cu_seqlens is None or (cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous() and cu_seqlens.shape[0] > n_seqs)
+    assert table_rows is None or (table_rows.dtype == torch.int32 and table_rows.is_contiguous() and table_rows.shape[0] >= n_seqs)
+    assert table_rows is not None or block_tables.shape[0] >= n_seqs, "block_tables has a row per sequence"
+    N, n_heads, head_dim = q.shape
+    num_blocks, block_size, n_kv_heads, hd = k_pool.shape
+    assert hd == head_dim and (cu_seqlens is not None or N == n_seqs)
+    if out is None:
+        out = torch.empty(N, n_heads, head_dim, device=dev, dtype=q.dtype)
+    else:
+        assert out.shape == q.shape and out.stride(-1) == 1 and (out.stride(1) == head_dim or n_heads == 1) and out.dtype == q.dtype
+    common = (q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
+              _lib.ptr(table_rows), seq_lens.data_ptr(), _lib.ptr(cu_seqlens), out.data_ptr(), n_seqs, N, n_heads, n_kv_heads, head_dim,
+              block_size, num_blocks, block_tables.shape[1], block_tables.stride(0), q.stride(0), out.stride(0), *k_pool.stride()[:3],
+              *k_scale.stride(), float(scale), _lib.dtype_code(q.dtype), _lib.kv8_code(k_pool.dtype))
+    if simple:
+        _lib.call_on(dev, "ns_ragged_paged_attn_q8_simple", *common)
+        return out
+    with torch.cuda.device(dev):
+        ws = workspace or _workspace_q8(dev, n_seqs, N, n_heads, head_dim)
+        mixed = cu_seqlens is not None and N > n_seqs
+        if mixed and not planned:
+            ws.plan(seq_lens, cu_seqlens, n_seqs, block_size, table_rows)
+        _lib.call("ns_ragged_paged_attn_q8", *common, ws.buf.data_ptr(), ws.nbytes, ws.max_seqs, ws.max_tokens, _lib.stream_ptr())
+    if mixed:
+        _lib.note_launches(1)          # the prefill-tile kernel is launched next to the decode kernel
+    return out
+
+
 def paged_attention_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Tensor,
-                           context_lens: torch.Tensor, scale: float, workspace: AttnWorkspace | None = None) -> torch.Tensor:
+                           context_lens: torch.Tensor, scale: float, workspace: AttnWorkspace | None = None,
+                           k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> torch.Tensor:
     """q: [B, n_heads, head_dim]; k_pool/v_pool: ONE layer's pool [num_blocks, block_size, n_kv_heads, head_dim];
     block_tables: int32 [B, max_blocks]; context_lens: int32 [B] (includes the new token, whose K/V must already
-    be written). Returns [B, n_heads, head_dim]."""
+    be written). An int8 / float8_e4m3fn pool comes with k_scale / v_scale, fp32 [num_blocks, n_kv_heads] (q may then be
+    bf16 or fp32). Returns [B, n_heads, head_dim]."""
+    if _lib.kv8_code(k_pool.dtype) is not None:
+        return _attend_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, None, context_lens, None, scale, q.shape[0], workspace, False,
+                          None, False)
+    assert k_scale is None and v_scale is None, "scales belong to 8-bit pools"
     _lib.require_cuda(q, k_pool, v_pool, block_tables, context_lens)
     _check_pool(q, k_pool, v_pool)
     assert block_tables.dtype == torch.int32 and context_lens.dtype == torch.int32
@@ -110,13 +169,19 @@ def ragged_paged_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.
                            seq_lens: torch.Tensor, cu_seqlens: torch.Tensor | None, scale: float, *,
                            n_seqs: int | None = None, table_rows: torch.Tensor | None = None,
                            workspace: AttnWorkspace | None = None, planned: bool = False,
-                           out: torch.Tensor | None = None, simple: bool = False) -> torch.Tensor:
+                           out: torch.Tensor | None = None, simple: bool = False, k_scale: torch.Tensor | None = None,
+                           v_scale: torch.Tensor | None = None) -> torch.Tensor:
     """Attention for a mixed step. q: [N, n_heads, head_dim] = the flattened query tokens of S sequences;
     sequence s owns rows cu_seqlens[s]..cu_seqlens[s+1]-1 and seq_lens[s] keys (context + its new tokens,
     already in the pool), reached through block_tables[table_rows[s] if given else s]. cu_seqlens=None means
     one token per sequence. `planned=True` says workspace.plan(...) was already called for this step (the
     per-layer fast path); otherwise the plan is built here. `simple=True` forces the scalar fp32-accumulating
-    kernel. Returns [N, n_heads, head_dim]."""
+    kernel. An int8 / float8_e4m3fn pool comes with k_scale / v_scale, fp32 [num_blocks, n_kv_heads]; q is then bf16 or
+    fp32, and a plan is needed only when some sequence has more than one token. Returns [N, n_heads, head_dim]."""
+    if _lib.kv8_code(k_pool.dtype) is not None:
+        return _attend_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, seq_lens, cu_seqlens, scale,
+                          int(n_seqs) if n_seqs is not None else seq_lens.shape[0], workspace, planned, out, simple)
+    assert k_scale is None and v_scale is None, "scales belong to 8-bit pools"
     _lib.require_cuda(q, k_pool, v_pool, block_tables, seq_lens, cu_seqlens, table_rows)
     _check_pool(q, k_pool, v_pool)
     assert block_tables.dtype == torch.int32 and seq_lens.dtype == torch.int32 and block_tables.stride(-1) == 1

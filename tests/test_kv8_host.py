@@ -1,0 +1,146 @@
+"""8-bit KV pools and rotary positions: what is refused (before any launch), and the frequencies' formulas. No GPU."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from nanoserve_b200 import _lib
+from nanoserve_b200.kernels.rotary import check_kv8_scales, kv_values, rope_append, rope_tables, rotary_frequencies
+
+P, NUL, F = ctypes.c_void_p, None, ctypes.c_float
+INVALID, UNSUPPORTED, WORKSPACE = 1, 2, 3
+
+
+def msg():
+    return _lib.load().ns_last_error().decode()
+
+
+def rope_args(**kw):
+    a = dict(q=P(256), k=P(512), v=P(1024), qs=1152, ks=1152, vs=1152, cos=P(2048), sin=P(4096), rot=64, inter=0, qo=P(8192), ko=NUL, vo=NUL,
+             kp=P(16384), vp=P(32768), ksc=P(65536), vsc=P(131072), slots=P(262144), n=4, n_slots=1024, nh=14, nkv=2, hd=64, bs=16, sb=2048,
+             sp=128, sh=64, scb=2, sch=1, dt=_lib.NS_BF16, pdt=_lib.NS_INT8, st=NUL)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return list(a.values())
+
+
+def test_rope_append_refusals():
+    f = _lib.load().ns_rope_append
+    assert f(*rope_args(n=0)) == 0
+    assert f(*rope_args(n=-1)) == INVALID
+    assert f(*rope_args(rot=63)) == INVALID and "rotary dim 63" in msg()
+    assert f(*rope_args(rot=66)) == INVALID
+    assert f(*rope_args(cos=NUL)) == INVALID and "without tables" in msg()
+    assert f(*rope_args(vp=NUL)) == INVALID and "both pools" in msg()
+    assert f(*rope_args(slots=NUL)) == INVALID and "slots" in msg()
+    assert f(*rope_args(vsc=NUL)) == INVALID and "scales" in msg()
+    assert f(*rope_args(bs=24)) == UNSUPPORTED and "blocks of" in msg()
+    assert f(*rope_args(bs=128)) == UNSUPPORTED
+    assert f(*rope_args(dt=7)) == UNSUPPORTED
+    assert f(*rope_args(pdt=_lib.NS_F32)) == UNSUPPORTED and "pool dtype" in msg()
+    assert f(*rope_args(pdt=9)) == UNSUPPORTED
+    assert f(*rope_args(k=NUL)) == INVALID and "null" in msg()
+
+
+def attn_args(**kw):
+    a = dict(q=P(256), k=P(512), v=P(1024), ks=P(2048), vs=P(4096), bt=P(8192), rows=NUL, lens=P(16384), cu=NUL, out=P(32768), S=2, N=2, nh=14,
+             nkv=2, hd=64, bs=16, nb=64, tw=4, ts=4, qs=896, os=896, pb=2048, pp=128, ph=64, sb=2, sh=1, scale=F(0.125), dt=_lib.NS_BF16,
+             pdt=_lib.NS_INT8, ws=NUL, wsb=0, wss=0, wst=0, st=NUL)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return list(a.values())
+
+
+def test_attention_refusals():
+    lib = _lib.load()
+    f = lib.ns_ragged_paged_attn_q8
+    simple = lambda **kw: lib.ns_ragged_paged_attn_q8_simple(*(attn_args(**kw)[:-5] + [NUL]))
+    for call in (lambda **kw: f(*attn_args(**kw)), simple):
+        assert call(S=0, N=0) == 0
+        assert call(S=-1) == INVALID
+        assert call(nh=15) == INVALID and "not divisible" in msg()
+        assert call(dt=2) == UNSUPPORTED
+        assert call(pdt=_lib.NS_BF16) == UNSUPPORTED and "8-bit" in msg()
+        assert call(N=3) == INVALID and "one token" in msg()
+        assert call(vs=NUL) == INVALID and "null" in msg()
+        assert call(tw=-1) == INVALID
+    assert simple(hd=300) == UNSUPPORTED and "head_dim" in msg()
+
+
+def test_values_and_tables_refusals():
+    lib = _lib.load()
+    v = lambda dt, pdt, **kw: lib.ns_kv_values(P(256), kw.get("scale", P(512)), P(1024), kw.get("nb", 2), 16, 2, 64, 2048, 128, 64, 2, 1, dt, pdt, NUL)
+    assert v(_lib.NS_BF16, _lib.NS_INT8, nb=0) == 0
+    assert v(_lib.NS_INT8, _lib.NS_INT8) == UNSUPPORTED
+    assert v(_lib.NS_F32, _lib.NS_F32) == UNSUPPORTED
+    assert v(_lib.NS_F32, _lib.NS_E4M3, scale=NUL) == INVALID
+    assert lib.ns_rope_tables(NUL, NUL, ctypes.c_double(1.0), NUL, NUL, 0, 4, NUL) == 0
+    assert lib.ns_rope_tables(NUL, NUL, ctypes.c_double(1.0), NUL, NUL, 1, 4, NUL) == INVALID
+
+
+def test_python_refusals():
+    i8 = torch.zeros(2, 16, 2, 64, dtype=torch.int8)
+    with pytest.raises(ValueError):
+        check_kv8_scales(i8, None, None)
+    with pytest.raises(AssertionError):
+        check_kv8_scales(i8, torch.zeros(2, 3))
+    with pytest.raises(AssertionError):
+        check_kv8_scales(i8, torch.zeros(2, 2), torch.zeros(2, 2, dtype=torch.float64))
+    with pytest.raises(_lib.NanoserveB200Error):
+        kv_values(i8, torch.zeros(2, 2))
+    with pytest.raises(_lib.NanoserveB200Error):
+        rope_tables(torch.zeros(2, dtype=torch.int64), torch.ones(4))
+    qkv, c = torch.zeros(3, 18 * 64, dtype=torch.bfloat16), torch.zeros(3, 32)
+    with pytest.raises(_lib.NanoserveB200Error):
+        rope_append(qkv, c, c, 14, 2, 64)
+    with pytest.raises(AssertionError):
+        rope_append(qkv, c[:2], c[:2], 14, 2, 64)
+    with pytest.raises(AssertionError):
+        rope_append(qkv.half(), c, c, 14, 2, 64)
+    from nanoserve_b200.kernels.paged_attention import paged_attention_decode, ragged_paged_attention
+    q, t, L = torch.zeros(2, 14, 64, dtype=torch.bfloat16), torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    with pytest.raises(_lib.NanoserveB200Error):
+        paged_attention_decode(q, i8, i8, t, L, 0.125, k_scale=torch.zeros(2, 2), v_scale=torch.zeros(2, 2))
+    bf = torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(AssertionError):
+        ragged_paged_attention(q, bf, bf, t, L, None, 0.125, k_scale=torch.zeros(2, 2))
+
+
+# ------------------------------------------------------------------------------------------------------ frequencies
+def test_frequencies_default_linear_ntk():
+    inv, f = rotary_frequencies(64, 1e6)
+    want = [1e6 ** (-2 * i / 64) for i in range(32)]
+    assert f == 1.0 and inv.dtype == torch.float32 and inv.tolist() == torch.tensor(want, dtype=torch.float64).float().tolist()
+    lin, _ = rotary_frequencies(64, 1e6, {"type": "linear", "factor": 4.0})
+    assert torch.equal(lin, inv / 4)                                            # a power of two: exact
+    ntk, _ = rotary_frequencies(64, 1e4, {"rope_type": "ntk", "factor": 8.0})
+    base, _ = rotary_frequencies(64, 1e4)
+    assert ntk[0] == base[0] and abs(ntk[-1].item() * 8 / base[-1].item() - 1) < 2 ** -22
+
+
+def test_frequencies_yarn():
+    """Fast pairs keep their frequency, slow ones are divided by the factor, the ramp between is monotone."""
+    sc = {"type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768}
+    inv, f = rotary_frequencies(128, 1e6, sc)
+    base, _ = rotary_frequencies(128, 1e6)
+    ratio = inv.double() / base.double()
+    turns = 32768 * base.double() / (2 * math.pi)
+    assert abs(f - (0.1 * math.log(4.0) + 1.0)) < 1e-12
+    assert bool((ratio[turns > 40] == 1.0).all()) and bool(((ratio[turns < 0.8] - 0.25).abs() < 2 ** -23).all())
+    assert bool((ratio[1:] <= ratio[:-1] + 2 ** -22).all())
+    assert rotary_frequencies(128, 1e6, dict(sc, attention_factor=1.5))[1] == 1.5
+
+
+@pytest.mark.parametrize("bad", [dict(rotary_dim=63), dict(rotary_dim=0), dict(theta=0.5), dict(scaling={"type": "linear", "factor": 0.5}),
+                                 dict(scaling={"type": "yarn", "factor": 2.0}), dict(rotary_dim=2, scaling={"type": "ntk", "factor": 2.0})])
+def test_frequencies_refusals(bad):
+    args = dict(rotary_dim=64, theta=1e4, scaling=None)
+    args.update(bad)
+    with pytest.raises(ValueError):
+        rotary_frequencies(**args)
+
+
+def test_unknown_scaling_type():
+    with pytest.raises(NotImplementedError):
+        rotary_frequencies(64, 1e4, {"type": "other", "factor": 2.0})
