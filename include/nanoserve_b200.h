@@ -348,8 +348,8 @@ int ns_kv_values(const void* pool, const float* scale, void* out, int64_t num_bl
 /* ns_ragged_paged_attn over 8-bit pools: the same batch description, q and out bf16 or fp32 (dtype). num_blocks and
  * table_width (entries of a block-table row) bound every access: keys past a table row's width and blocks outside the pool
  * count as absent. A query that sees no key gets zeros; rows of no sequence are left as they were.
- * Sequences of one token need no plan; a call with cu_seqlens and n_tokens > n_seqs takes its prefill tiles from the plan in
- * the workspace (ns_attn_plan with the same seq_lens / cu_seqlens / table_rows). workspace as in ns_ragged_paged_attn; calls
+ * Sequences of one token need no plan; a call with cu_seqlens takes its prefill tiles from the plan in the workspace
+ * (ns_attn_plan with the same seq_lens / cu_seqlens / table_rows). workspace as in ns_ragged_paged_attn; calls
  * that share one must not overlap. Tensor-core kernels: block_size a multiple of 16 (prefill chunks: 16), head_dim 64 / 128,
  * 16-byte aligned pools; everything else runs ns_ragged_paged_attn_q8_simple, which needs no workspace (head_dim <= 256).
  * Replaces, for 8-bit pools: nanoserve/model.py:262-323 _attend and nanoserve/kernels/paged_attention.py:85-105. */

@@ -139,10 +139,15 @@ def dtype_code(dtype) -> int:
     raise NotImplementedError(f"nanoserve_b200 kernels handle bfloat16 and float32, not {dtype}")
 
 
+_KV8_CODES: dict = {}
+
+
 def kv8_code(dtype) -> int | None:
     """The code of an 8-bit KV pool's element type, None for any other dtype."""
-    import torch
-    return {torch.int8: NS_INT8, torch.float8_e4m3fn: NS_E4M3}.get(dtype)
+    if not _KV8_CODES:
+        import torch
+        _KV8_CODES.update({torch.int8: NS_INT8, torch.float8_e4m3fn: NS_E4M3})
+    return _KV8_CODES.get(dtype)
 
 
 def stream_ptr() -> int:
@@ -160,20 +165,27 @@ def require_cuda(*tensors) -> None:
             raise NanoserveB200Error("nanoserve_b200 kernels run on CUDA tensors only (there is no CPU path)")
 
 
-def same_device(*tensors):
-    """The one CUDA device all of the given tensors live on; raises for CPU tensors and for tensors of several devices."""
-    require_cuda(*tensors)
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) != 1:
-        raise NanoserveB200Error(f"tensors of one call live on several devices: {sorted(map(str, devices))}")
-    return devices.pop()
+def same_device(*tensors) -> int:
+    """Index of the one CUDA device all of the given tensors live on; raises for CPU tensors and for tensors of several
+    devices."""
+    dev = -1
+    for t in tensors:
+        if t is not None:
+            d = t.get_device()
+            if d < 0:
+                require_cuda(t)
+            if d != dev:
+                if dev >= 0:
+                    raise NanoserveB200Error(f"tensors of one call live on several devices: cuda:{dev} and cuda:{d}")
+                dev = d
+    return dev
 
 
-def call_on(device, name: str, *args) -> None:
-    """call() with `device` current and its current stream as the last argument (a kernel launch needs both)."""
+def call_on(device: int, name: str, *args) -> None:
+    """call() with CUDA device `device` current (a launch needs that) and its current stream as the last argument."""
     import torch
-    if device.index == torch.cuda.current_device():
-        call(name, *args, stream_ptr())
+    if device == torch._C._cuda_getDevice():
+        call(name, *args, torch._C._cuda_getCurrentRawStream(device))
         return
     with torch.cuda.device(device):
-        call(name, *args, stream_ptr())
+        call(name, *args, torch._C._cuda_getCurrentRawStream(device))

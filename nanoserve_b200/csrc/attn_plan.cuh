@@ -60,6 +60,7 @@ struct WsLayout {
     int64_t counters;       // int32[max_seqs*kMaxKvHeads] arrivals per (decode row, kv head); zero between launches
     int64_t prefill_items;  // int2[max_prefill_items] (batch index, first query token of the tile)
     int64_t partials;       // float[kMaxDecodeCtas*2][n_heads][head_dim+4]
+    int64_t q8_counters;    // int32[max_ctas] arrivals per CTA that begins a split unit (8-bit pools); zero between launches
     int64_t total;
 };
 
@@ -90,6 +91,7 @@ __host__ __device__ inline WsLayout ws_layout(int max_seqs, int max_tokens, int 
     const int64_t max_items = (int64_t)max_tokens / kPrefillTileTokens + max_seqs + 1;
     L.prefill_items = o;  o = align256(o + 8 * max_items);
     L.partials = o;       o = align256(o + 4 * (int64_t)max_ctas * 2 * n_heads * (head_dim + 4));
+    L.q8_counters = o;    o = align256(o + 4 * (int64_t)max_ctas);
     L.total = o;
     return L;
 }

@@ -3,6 +3,8 @@
 
 namespace ns {
 int launch_q8_simple(const Q8Params& p, int dtype, int pool_dtype, cudaStream_t st);
+bool q8_decode_supported(const Q8Params& p, int dtype);
+int launch_q8_decode(const Q8Params& p, int dtype, int pool_dtype, cudaStream_t st);
 }
 
 using namespace ns;
@@ -58,9 +60,25 @@ extern "C" int ns_ragged_paged_attn_q8(const void* q, const void* k_pool, const 
                                        int64_t pool_pos_stride, int64_t pool_head_stride, int64_t scale_block_stride,
                                        int64_t scale_head_stride, float scale, int dtype, int pool_dtype, void* workspace,
                                        int64_t workspace_bytes, int32_t ws_max_seqs, int32_t ws_max_tokens, void* stream) {
-    (void)workspace; (void)workspace_bytes; (void)ws_max_seqs; (void)ws_max_tokens;
-    return ns_ragged_paged_attn_q8_simple(q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, seq_lens, cu_seqlens, out, n_seqs,
-                                          n_tokens, n_heads, n_kv_heads, head_dim, block_size, num_blocks, table_width, table_stride, q_stride,
-                                          out_stride, pool_block_stride, pool_pos_stride, pool_head_stride, scale_block_stride,
-                                          scale_head_stride, scale, dtype, pool_dtype, stream);
+    Q8Params p;
+    int rc = fill_params(p, q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, seq_lens, cu_seqlens, out, n_seqs, n_tokens,
+                         n_heads, n_kv_heads, head_dim, block_size, num_blocks, table_width, table_stride, q_stride, out_stride,
+                         pool_block_stride, pool_pos_stride, pool_head_stride, scale_block_stride, scale_head_stride, scale, dtype, pool_dtype);
+    if (rc != NS_OK || n_seqs == 0 || n_tokens == 0) return rc;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (!q8_decode_supported(p, dtype)) return launch_q8_simple(p, dtype, pool_dtype, st);
+    NS_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0, NS_ERR_INVALID_ARG,
+               "attn_q8: workspace is null or not 256-byte aligned");
+    NS_REQUIRE(n_seqs <= ws_max_seqs && n_tokens <= ws_max_tokens, NS_ERR_WORKSPACE,
+               "attn_q8: batch (%d seqs, %lld tokens) exceeds workspace capacity (%d, %d)", n_seqs, (long long)n_tokens, ws_max_seqs, ws_max_tokens);
+    p.L = ws_layout(ws_max_seqs, ws_max_tokens, n_heads, head_dim);
+    NS_REQUIRE(workspace_bytes >= p.L.total, NS_ERR_WORKSPACE, "attn_q8: workspace of %lld bytes < %lld needed", (long long)workspace_bytes,
+               (long long)p.L.total);
+    p.ws = (uint8_t*)workspace;
+    p.sm_count = device_sm_count();
+    NS_REQUIRE(p.sm_count > 0, NS_ERR_CUDA, "attn_q8: cannot query the SM count");
+    rc = launch_q8_decode(p, dtype, pool_dtype, st);
+    if (rc != NS_OK || cu_seqlens == nullptr || n_tokens < 2) return rc;
+    p.only_prefill = 1;
+    return launch_q8_simple(p, dtype, pool_dtype, st);
 }

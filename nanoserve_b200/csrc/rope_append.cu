@@ -8,8 +8,8 @@ namespace ns {
 // cos/sin[t][i] = factor * cos/sin(pos_t * f_i). The angle of a far position needs more than fp32: at position 10^6 an fp32
 // angle is off by 0.03 rad. The product and its reduction to a fraction of a turn are in fp64 (exact to 2^-53 of the
 // angle), and so are sincospi of the reduced angle and the factor: one rounding to fp32 at the end.
-__global__ void __launch_bounds__(256) rope_tables_kernel(const int64_t* __restrict__ pos, const float* __restrict__ inv_freq,
-                                                          double factor, float* __restrict__ cos_out, float* __restrict__ sin_out,
+__global__ void __launch_bounds__(256) rope_tables_kernel(const int64_t* pos, const float* inv_freq,
+                                                          double factor, float* cos_out, float* sin_out,
                                                           int64_t total, int half) {
     constexpr double kInvPi = 0.31830988618379067154;
     pdl_launch_dependents();
@@ -336,7 +336,7 @@ template <typename T, int V> static int dispatch_pool(const RopeAppendParams& p,
 
 // ------------------------------------------------------------------------------------------------ values of an 8-bit pool
 template <typename T, typename KV, int V>
-__global__ void __launch_bounds__(256) kv_values_kernel(const uint8_t* __restrict__ pool, const float* __restrict__ scale, T* __restrict__ out,
+__global__ void __launch_bounds__(256) kv_values_kernel(const uint8_t* pool, const float* scale, T* out,
                                                         int64_t rows, int block_size, int n_kv_heads, int head_dim, int64_t blk_stride,
                                                         int64_t pos_stride, int64_t head_stride, int64_t sc_blk, int64_t sc_head) {
     pdl_launch_dependents();

@@ -14,6 +14,7 @@ from __future__ import annotations
 import torch
 
 from nanoserve_b200 import _lib
+from nanoserve_b200.kernels.rotary import check_kv8_scales
 
 
 class AttnWorkspace:
@@ -80,40 +81,55 @@ def _check_pool(q, k_pool, v_pool):
 def _attend_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, seq_lens, cu_seqlens, scale, n_seqs, workspace, planned, out,
                simple) -> torch.Tensor:
     """Ragged attention over an int8 / float8_e4m3fn pool (ns_ragged_paged_attn_q8)."""
-    from nanoserve_b200.kernels.rotary import check_kv8_scales
-    dev = _lib.same_device(q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, seq_lens, cu_seqlens, out)
-    assert k_pool.dim() == 4 and q.dim() == 3 and v_pool.shape == k_pool.shape
-    assert q.stride(-1) == 1 and k_pool.stride(-1) == 1 and v_pool.stride() == k_pool.stride() and v_pool.dtype == k_pool.dtype
-    assert q.stride(1) == q.shape[2] or q.shape[1] == 1, "query heads must be adjacent (head stride == head_dim)"
-    check_kv8_scales(k_pool, k_scale, v_scale)
-    assert block_tables.dtype == torch.int32 and block_tables.dim() == 2 and (block_tables.stride(1) == 1 or block_tables.shape[1] <= 1)
-    assert seq_lens.dtype == torch.int32 and seq_lens.is_contiguous() and seq_lens.shape[0] >= n_seqs
-    assert cu_seqlens is None or (cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous() and cu_seqlens.shape[0] > n_seqs)
-    assert table_rows is None or (table_rows.dtype == torch.int32 and table_rows.is_contiguous() and table_rows.shape[0] >= n_seqs)
-    assert table_rows is not None or block_tables.shape[0] >= n_seqs, "block_tables has a row per sequence"
     N, n_heads, head_dim = q.shape
     num_blocks, block_size, n_kv_heads, hd = k_pool.shape
-    assert hd == head_dim and (cu_seqlens is not None or N == n_seqs)
-    if out is None:
-        out = torch.empty(N, n_heads, head_dim, device=dev, dtype=q.dtype)
+    rows, width = block_tables.shape
+    qs, ps, ts, i32 = q.stride(), k_pool.stride(), block_tables.stride(), torch.int32
+    if v_scale is None:
+        raise ValueError(f"a {k_pool.dtype} pool needs k_scale and v_scale (fp32 [num_blocks, n_kv_heads])")
+    ss = check_kv8_scales(k_pool, k_scale, v_scale)
+    assert hd == head_dim and v_pool.shape == k_pool.shape and v_pool.stride() == ps and v_pool.dtype is k_pool.dtype and ps[3] == 1
+    assert qs[2] == 1 and (qs[1] == head_dim or n_heads == 1), "query heads must be adjacent (head stride == head_dim)"
+    assert block_tables.dtype is i32 and (ts[1] == 1 or width <= 1)
+    assert seq_lens.dtype is i32 and seq_lens.is_contiguous() and seq_lens.shape[0] >= n_seqs
+    if cu_seqlens is None:
+        assert N == n_seqs, "without cu_seqlens every sequence has one token"
     else:
-        assert out.shape == q.shape and out.stride(-1) == 1 and (out.stride(1) == head_dim or n_heads == 1) and out.dtype == q.dtype
+        assert cu_seqlens.dtype is i32 and cu_seqlens.is_contiguous() and cu_seqlens.shape[0] > n_seqs
+    if table_rows is None:
+        assert rows >= n_seqs, "block_tables has a row per sequence"
+    else:
+        assert table_rows.dtype is i32 and table_rows.is_contiguous() and table_rows.shape[0] >= n_seqs
+    dev = _lib.same_device(q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, seq_lens, cu_seqlens, out)
+    if out is None:
+        out = torch.empty((N, n_heads, head_dim), device=q.device, dtype=q.dtype)
+    else:
+        assert out.shape == q.shape and out.stride(2) == 1 and (out.stride(1) == head_dim or n_heads == 1) and out.dtype is q.dtype
     common = (q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
-              _lib.ptr(table_rows), seq_lens.data_ptr(), _lib.ptr(cu_seqlens), out.data_ptr(), n_seqs, N, n_heads, n_kv_heads, head_dim,
-              block_size, num_blocks, block_tables.shape[1], block_tables.stride(0), q.stride(0), out.stride(0), *k_pool.stride()[:3],
-              *k_scale.stride(), float(scale), _lib.dtype_code(q.dtype), _lib.kv8_code(k_pool.dtype))
+              None if table_rows is None else table_rows.data_ptr(), seq_lens.data_ptr(),
+              None if cu_seqlens is None else cu_seqlens.data_ptr(), out.data_ptr(), n_seqs, N, n_heads, n_kv_heads, head_dim, block_size,
+              num_blocks, width, ts[0], qs[0], out.stride(0), *ps[:3], *ss, scale, _lib.dtype_code(q.dtype), _lib.kv8_code(k_pool.dtype))
     if simple:
         _lib.call_on(dev, "ns_ragged_paged_attn_q8_simple", *common)
         return out
-    with torch.cuda.device(dev):
-        ws = workspace or _workspace_q8(dev, n_seqs, N, n_heads, head_dim)
-        mixed = cu_seqlens is not None and N > n_seqs
-        if mixed and not planned:
-            ws.plan(seq_lens, cu_seqlens, n_seqs, block_size, table_rows)
-        _lib.call("ns_ragged_paged_attn_q8", *common, ws.buf.data_ptr(), ws.nbytes, ws.max_seqs, ws.max_tokens, _lib.stream_ptr())
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            _launch_q8(common, dev, q.device, workspace, planned, seq_lens, cu_seqlens, table_rows)
+    else:
+        _launch_q8(common, dev, q.device, workspace, planned, seq_lens, cu_seqlens, table_rows)
+    return out
+
+
+def _launch_q8(common, dev, device, ws, planned, seq_lens, cu_seqlens, table_rows) -> None:
+    n_seqs, N, n_heads, _, head_dim, block_size = common[10:16]
+    if ws is None:
+        ws = _workspace_q8(device, n_seqs, N, n_heads, head_dim)
+    mixed = cu_seqlens is not None and N > 1
+    if mixed and not planned:
+        ws.plan(seq_lens, cu_seqlens, n_seqs, block_size, table_rows)
+    _lib.call_on(dev, "ns_ragged_paged_attn_q8", *common, ws.buf.data_ptr(), ws.nbytes, ws.max_seqs, ws.max_tokens)
     if mixed:
         _lib.note_launches(1)          # the prefill-tile kernel is launched next to the decode kernel
-    return out
 
 
 def paged_attention_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Tensor,

@@ -64,47 +64,52 @@ def rotary_frequencies(rotary_dim: int, theta: float, scaling: dict | None = Non
 def rope_tables(positions: torch.Tensor, inv_freq: torch.Tensor, factor: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
     """factor * cos / sin of positions[t] * inv_freq[i], fp32 [T, len(inv_freq)] each (angles in fp64, rounded once)."""
     dev = _lib.same_device(positions, inv_freq)
-    assert positions.dtype == torch.int64 and positions.dim() == 1 and positions.is_contiguous()
-    assert inv_freq.dtype == torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous()
+    assert positions.dtype is torch.int64 and positions.dim() == 1 and positions.is_contiguous()
+    assert inv_freq.dtype is torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous()
     t, half = positions.shape[0], inv_freq.shape[0]
-    cos = torch.empty(t, half, device=dev, dtype=torch.float32)
+    cos = torch.empty((t, half), device=positions.device, dtype=torch.float32)
     sin = torch.empty_like(cos)
     _lib.call_on(dev, "ns_rope_tables", positions.data_ptr(), inv_freq.data_ptr(), float(factor), cos.data_ptr(), sin.data_ptr(), t, half)
     return cos, sin
 
 
-def check_kv8_scales(pool: torch.Tensor, *scales: torch.Tensor | None) -> None:
-    """An 8-bit pool's scales: fp32 [num_blocks, n_kv_heads], one for K and one for V, of equal strides."""
-    for s in scales:
-        if s is None:
-            raise ValueError(f"a {pool.dtype} pool needs k_scale and v_scale (fp32 [num_blocks, n_kv_heads])")
-        assert s.dtype == torch.float32 and s.shape == (pool.shape[0], pool.shape[2]), "scales are fp32 [num_blocks, n_kv_heads]"
-        assert s.stride() == scales[0].stride(), "k_scale and v_scale must have equal strides"
+def check_kv8_scales(pool: torch.Tensor, scale: torch.Tensor | None, other: torch.Tensor | None = None) -> tuple[int, int]:
+    """An 8-bit pool's scales: fp32 [num_blocks, n_kv_heads], one for K and one for V, of equal strides; returns the strides."""
+    if scale is None:
+        raise ValueError(f"a {pool.dtype} pool needs k_scale and v_scale (fp32 [num_blocks, n_kv_heads])")
+    shape, strides = (pool.shape[0], pool.shape[2]), scale.stride()
+    assert scale.dtype is torch.float32 and scale.shape == shape, "scales are fp32 [num_blocks, n_kv_heads]"
+    if other is not None:
+        assert other.dtype is torch.float32 and other.shape == shape, "scales are fp32 [num_blocks, n_kv_heads]"
+        assert other.stride() == strides, "k_scale and v_scale must have equal strides"
+    return strides
 
 
-def _append(q, k, v, cos, sin, rot, interleaved, q_out, k_out, v_out, k_cache, v_cache, slots, k_scale, v_scale, n, n_heads, n_kv_heads,
-            head_dim, dtype) -> None:
-    dev = _lib.same_device(q, k, v, cos, sin, k_cache, v_cache, slots, k_scale, v_scale)
-    pool_strides, n_slots, block_size, pool_code, sc = (0, 0, 0), 0, 1, _lib.dtype_code(dtype), (0, 0)
-    if k_cache is not None:
-        if v_cache is None or slots is None:
-            raise ValueError("a cache layer needs k_cache, v_cache and slots")
-        assert k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.shape[2:] == (n_kv_heads, head_dim)
-        assert k_cache.stride() == v_cache.stride() and k_cache.stride(3) == 1 and k_cache.dtype == v_cache.dtype
-        assert slots.dtype == torch.int64 and slots.is_contiguous() and slots.shape[0] >= n
-        pool_strides, block_size = k_cache.stride()[:3], k_cache.shape[1]
-        n_slots = k_cache.shape[0] * block_size
-        code = _lib.kv8_code(k_cache.dtype)
-        if code is None:
-            assert k_cache.dtype == dtype, "the pool holds the activations' dtype, int8 or float8_e4m3fn"
-            assert k_scale is None and v_scale is None, "scales belong to 8-bit pools"
-        else:
-            check_kv8_scales(k_cache, k_scale, v_scale)
-            pool_code, sc = code, k_scale.stride()
-    _lib.call_on(dev, "ns_rope_append", _lib.ptr(q), k.data_ptr(), v.data_ptr(), 0 if q is None else q.stride(0), k.stride(0), v.stride(0),
-                 _lib.ptr(cos), _lib.ptr(sin), rot, int(bool(interleaved)), _lib.ptr(q_out), _lib.ptr(k_out), _lib.ptr(v_out),
-                 _lib.ptr(k_cache), _lib.ptr(v_cache), _lib.ptr(k_scale), _lib.ptr(v_scale), _lib.ptr(slots), n, n_slots, n_heads, n_kv_heads,
-                 head_dim, block_size, *pool_strides, *sc, _lib.dtype_code(dtype), pool_code)
+_NO_POOL = (None, None, None, None, None)
+
+
+def _pool_args(dtype, n, n_kv_heads, head_dim, k_cache, v_cache, slots, k_scale, v_scale):
+    """Checked cache layer of an append: (pointers, sizes and strides, pool dtype code)."""
+    if k_cache is None:
+        return _NO_POOL, 0, 1, (0, 0, 0, 0, 0), _lib.dtype_code(dtype)
+    if v_cache is None or slots is None:
+        raise ValueError("a cache layer needs k_cache, v_cache and slots")
+    shape, strides = k_cache.shape, k_cache.stride()
+    assert len(shape) == 4 and v_cache.shape == shape and shape[2] == n_kv_heads and shape[3] == head_dim, "cache layer shape"
+    assert v_cache.stride() == strides and strides[3] == 1 and v_cache.dtype is k_cache.dtype
+    assert slots.dtype is torch.int64 and slots.is_contiguous() and slots.shape[0] >= n
+    code, sc = _lib.kv8_code(k_cache.dtype), (0, 0)
+    if code is None:
+        assert k_cache.dtype is dtype, "the pool holds the activations' dtype, int8 or float8_e4m3fn"
+        assert k_scale is None and v_scale is None, "scales belong to 8-bit pools"
+        code = _lib.dtype_code(dtype)
+        scales = (None, None)
+    else:
+        if v_scale is None:
+            raise ValueError(f"a {k_cache.dtype} pool needs k_scale and v_scale (fp32 [num_blocks, n_kv_heads])")
+        sc = check_kv8_scales(k_cache, k_scale, v_scale)
+        scales = (k_scale.data_ptr(), v_scale.data_ptr())
+    return ((k_cache.data_ptr(), v_cache.data_ptr(), *scales, slots.data_ptr()), shape[0] * shape[1], shape[1], strides[:3] + sc, code)
 
 
 def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int,
@@ -117,32 +122,40 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_heads
     (k_cache / v_cache [blocks, block_size, n_kv_heads, hd], int64 slots [N]) K and V are stored there; a negative slot stores
     nothing. An int8 or float8_e4m3fn layer needs k_scale / v_scale fp32 [blocks, n_kv_heads], which the call keeps up (see
     ns_rope_append in the header for the format)."""
-    assert qkv.dim() == 2 and qkv.stride(1) == 1 and qkv.shape[1] == (n_heads + 2 * n_kv_heads) * head_dim
-    if qkv.dtype not in (torch.bfloat16, torch.float32):
+    n, width = qkv.shape
+    row, one = qkv.stride()
+    dtype = qkv.dtype
+    assert width == (n_heads + 2 * n_kv_heads) * head_dim and (one == 1 or width == 1)
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise AssertionError("rope_append handles bfloat16 and float32")
-    n, rot = qkv.shape[0], 2 * cos.shape[1]
-    assert cos.dtype == torch.float32 and sin.dtype == torch.float32 and cos.shape == sin.shape == (n, rot // 2)
-    assert cos.is_contiguous() and sin.is_contiguous() and rot <= head_dim
-    dev, dtype = qkv.device, qkv.dtype
-    _lib.require_cuda(qkv)
-    q = torch.empty(n, n_heads, head_dim, device=dev, dtype=dtype)
-    k = torch.empty(n, n_kv_heads, head_dim, device=dev, dtype=dtype) if dense_kv else None
+    half = cos.shape[1]
+    assert cos.dtype is torch.float32 and sin.dtype is torch.float32 and cos.shape == (n, half) and sin.shape == (n, half)
+    assert cos.is_contiguous() and sin.is_contiguous() and 2 * half <= head_dim
+    pool, n_slots, block_size, strides, code = _pool_args(dtype, n, n_kv_heads, head_dim, k_cache, v_cache, slots, k_scale, v_scale)
+    dev = _lib.same_device(qkv, cos, sin, k_cache, v_cache, slots, k_scale, v_scale)
+    q = torch.empty((n, n_heads, head_dim), device=qkv.device, dtype=dtype)
+    k = torch.empty((n, n_kv_heads, head_dim), device=qkv.device, dtype=dtype) if dense_kv else None
     v = torch.empty_like(k) if dense_kv else None
-    nq, nk = n_heads * head_dim, n_kv_heads * head_dim
-    _append(qkv, qkv[:, nq:nq + nk], qkv[:, nq + nk:], cos, sin, rot, interleaved, q, k, v, k_cache, v_cache, slots, k_scale, v_scale, n,
-            n_heads, n_kv_heads, head_dim, dtype)
+    base, size = qkv.data_ptr(), 2 if dtype is torch.bfloat16 else 4
+    base_k = base + n_heads * head_dim * size
+    _lib.call_on(dev, "ns_rope_append", base, base_k, base_k + n_kv_heads * head_dim * size, row, row, row, cos.data_ptr(), sin.data_ptr(),
+                 2 * half, 1 if interleaved else 0, q.data_ptr(), None if k is None else k.data_ptr(), None if v is None else v.data_ptr(),
+                 *pool, n, n_slots, n_heads, n_kv_heads, head_dim, block_size, *strides, _lib.dtype_code(dtype), code)
     return q, k, v
 
 
 def kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
               k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> None:
     """rope_append without a rotation: store k_new / v_new [N, n_kv_heads, hd] (rotated already) at their slots."""
-    assert k_new.dim() == 3 and v_new.shape == k_new.shape and k_new.dtype == v_new.dtype
+    assert k_new.dim() == 3 and v_new.shape == k_new.shape and k_new.dtype is v_new.dtype
     for t in (k_new, v_new):
         assert t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == t.shape[2]), "heads of a token must be adjacent"
     n, n_kv_heads, head_dim = k_new.shape
-    _append(None, k_new, v_new, None, None, 0, False, None, None, None, k_cache, v_cache, slots, k_scale, v_scale, n, 0, n_kv_heads, head_dim,
-            k_new.dtype)
+    dtype = k_new.dtype
+    pool, n_slots, block_size, strides, code = _pool_args(dtype, n, n_kv_heads, head_dim, k_cache, v_cache, slots, k_scale, v_scale)
+    dev = _lib.same_device(k_new, v_new, k_cache, v_cache, slots, k_scale, v_scale)
+    _lib.call_on(dev, "ns_rope_append", None, k_new.data_ptr(), v_new.data_ptr(), 0, k_new.stride(0), v_new.stride(0), None, None, 0, 0, None,
+                 None, None, *pool, n, n_slots, 0, n_kv_heads, head_dim, block_size, *strides, _lib.dtype_code(dtype), code)
 
 
 def kv_values(pool: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -152,8 +165,8 @@ def kv_values(pool: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torc
     if code is None:
         raise NotImplementedError(f"kv_values reads int8 and float8_e4m3fn pools, not {pool.dtype}")
     assert pool.dim() == 4 and pool.stride(3) == 1
-    check_kv8_scales(pool, scale)
-    out = torch.empty(pool.shape, device=dev, dtype=dtype)
-    _lib.call_on(dev, "ns_kv_values", pool.data_ptr(), scale.data_ptr(), out.data_ptr(), *pool.shape, *pool.stride()[:3], *scale.stride(),
+    strides = check_kv8_scales(pool, scale)
+    out = torch.empty(pool.shape, device=pool.device, dtype=dtype)
+    _lib.call_on(dev, "ns_kv_values", pool.data_ptr(), scale.data_ptr(), out.data_ptr(), *pool.shape, *pool.stride()[:3], *strides,
                  _lib.dtype_code(dtype), code)
     return out
