@@ -5,6 +5,8 @@ namespace ns {
 int launch_q8_simple(const Q8Params& p, int dtype, int pool_dtype, cudaStream_t st);
 bool q8_decode_supported(const Q8Params& p, int dtype);
 int launch_q8_decode(const Q8Params& p, int dtype, int pool_dtype, cudaStream_t st);
+bool q8_prefill_supported(const Q8Params& p, int dtype);
+int launch_q8_prefill(const Q8Params& p, int pool_dtype, int max_items, cudaStream_t st);
 }
 
 using namespace ns;
@@ -77,8 +79,18 @@ extern "C" int ns_ragged_paged_attn_q8(const void* q, const void* k_pool, const 
     p.ws = (uint8_t*)workspace;
     p.sm_count = device_sm_count();
     NS_REQUIRE(p.sm_count > 0, NS_ERR_CUDA, "attn_q8: cannot query the SM count");
+    const bool prefill = cu_seqlens != nullptr && n_tokens > 1, tc = prefill && q8_prefill_supported(p, dtype);
+    p.overlap_prefill = tc ? 1 : 0;
     rc = launch_q8_decode(p, dtype, pool_dtype, st);
-    if (rc != NS_OK || cu_seqlens == nullptr || n_tokens < 2) return rc;
+    if (rc != NS_OK || !prefill) return rc;
+    rc = NS_ERR_UNSUPPORTED;
+    if (tc) {
+        // upper bound on prefill tiles from sizes the host knows (graph-safe)
+        int64_t max_items = n_tokens / kPrefillTileTokens + n_seqs;
+        const int64_t cap = (int64_t)ws_max_tokens / kPrefillTileTokens + ws_max_seqs + 1;
+        rc = launch_q8_prefill(p, pool_dtype, (int)(max_items < cap ? max_items : cap), st);
+    }
+    if (rc != NS_ERR_UNSUPPORTED) return rc;
     p.only_prefill = 1;
     return launch_q8_simple(p, dtype, pool_dtype, st);
 }

@@ -31,4 +31,23 @@ __device__ __forceinline__ int q8_len(const Q8Params& p, int s) {
     return len < 0 ? 0 : (len > cap ? (int)cap : len);
 }
 
+namespace q8 {
+
+// The four codes of a word as f16: bytes 0 and 1, bytes 2 and 3.
+template <typename KV> __device__ __forceinline__ void expand(uint32_t w, uint32_t& lo, uint32_t& hi);
+template <> __device__ __forceinline__ void expand<KvInt8>(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    const uint32_t u = w ^ 0x80808080u;                     // 0 .. 255: u + 1024 is the f16 0x6400 | u
+    const uint32_t bias = 0x64806480u;                      // 1024 + 128
+    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+    __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<const __half2*>(&bias));
+    __half2 y = __hsub2(*reinterpret_cast<__half2*>(&b), *reinterpret_cast<const __half2*>(&bias));
+    lo = *reinterpret_cast<uint32_t*>(&x);
+    hi = *reinterpret_cast<uint32_t*>(&y);
+}
+template <> __device__ __forceinline__ void expand<KvE4m3>(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+
+}  // namespace q8
+
 }  // namespace ns

@@ -54,21 +54,6 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// The four codes of a word as f16: bytes 0 and 1, bytes 2 and 3.
-template <typename KV> __device__ __forceinline__ void expand(uint32_t w, uint32_t& lo, uint32_t& hi);
-template <> __device__ __forceinline__ void expand<KvInt8>(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    const uint32_t u = w ^ 0x80808080u;                     // 0 .. 255: u + 1024 is the f16 0x6400 | u
-    const uint32_t bias = 0x64806480u;                      // 1024 + 128
-    uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-    __half2 x = __hsub2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<const __half2*>(&bias));
-    __half2 y = __hsub2(*reinterpret_cast<__half2*>(&b), *reinterpret_cast<const __half2*>(&bias));
-    lo = *reinterpret_cast<uint32_t*>(&x);
-    hi = *reinterpret_cast<uint32_t*>(&y);
-}
-template <> __device__ __forceinline__ void expand<KvE4m3>(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    asm("{.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;}" : "=r"(lo), "=r"(hi) : "r"(w));
-}
-
 // One tile of a unit as a lane holds it.
 template <int HD> struct Tile {
     static constexpr int KW = HD / 64, VW = HD / 32;        // 16-byte pieces per K row, words per V row
@@ -101,8 +86,11 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
     __shared__ int join_of[2];             // chain index of a unit this CTA is the last to deliver, by piece: head, tail
     __shared__ float join_w[8][2];         // not used by the main loop: per head {max, 1 / sum} of a join
 
-    pdl_launch_dependents();
+    // A mixed call's prefill kernel, launched next, does not wait for this one (it reads the same inputs and writes other rows):
+    // it may start only once the inputs exist, that is after this kernel's own wait.
+    if (!p.overlap_prefill) pdl_launch_dependents();
     pdl_wait();
+    if (p.overlap_prefill) pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int G = gridDim.x, cta = blockIdx.x;
     const int sub = (p.group + 7) >> 3, VH = p.n_kv_heads * sub;

@@ -1,0 +1,531 @@
+// Prefill-chunk attention over 8-bit pools on the 5th-generation tensor cores (tcgen05), accumulators in tensor memory.
+//
+// Work item = (sequence, 16 query tokens, eight query heads of a KV head), from the plan: 128 rows of one UMMA tile (row r =
+// token r / 8, head r % 8) against key tiles of 64.
+//   S[128 x 64]  = Q[128 x HD] . K_tile[64 x HD]^T      f16 operands, fp32 accumulators
+//   O[128 x HD] += P[128 x 64] . V_tile[64 x HD]
+// The codes become f16 on their way into shared memory (exact for int8 and e4m3, so K and V are never rounded): three converting
+// warps read 16-byte pieces of the pool's rows, one tile ahead, and store them in the swizzled layout the UMMA descriptors
+// expect. Rows past the sequence and blocks outside the pool become zeros there. Scales stay out of the operands:
+//   x = s * (scale log2 e * 2^e_q * sk) + log2 sv,   P = 2^(x - m),   l += sum(P) / sv   per block of 16 keys
+// (Q is scaled by a power of two per row, P is relative to the row's largest contribution; see attn_q8_decode.cu.)
+// Two warpgroups, 256 threads, two CTAs per SM:
+//   warps 0-3  one softmax thread per row. 176 registers a thread
+//   warp 4     lane 0 issues every tcgen05.mma
+//   warps 5-7  convert K and V tiles. 80 registers a thread: (176 + 80) * 128 = 128 * 256, what the block was launched with
+// Pipeline over the key tiles as in the 16-bit kernel: S runs two tiles ahead, P double buffered, O stays in tensor memory and
+// is rescaled only when a row's reference has to move. Every mbarrier wait is bounded: on expiry the CTA counts an error in the
+// plan header (ns_collect_status), skips its stores, frees its tensor memory and returns.
+#include "attn_q8.cuh"
+#include "tc_common.cuh"
+
+namespace ns {
+
+namespace q8p {
+
+using namespace tc;
+
+constexpr int kRows = 128, kKeys = 64, kThreads = 256, kConv = 96;     // softmax rows, keys per tile, threads, converting threads
+constexpr int kConvWarps = kConv / 32;
+constexpr int kRegsSoftmax = 176, kRegsOther = 80;
+constexpr int kScaleRing = 8;       // a converter is at most five tiles ahead of the slowest softmax thread
+template <int HD> struct Depth {
+    static constexpr int K = HD == 64 ? 3 : 1, V = HD == 64 ? 4 : 2, P = 2;
+    // mbarriers: S0 S1 PV0 PV1 | K full | V full | K free | V free | P0 P1 ready | scales of a tile
+    static constexpr int BarS = 0, BarPV = 2, BarKFull = 4, BarVFull = BarKFull + K, BarKFree = BarVFull + V, BarVFree = BarKFree + K,
+                         BarPReady = BarVFree + V, BarScale = BarPReady + 2, Bars = BarScale + kScaleRing;
+};
+constexpr int kTailBytes = 832;     // mbarriers, two words, the scale ring [8][3][4], the NaN-key ring [8][3]
+constexpr float kLazy = 8.f;
+constexpr float kMinScale = 7.8886090522101181e-31f;    // 2^-100
+
+// Instruction descriptor for kind::f16: fp32 accumulate, f16 A and B, M = 128, N = n.
+__host__ __device__ constexpr uint32_t instr_desc(bool b_mn_major, int n) {
+    return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void st_shared16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// Named barrier 1: the softmax threads and the issuing warp meet once, when Q is in place.
+__device__ __forceinline__ void q_ready_barrier() { asm volatile("bar.sync 1, %0;" ::"r"(kRows + 32) : "memory"); }
+
+}  // namespace q8p
+
+template <int HD, typename KV>
+__global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Params p) {
+    using namespace q8p;
+    using D = Depth<HD>;
+    constexpr int kStagesK = D::K, kStagesV = D::V, kBufsP = D::P;
+    constexpr int ATOMS = HD / 64;
+    constexpr int Q_BYTES = kRows * 128 * ATOMS, KV_BYTES = kKeys * 128 * ATOMS, P_BYTES = kRows * 128;
+    constexpr uint32_t COL_S = 0, COL_O = 2 * kKeys, TMEM_COLS = 256;
+    static_assert(D::Bars * 8 + 16 + kScaleRing * (48 + 8 * kConvWarps) <= kTailBytes, "the tail holds the barriers, two words and the rings");
+    // V codes that are NaN (e4m3 only): 0 x NaN would reach rows that must not see the key, so the operand gets 0 there and the
+    // key goes on a list: the score of a row that does see it becomes NaN (its whole output row then is).
+    constexpr bool kNanCodes = std::is_same<KV, KvE4m3>::value;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+
+    const PlanHeader* hdr = reinterpret_cast<const PlanHeader*>(p.ws + p.L.header);
+    const int sub = (p.group + 7) >> 3;
+    int item_idx, vh;
+    {
+        // the plan lists the items heaviest first; where they are one wave of two CTAs per SM, an SM's second CTA is light
+        const int n_items = hdr->n_prefill_items, n_kv = (int)gridDim.y;
+        const int units = n_items * n_kv, S = p.sm_count;
+        const int lin = (int)(blockIdx.x + gridDim.x * blockIdx.y);
+        int r = lin;
+        if (S > 0 && units > S && units <= 2 * S && lin >= S) r = units - 1 - (lin - S);
+        item_idx = lin < units ? r / n_kv : n_items;
+        vh = r % n_kv;
+        if (item_idx >= n_items) {
+            pdl_wait();                           // the grid must not complete before the decode kernel it overlaps
+            return;
+        }
+    }
+    const int2 item = reinterpret_cast<const int2*>(p.ws + p.L.prefill_items)[item_idx];
+    const int s = item.x, q_start = item.y;
+    if (s < 0 || s >= p.n_seqs) {                 // a plan of another batch
+        pdl_wait();
+        return;
+    }
+    const int g = vh / sub, h0 = (vh - g * sub) * 8, heads = min(8, p.group - h0);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int q0 = p.cu_seqlens[s];
+    const int T = p.cu_seqlens[s + 1] - q0;
+    const int len = q8_len(p, s);
+    const int ctx = len - T;
+    const int32_t* table = p.block_tables + (int64_t)(p.table_rows ? p.table_rows[s] : s) * p.table_stride;
+    const int kv_end = min(len, ctx + q_start + kPrefillTileTokens);
+    const int n_tiles = kv_end > 0 ? (kv_end + kKeys - 1) / kKeys : 0;
+
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    const uint32_t sQ = base, sK = sQ + Q_BYTES, sV = sK + kStagesK * KV_BYTES, sP = sV + kStagesV * KV_BYTES;
+    const uint32_t bar0 = sP + kBufsP * P_BYTES;
+    auto bar = [&](int i) -> uint32_t { return bar0 + 8u * (uint32_t)i; };
+    volatile uint32_t* tail_words = reinterpret_cast<volatile uint32_t*>(smem_raw + (bar0 - raw) + D::Bars * 8);
+    volatile uint32_t& tmem_slot = tail_words[0];
+    volatile uint32_t& abort_flag = tail_words[1];
+    float* const scale_ring = reinterpret_cast<float*>(smem_raw + (bar0 - raw) + ((D::Bars * 8 + 8 + 15) & ~15));   // [ring][sk | lv | 1/sv][4]
+    uint64_t* const nan_ring = reinterpret_cast<uint64_t*>(scale_ring + kScaleRing * 12);       // [ring][converting warp], bit = key of the tile
+    uint32_t dyn_bytes;
+    asm volatile("mov.u32 %0, %%dynamic_smem_size;" : "=r"(dyn_bytes));
+    if (bar0 - raw + kTailBytes > dyn_bytes) {    // the array did not start where the launcher's size assumes: never expected
+        if (tid == 0) atomicAdd(&reinterpret_cast<PlanHeader*>(p.ws + p.L.header)->errors, 1);
+        pdl_wait();
+        return;
+    }
+    if (tid == 0) {
+#pragma unroll
+        for (int i = 0; i < D::Bars; ++i) {
+            const uint32_t count = i >= D::BarScale ? (kNanCodes ? kConvWarps : 1) : i >= D::BarPReady ? kRows : (i >= D::BarKFull && i < D::BarKFree) ? kConv : 1;
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar(i)), "r"(count) : "memory");
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        abort_flag = 0;
+    }
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar0 + D::Bars * 8), "r"(TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = tmem_slot;
+    bool ok = true;
+
+    if (warp >= 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+        if (warp == 4) {
+            q_ready_barrier();
+            if (lane == 0) {
+                constexpr uint32_t idesc_s = instr_desc(false, kKeys), idesc_pv = instr_desc(true, HD);
+                const uint64_t dQ = smem_desc(sQ, 16, 1024), dK = smem_desc(sK, 16, 1024), dP = smem_desc(sP, 16, 1024);
+                const uint64_t dV = smem_desc(sV, kKeys * 128, 1024);
+                auto issue_s = [&](int kt) {
+                    const int sk = kt % kStagesK;
+                    if (!mbar_wait_or_abort(bar(D::BarKFull + sk), (uint32_t)((kt / kStagesK) & 1), tail_words + 1)) { ok = false; return; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t k0 = dK + (uint64_t)((sk * KV_BYTES) >> 4);
+                    const uint32_t d = tmem + COL_S + (uint32_t)((kt & 1) * kKeys);
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; ++kk) {
+                        const uint32_t a_off = (uint32_t)(((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4);
+                        const uint32_t b_off = (uint32_t)(((kk >> 2) * (kKeys * 128) + (kk & 3) * 32) >> 4);
+                        tc::mma_f16(d, dQ + a_off, k0 + b_off, idesc_s, kk > 0);
+                    }
+                    mma_commit(bar(D::BarS + (kt & 1)));
+                    mma_commit(bar(D::BarKFree + sk));
+                };
+                auto issue_pv = [&](int kt) {
+                    const int sv = kt % kStagesV;
+                    if (!mbar_wait_or_abort(bar(D::BarVFull + sv), (uint32_t)((kt / kStagesV) & 1), tail_words + 1)) { ok = false; return; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint64_t p0 = dP + (uint64_t)(((kt % kBufsP) * P_BYTES) >> 4);
+                    const uint64_t v0 = dV + (uint64_t)((sv * KV_BYTES) >> 4);
+#pragma unroll
+                    for (int kk = 0; kk < kKeys / 16; ++kk)
+                        tc::mma_f16(tmem + COL_O, p0 + (uint32_t)((kk * 32) >> 4), v0 + (uint32_t)((kk * 2048) >> 4), idesc_pv,
+                                    (kt > 0 || kk > 0) ? 1u : 0u);
+                    mma_commit(bar(D::BarPV + (kt & 1)));
+                    mma_commit(bar(D::BarVFree + sv));
+                };
+                if (n_tiles > 0) issue_s(0);
+                if (n_tiles > 1) issue_s(1);
+                for (int kt = 0; kt < n_tiles && ok; ++kt) {
+                    if (!mbar_wait_or_abort(bar(D::BarPReady + (kt & 1)), (uint32_t)((kt >> 1) & 1), tail_words + 1)) { ok = false; break; }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    issue_pv(kt);
+                    if (kt + 2 < n_tiles) issue_s(kt + 2);
+                }
+                if (!ok) abort_flag = 1;
+            }
+        } else {
+            // ---- converting warps. An item is 32 consecutive 16-code pieces of a tile: ROWS rows of it.
+            constexpr int CPR = HD / 16, ROWS = 32 / CPR, ITEMS = kKeys / ROWS, MINE = (ITEMS + kConvWarps - 1) / kConvWarps;
+            const int cw = warp - 5, row_in = lane / CPR, piece = lane % CPR;
+            const uint8_t* kb = p.k_pool + g * p.head_stride + piece * 16;
+            const uint8_t* vb = p.v_pool + g * p.head_stride + piece * 16;
+            uint4 kr[MINE], vr[MINE];
+            auto fetch_ids = [&](int kt) -> int {              // lane b < 4: block of keys 16 b .. of the tile, -1: absent
+                const int key = kt * kKeys + 16 * (lane & 3);
+                if (kt >= n_tiles || key >= kv_end) return -1;
+                const int id = table[key / p.block_size];
+                return (unsigned)id < (unsigned)p.num_blocks ? id : -1;
+            };
+            auto item_at = [&](int n, bool v) -> int { const int i = (v ? kConvWarps - 1 - cw : cw) + kConvWarps * n; return i < ITEMS ? i : -1; };
+            auto load_item = [&](int kt, int i, int ids, const uint8_t* pool) -> uint4 {
+                const int row = i * ROWS + row_in, key = kt * kKeys + row;
+                const int id = __shfl_sync(0xffffffffu, ids, row >> 4);
+                if (id < 0 || key >= len) return make_uint4(0u, 0u, 0u, 0u);
+                return __ldcg(reinterpret_cast<const uint4*>(pool + (int64_t)id * p.blk_stride + (int64_t)(key % p.block_size) * p.pos_stride));
+            };
+            auto store_item = [&](uint32_t tile, int i, const uint4& w) {      // 16 codes -> two 16-byte pieces of f16
+                const int row = i * ROWS + row_in;
+                const uint32_t dst = tile + (uint32_t)((piece >> 2) * (kKeys * 128) + row * 128);
+                uint32_t a, b, c, d;
+                const uint32_t c0 = (uint32_t)((piece & 3) * 2);
+                q8::expand<KV>(w.x, a, b);
+                q8::expand<KV>(w.y, c, d);
+                st_shared16(dst + (((c0) ^ (row & 7)) << 4), a, b, c, d);
+                q8::expand<KV>(w.z, a, b);
+                q8::expand<KV>(w.w, c, d);
+                st_shared16(dst + (((c0 + 1) ^ (row & 7)) << 4), a, b, c, d);
+            };
+            auto write_scales = [&](int kt, float sk, float sv, int id) {      // lanes 0..3 of the first converting warp
+                sv = sv < kMinScale ? kMinScale : sv;
+                float* e = scale_ring + (kt % kScaleRing) * 12 + lane;
+                e[0] = id >= 0 ? sk : 0.f;
+                e[4] = id >= 0 ? log2f(sv) : -INFINITY;
+                e[8] = id >= 0 ? 1.f / sv : 0.f;
+            };
+            int ids = fetch_ids(0);
+            float sk = 0.f, sv = 1.f;
+            auto load_scales = [&](int id) {
+                if (cw == 0 && lane < 4 && id >= 0) {
+                    const int64_t o = (int64_t)id * p.sc_blk_stride + (int64_t)g * p.sc_head_stride;
+                    sk = p.k_scale[o];
+                    sv = p.v_scale[o];
+                }
+            };
+            load_scales(ids);
+#pragma unroll
+            for (int n = 0; n < MINE; ++n) {
+                const int ik = item_at(n, false), iv = item_at(n, true);
+                if (n_tiles > 0 && ik >= 0) kr[n] = load_item(0, ik, ids, kb);
+                if (n_tiles > 0 && iv >= 0) vr[n] = load_item(0, iv, ids, vb);
+            }
+            int ids_next = fetch_ids(1);
+            for (int kt = 0; kt < n_tiles; ++kt) {
+                const int st_k = kt % kStagesK, st_v = kt % kStagesV;
+                const int ids_after = fetch_ids(kt + 2);
+                if (kt >= kStagesK)
+                    ok = mbar_wait_or_abort(bar(D::BarKFree + st_k), (uint32_t)((kt / kStagesK - 1) & 1), tail_words + 1);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                if (kNanCodes) {
+                    uint64_t keys = 0;
+#pragma unroll
+                    for (int n = 0; n < MINE; ++n) {
+                        const int i = item_at(n, true);
+                        if (i < 0) continue;
+                        auto nan_of = [](uint32_t w) -> uint32_t { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };   // bit 7 of a NaN byte
+                        const uint32_t fx = nan_of(vr[n].x), fy = nan_of(vr[n].y), fz = nan_of(vr[n].z), fw = nan_of(vr[n].w);
+                        const uint32_t lanes = __ballot_sync(0xffffffffu, (fx | fy | fz | fw) != 0);
+                        if (lanes != 0) {
+                            vr[n].x &= ~((fx >> 7) * 0xffu);
+                            vr[n].y &= ~((fy >> 7) * 0xffu);
+                            vr[n].z &= ~((fz >> 7) * 0xffu);
+                            vr[n].w &= ~((fw >> 7) * 0xffu);
+                            for (int r = 0; r < ROWS; ++r)
+                                if ((lanes >> (r * CPR)) & ((1u << CPR) - 1u)) keys |= 1ull << (i * ROWS + r);
+                        }
+                    }
+                    if (lane == 0) nan_ring[(kt % kScaleRing) * kConvWarps + cw] = keys;
+                }
+                if (cw == 0 && lane < 4) write_scales(kt, sk, sv, ids);
+                if (cw == 0 || kNanCodes) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(D::BarScale + kt % kScaleRing));
+                }
+#pragma unroll
+                for (int n = 0; n < MINE; ++n) {
+                    const int i = item_at(n, false);
+                    if (i >= 0) {
+                        store_item(sK + st_k * KV_BYTES, i, kr[n]);
+                        if (kt + 1 < n_tiles) kr[n] = load_item(kt + 1, i, ids_next, kb);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(bar(D::BarKFull + st_k));
+                if (kt >= kStagesV)
+                    ok = mbar_wait_or_abort(bar(D::BarVFree + st_v), (uint32_t)((kt / kStagesV - 1) & 1), tail_words + 1);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+#pragma unroll
+                for (int n = 0; n < MINE; ++n) {
+                    const int i = item_at(n, true);
+                    if (i >= 0) {
+                        store_item(sV + st_v * KV_BYTES, i, vr[n]);
+                        if (kt + 1 < n_tiles) vr[n] = load_item(kt + 1, i, ids_next, vb);
+                    }
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(bar(D::BarVFull + st_v));
+                ids = ids_next;
+                ids_next = ids_after;
+                load_scales(ids);
+            }
+            if (!ok) abort_flag = 1;
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+        const uint32_t t_lane = tmem + ((uint32_t)(32 * warp) << 16);     // this warp's 32 lanes; lane = row
+        const int tok = q_start + (tid >> 3), hh = tid & 7;
+        const bool row_ok = tok < T && hh < heads && q0 + tok >= 0 && q0 + tok < p.n_tokens;
+        // Q row: scaled by a power of two so that its largest element lies in [1, 2), as f16
+        float f_row;
+        {
+            const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(p.q) + (int64_t)(row_ok ? q0 + tok : 0) * p.q_stride +
+                                       (int64_t)(row_ok ? g * p.group + h0 + hh : 0) * HD;
+            float top = 0.f;
+            if (row_ok)
+                for (int c = 0; c < HD / 8; ++c) {
+                    const Vec16<__nv_bfloat16> v = load16(src + 8 * c);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v.get(i)));
+                }
+            int e = (int)((uint32_t)__float_as_int(top) >> 23) - 127;
+            e = top == 0.f || e > 127 ? 0 : min(max(e, -126), 126);
+            const float mult = __int_as_float((127 - e) << 23);
+            f_row = p.scale_log2 * __int_as_float((127 + e) << 23);
+            for (int c = 0; c < HD / 8; ++c) {
+                uint32_t w[4] = {0u, 0u, 0u, 0u};
+                if (row_ok) {
+                    const Vec16<__nv_bfloat16> v = load16(src + 8 * c);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = pack_f16x2(v.get(2 * i) * mult, v.get(2 * i + 1) * mult);
+                }
+                st_shared16(sQ + (c >> 3) * (kRows * 128) + tid * 128 + (((c & 7) ^ (tid & 7)) << 4), w[0], w[1], w[2], w[3]);
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        q_ready_barrier();
+        const int limit = ctx + tok;      // last key this row may see
+        const uint32_t t_o = t_lane + COL_O;
+        const volatile uint32_t* abort_now = tail_words + 1;
+        float m_run = -INFINITY, l_run = 0.f;
+        for (int kt = 0; kt < n_tiles; ++kt) {
+            // (a warp gives up as a whole: its tensor-memory accesses and votes are warp-wide)
+            ok = __all_sync(0xffffffffu, mbar_wait_or_abort(bar(D::BarScale + kt % kScaleRing), (uint32_t)((kt / kScaleRing) & 1), abort_now) && !*abort_now);
+            if (!ok) break;
+            const float* ring = scale_ring + (kt % kScaleRing) * 12;
+            const float4 sk4 = *reinterpret_cast<const float4*>(ring), lv4 = *reinterpret_cast<const float4*>(ring + 4),
+                         iv4 = *reinterpret_cast<const float4*>(ring + 8);
+            const float fac[4] = {f_row * sk4.x, f_row * sk4.y, f_row * sk4.z, f_row * sk4.w};
+            const float lv[4] = {lv4.x, lv4.y, lv4.z, lv4.w}, isv[4] = {iv4.x, iv4.y, iv4.z, iv4.w};
+            ok = __all_sync(0xffffffffu, mbar_wait_or_abort(bar(D::BarS + (kt & 1)), (uint32_t)((kt >> 1) & 1), abort_now));
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const uint32_t s_src = t_lane + COL_S + (uint32_t)((kt & 1) * kKeys);
+            const int key_base = kt * kKeys;
+            const bool masked = key_base + kKeys - 1 > ctx + q_start;      // else every row sees every key of the tile
+            uint32_t sr[2][32];
+            tmem_ld32_issue(s_src, sr[0]);
+            tmem_ld32_issue(s_src + 32, sr[1]);
+            tmem_ld_wait();
+            // x = s * factor + log2(sv), two at a time
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                for (int i = 0; i < 32; i += 2) {
+                    const int b = 2 * hf + (i >> 4);
+                    float x0, x1;
+                    unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(sr[hf][i]), __uint_as_float(sr[hf][i + 1])), pack_f32x2(fac[b], fac[b]),
+                                           pack_f32x2(lv[b], lv[b])), x0, x1);
+                    sr[hf][i] = __float_as_uint(x0);
+                    sr[hf][i + 1] = __float_as_uint(x1);
+                }
+            if (kNanCodes) {
+                const uint64_t* nr = nan_ring + (kt % kScaleRing) * kConvWarps;
+                const uint64_t keys = nr[0] | nr[1] | nr[2];
+                if (keys != 0) {
+#pragma unroll
+                    for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if ((keys >> (32 * hf + i)) & 1ull) sr[hf][i] = 0x7fffffffu;
+                }
+            }
+            if (masked) {
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (key_base + 32 * hf + i > limit) sr[hf][i] = 0xff800000u;
+            }
+            float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+                for (int i = 0; i < 32; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], __uint_as_float(sr[hf][i]));
+            const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+            const bool move = __any_sync(0xffffffffu, mx > m_run + kLazy);
+            if (move && kt > 0) {                                          // the output is rewritten: PV(kt - 1) has to be over
+                ok = __all_sync(0xffffffffu, mbar_wait_or_abort(bar(D::BarPV + ((kt - 1) & 1)), (uint32_t)(((kt - 1) >> 1) & 1), abort_now));
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            }
+            if (move) {
+                const float m_new = fmaxf(m_run, mx);
+                const float alpha = m_new == -INFINITY ? 1.f : ex2(m_run - m_new);
+                m_run = m_new;
+                l_run *= alpha;
+                if (kt > 0) {
+#pragma unroll
+                    for (int c = 0; c < HD / 32; ++c) {
+                        uint32_t r[32];
+                        tmem_ld32_issue(t_o + 32 * c, r);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+                        tmem_st32(t_o + 32 * c, r);
+                    }
+                    tmem_st_wait();
+                }
+            }
+            const float m_ref = m_run == -INFINITY ? 0.f : m_run;
+            const uint64_t neg_m2 = pack_f32x2(-m_ref, -m_ref);
+            const uint32_t p_dst = sP + (kt % kBufsP) * P_BYTES + tid * 128;
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                float v[32];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {                              // a block of 16 keys: one V scale
+                    uint64_t ps2[2] = {0ull, 0ull};
+#pragma unroll
+                    for (int i = 16 * q; i < 16 * q + 16; i += 2) {
+                        float x0, x1;
+                        unpack_f32x2(add_f32x2(pack_f32x2(__uint_as_float(sr[hf][i]), __uint_as_float(sr[hf][i + 1])), neg_m2), x0, x1);
+                        v[i] = ex2(x0);
+                        v[i + 1] = ex2(x1);
+                        ps2[(i >> 1) & 1] = add_f32x2(ps2[(i >> 1) & 1], pack_f32x2(v[i], v[i + 1]));
+                    }
+                    float a0, a1, b0, b1;
+                    unpack_f32x2(ps2[0], a0, a1);
+                    unpack_f32x2(ps2[1], b0, b1);
+                    const float sum = (a0 + a1) + (b0 + b1);
+                    l_run = sum == 0.f ? l_run : fmaf(sum, isv[2 * hf + q], l_run);      // (a block the row does not see may have any scale)
+                }
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    st_shared16(p_dst + (((4 * hf + c) ^ (tid & 7)) << 4), pack_f16x2(v[8 * c + 0], v[8 * c + 1]), pack_f16x2(v[8 * c + 2], v[8 * c + 3]),
+                                pack_f16x2(v[8 * c + 4], v[8 * c + 5]), pack_f16x2(v[8 * c + 6], v[8 * c + 7]));
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            if (!ok) break;
+            mbar_arrive(bar(D::BarPReady + (kt & 1)));
+        }
+        if (!ok) abort_flag = 1;
+        // ---- the row's output: after the last PV, 32 columns at a time
+        const bool have_o = n_tiles > 0 && ok;                             // (a wait of another role that ran out makes this one run out too)
+        if (have_o) {
+            ok = __all_sync(0xffffffffu, mbar_wait_or_abort(bar(D::BarPV + ((n_tiles - 1) & 1)), (uint32_t)(((n_tiles - 1) >> 1) & 1), abort_now));
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
+        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+        __nv_bfloat16* out_row = reinterpret_cast<__nv_bfloat16*>(p.out) + (int64_t)(row_ok ? q0 + tok : 0) * p.out_stride +
+                                 (int64_t)(row_ok ? g * p.group + h0 + hh : 0) * HD;
+#pragma unroll
+        for (int c = 0; c < HD / 32; ++c) {
+            float v[32];
+            if (ok && have_o) {                                            // (warp-uniform)
+                uint32_t r[32];
+                tmem_ld32_issue(t_o + 32 * c, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * inv;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = 0.f;
+            }
+            if (ok && row_ok) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint4 w;
+                    w.x = pack_bf16x2(v[8 * e + 0], v[8 * e + 1]);
+                    w.y = pack_bf16x2(v[8 * e + 2], v[8 * e + 3]);
+                    w.z = pack_bf16x2(v[8 * e + 4], v[8 * e + 5]);
+                    w.w = pack_bf16x2(v[8 * e + 6], v[8 * e + 7]);
+                    *reinterpret_cast<uint4*>(out_row + 32 * c + 8 * e) = w;
+                }
+            }
+        }
+        if (!ok) abort_flag = 1;
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (abort_flag && tid == 0)        // a wait expired: count it where the host can read it (ns_collect_status)
+        atomicAdd(&reinterpret_cast<PlanHeader*>(p.ws + p.L.header)->errors, 1);
+    if (warp == 0)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+    pdl_wait();                        // complete only after the decode kernel this one ran beside
+}
+
+bool q8_prefill_supported(const Q8Params& p, int dtype) {
+    return dtype == NS_BF16 && ((uintptr_t)p.out & 15) == 0 && p.out_stride % 8 == 0;      // beside what the decode kernel asks for
+}
+
+// NS_ERR_UNSUPPORTED: the kernel was not built with the register count its split needs; the scalar kernel serves then.
+template <int HD, typename KV> static int launch_prefill_q8_hd(const Q8Params& p, int max_items, cudaStream_t st) {
+    constexpr int atoms = HD / 64;
+    using D = q8p::Depth<HD>;
+    // tiles + tail; 1 KB of slack for the 1024-byte alignment
+    constexpr int smem = q8p::kRows * 128 * atoms + (D::K + D::V) * q8p::kKeys * 128 * atoms + D::P * q8p::kRows * 128 + q8p::kTailBytes +
+                         (HD == 64 ? 1024 : 0);
+    static SmemOptIn optin;
+    if (optin.needs((size_t)smem)) {
+        // setmaxnreg moves registers between the warpgroups within what the block was launched with: it must be all of 128 a thread
+        cudaFuncAttributes attr;
+        cudaError_t e = cudaFuncGetAttributes(&attr, prefill_q8_kernel<HD, KV>);
+        if (e != cudaSuccess) return fail(NS_ERR_CUDA, "prefill_q8: cannot query the kernel: %s", cudaGetErrorString(e));
+        if (attr.numRegs * q8p::kThreads < (q8p::kRegsSoftmax + q8p::kRegsOther) * 128) return NS_ERR_UNSUPPORTED;
+        e = cudaFuncSetAttribute(prefill_q8_kernel<HD, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return fail(NS_ERR_CUDA, "prefill_q8: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
+        optin.done((size_t)smem);
+    }
+    cudaError_t e = launch_pdl(prefill_q8_kernel<HD, KV>, dim3((unsigned)max_items, (unsigned)(p.n_kv_heads * ((p.group + 7) / 8))),
+                               dim3(q8p::kThreads), (size_t)smem, st, p);
+    if (e != cudaSuccess) return fail(NS_ERR_CUDA, "prefill_q8: launch failed: %s", cudaGetErrorString(e));
+    return NS_OK;
+}
+
+int launch_q8_prefill(const Q8Params& p, int pool_dtype, int max_items, cudaStream_t st) {
+    if (p.head_dim == 64)
+        return pool_dtype == NS_INT8 ? launch_prefill_q8_hd<64, KvInt8>(p, max_items, st) : launch_prefill_q8_hd<64, KvE4m3>(p, max_items, st);
+    return pool_dtype == NS_INT8 ? launch_prefill_q8_hd<128, KvInt8>(p, max_items, st) : launch_prefill_q8_hd<128, KvE4m3>(p, max_items, st);
+}
+
+}  // namespace ns
