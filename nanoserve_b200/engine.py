@@ -15,6 +15,9 @@ VALUE for the end-of-sequence test, so this is done only for steps whose samplin
 ignore_eos=True; any other step is waited for before the host goes on, exactly as without the option. Scheduling
 decisions, and therefore tokens, are the same as without lookahead; `step()` returns a step's outputs one call
 later and `has_unfinished()` stays true until they have been returned.
+
+`kv_cache_dtype="int8"` or `"fp8_e4m3"` (not in the reference) keeps K and V in 8 bits with a scale per block and KV head:
+about half the cache bytes per token, so twice the context in the same pool; None keeps the model's dtype.
 """
 from __future__ import annotations
 
@@ -52,7 +55,8 @@ class LLMEngine:
                  batch_wait_s: float = 0.02, kv_cache: str = "paged", kv_cache_tokens: int | None = None,
                  block_size: int = 16, attn_backend: str | None = None, cuda_graphs: bool | None = None,
                  chunked_prefill: bool | None = None, piecewise_graphs: bool | None = None,
-                 fused_ops: bool | None = None, prefix_caching: bool = False, lookahead: bool = False):
+                 fused_ops: bool | None = None, prefix_caching: bool = False, lookahead: bool = False,
+                 kv_cache_dtype=None):
         if model.device.type != "cuda":
             raise ValueError("nanoserve_b200 engines run on a CUDA device only")
         if kv_cache != "paged":
@@ -73,7 +77,8 @@ class LLMEngine:
         self.model = model if model.fused else model.with_fused_ops()
         max_seats = max(max_num_seqs, 1)
         self.kv = PagedKVManager(model.cfg, budget, block_size, device=model.device, dtype=model.dtype,
-                                 attn_backend="native", prefix_caching=prefix_caching, max_seats=max_seats)
+                                 attn_backend="native", prefix_caching=prefix_caching, max_seats=max_seats,
+                                 kv_dtype=kv_cache_dtype)
         if chunked_prefill is None:
             chunked_prefill = True
         if not chunked_prefill:
@@ -129,6 +134,7 @@ class LLMEngine:
         s["num_preemptions"] = self.scheduler.num_preemptions
         s["kv_util_mean"] = s["kv_util_sum"] / s["kv_util_samples"] if s["kv_util_samples"] else None
         s["kv_cache"] = self.kv.kind
+        s["kv_cache_dtype"] = str(self.kv.pool.k.dtype).replace("torch.", "")
         s["attn_backend"] = self.attn_backend
         s["cuda_graphs"] = self.graph_runner is not None
         s["graph_buckets"] = self.graph_runner.captured_buckets if self.graph_runner else []

@@ -39,6 +39,7 @@ class EngineSpec:
     kv_cache_tokens: int | None = None
     prefix_caching: bool = False
     lookahead: bool = False
+    kv_cache_dtype: str | None = None    # None: the model's dtype; "int8" or "fp8_e4m3": an 8-bit cache
     capture_graphs: bool = True          # capture every CUDA graph before serving
     n_layers: int | None = None          # shrink the architecture (tests)
     vocab: int | None = None
@@ -59,7 +60,8 @@ def build_engine(spec: EngineSpec):
                                 n_layers=spec.n_layers, vocab=spec.vocab)
     return LLMEngine(Qwen2Model(ModelConfig(**cfg), sd), eos_token_ids=[], max_seq_len=spec.max_seq_len,
                      max_num_seqs=spec.max_num_seqs, max_num_batched_tokens=spec.max_num_batched_tokens,
-                     kv_cache_tokens=spec.kv_cache_tokens, prefix_caching=spec.prefix_caching, lookahead=spec.lookahead)
+                     kv_cache_tokens=spec.kv_cache_tokens, prefix_caching=spec.prefix_caching, lookahead=spec.lookahead,
+                     kv_cache_dtype=spec.kv_cache_dtype)
 
 
 # ---------------------------------------------------------------------------------------------------- child process

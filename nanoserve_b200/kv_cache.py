@@ -14,6 +14,27 @@ from collections import OrderedDict
 
 import torch
 
+# KV cache dtypes a caller may ask for by name; None / "auto" is the model's own dtype
+KV_CACHE_DTYPES = {"int8": torch.int8, "fp8_e4m3": torch.float8_e4m3fn}
+
+
+def resolve_kv_dtype(kv_dtype) -> torch.dtype | None:
+    """None for the model's dtype, or the element type of an 8-bit pool (given as a torch dtype or by name)."""
+    if kv_dtype is None or kv_dtype == "auto":
+        return None
+    if kv_dtype in KV_CACHE_DTYPES.values():
+        return kv_dtype
+    if kv_dtype in KV_CACHE_DTYPES:
+        return KV_CACHE_DTYPES[kv_dtype]
+    raise ValueError(f"kv cache dtype {kv_dtype!r}: expected None, 'auto' or one of {sorted(KV_CACHE_DTYPES)}")
+
+
+def kv_cache_bytes_per_block(cfg, block_size: int, dtype, kv_dtype=None) -> int:
+    """HBM bytes of one block over all layers: K and V rows, and for 8-bit pools a scale per KV head for each."""
+    if resolve_kv_dtype(kv_dtype) is None:
+        return block_size * cfg.kv_bytes_per_token(dtype)
+    return cfg.n_layers * 2 * cfg.n_kv_heads * (block_size * cfg.head_dim + 4)
+
 
 class NoFreeBlocks(Exception):
     """The pool is exhausted: the scheduler must preempt someone or wait."""
@@ -196,38 +217,64 @@ class BlockTable:
 
 
 class PagedKVCache:
-    """The shared block pool, allocated once [kv_cache.py:251-288]."""
+    """The shared block pool, allocated once [kv_cache.py:251-288]. With kv_dtype int8 / float8_e4m3fn the pool holds 8-bit
+    codes and k_scale / v_scale, fp32 [n_layers, num_blocks, n_kv_heads] (a scale per block and KV head); the reference
+    has no such pool."""
 
-    def __init__(self, cfg, num_blocks: int, block_size: int = 16, device="cuda", dtype=torch.bfloat16):
+    def __init__(self, cfg, num_blocks: int, block_size: int = 16, device="cuda", dtype=torch.bfloat16, kv_dtype=None):
+        self.kv_dtype = resolve_kv_dtype(kv_dtype)
         shape = (cfg.n_layers, num_blocks, block_size, cfg.n_kv_heads, cfg.head_dim)
-        self.k = torch.zeros(shape, device=device, dtype=dtype)
-        self.v = torch.zeros(shape, device=device, dtype=dtype)
+        self.k_scale = self.v_scale = None
+        if self.kv_dtype is not None:
+            if block_size not in (1, 2, 4, 8, 16, 32, 64):
+                raise ValueError(f"an 8-bit KV cache takes blocks of 1, 2, 4 ... 64 tokens, not {block_size}")
+            self.k_scale = torch.zeros(shape[:2] + shape[3:4], device=device, dtype=torch.float32)
+            self.v_scale = torch.zeros_like(self.k_scale)
+        self.k = torch.zeros(shape, device=device, dtype=dtype if self.kv_dtype is None else torch.int8)
+        self.v = torch.zeros_like(self.k)
+        if self.kv_dtype is not None:
+            self.k, self.v = self.k.view(self.kv_dtype), self.v.view(self.kv_dtype)       # (code 0 is the zero byte in both)
         self.cfg = cfg
         self.num_blocks = num_blocks
         self.block_size = block_size
         self.allocator = BlockAllocator(num_blocks)
-        self.reserved_bytes = num_blocks * block_size * cfg.kv_bytes_per_token(dtype)
+        self.reserved_bytes = num_blocks * kv_cache_bytes_per_block(cfg, block_size, dtype, kv_dtype)
 
     @classmethod
     def from_token_budget(cls, cfg, num_tokens: int, block_size: int = 16, device="cuda",
-                          dtype=torch.bfloat16) -> "PagedKVCache":
-        return cls(cfg, -(-num_tokens // block_size), block_size, device, dtype)
+                          dtype=torch.bfloat16, kv_dtype=None) -> "PagedKVCache":
+        return cls(cfg, -(-num_tokens // block_size), block_size, device, dtype, kv_dtype)
 
     @staticmethod
-    def tokens_for_bytes(cfg, nbytes: int, dtype=torch.bfloat16) -> int:
-        return nbytes // cfg.kv_bytes_per_token(dtype)
+    def tokens_for_bytes(cfg, nbytes: int, dtype=torch.bfloat16, kv_dtype=None, block_size: int = 16) -> int:
+        if resolve_kv_dtype(kv_dtype) is None:
+            return nbytes // cfg.kv_bytes_per_token(dtype)
+        return nbytes // kv_cache_bytes_per_block(cfg, block_size, dtype, kv_dtype) * block_size
+
+    def scales(self, layer: int) -> dict:
+        """The scale arguments of a layer's kernels: {} for a pool in the model's dtype."""
+        return {} if self.kv_dtype is None else {"k_scale": self.k_scale[layer], "v_scale": self.v_scale[layer]}
 
     def write(self, layer: int, k_new: torch.Tensor, v_new: torch.Tensor, slot_mapping: torch.Tensor) -> None:
         """Store this step's K/V ([N, n_kv_heads, head_dim]) at their slots: one scatter kernel for all
-        requests (ns_kv_write)."""
+        requests (ns_kv_write; 8-bit pools: ns_rope_append without a rotation)."""
+        if self.kv_dtype is not None:
+            from nanoserve_b200.kernels.rotary import kv_append
+            kv_append(k_new.contiguous(), v_new.contiguous(), self.k[layer], self.v[layer], slot_mapping, **self.scales(layer))
+            return
         from nanoserve_b200.kernels.fused import kv_write
         kv_write(k_new.contiguous(), v_new.contiguous(), self.k[layer], self.v[layer], slot_mapping)
 
     def gather(self, layer: int, block_table: torch.Tensor, length: int) -> tuple[torch.Tensor, torch.Tensor]:
         """Dense copy of one request's first `length` tokens, [1, n_kv_heads, length, head_dim]. Inspection
-        helper only: the attention kernel reads the blocks in place."""
+        helper only: the attention kernel reads the blocks in place. 8-bit pools: the values the codes stand for, fp32."""
         kvh, hd = self.cfg.n_kv_heads, self.cfg.head_dim
         idx = block_table.long()
+        if self.kv_dtype is not None:
+            from nanoserve_b200.kernels.rotary import kv_values
+            k, v = [kv_values(pool[layer].view(torch.int8)[idx].view(self.kv_dtype), scale[layer][idx]).reshape(-1, kvh, hd)[:length]
+                    for pool, scale in ((self.k, self.k_scale), (self.v, self.v_scale))]
+            return k.transpose(0, 1)[None], v.transpose(0, 1)[None]
         k = self.k[layer][idx].reshape(-1, kvh, hd)[:length]
         v = self.v[layer][idx].reshape(-1, kvh, hd)[:length]
         return k.transpose(0, 1)[None], v.transpose(0, 1)[None]

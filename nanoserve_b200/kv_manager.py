@@ -24,8 +24,8 @@ class PagedKVManager:
 
     def __init__(self, cfg: ModelConfig, budget_tokens: int, block_size: int = 16, device="cuda",
                  dtype=torch.bfloat16, watermark: float = 0.01, attn_backend: str = "native",
-                 prefix_caching: bool = False, max_seats: int = 256):
-        self.pool = PagedKVCache.from_token_budget(cfg, budget_tokens, block_size, device, dtype)
+                 prefix_caching: bool = False, max_seats: int = 256, kv_dtype=None):
+        self.pool = PagedKVCache.from_token_budget(cfg, budget_tokens, block_size, device, dtype, kv_dtype)
         self.block_size = block_size
         self.device = device
         self.attn_backend = attn_backend

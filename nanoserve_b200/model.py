@@ -36,15 +36,31 @@ class ModelConfig:
     rope_theta: float
     rms_norm_eps: float
     tie_word_embeddings: bool
+    # rotary positions beyond the reference's (half layout, whole head, unscaled): see kernels.rotary
+    rope_scaling: dict | None = None         # a checkpoint's rope_scaling entry (linear, ntk, yarn)
+    partial_rotary_factor: float = 1.0       # share of each head that is rotated
+    rope_interleaved: bool = False           # pairs (2i, 2i + 1) instead of (i, i + r/2)
+
+    @property
+    def rotary_dim(self) -> int:
+        return int(self.head_dim * self.partial_rotary_factor) // 2 * 2
+
+    @property
+    def plain_rope(self) -> bool:
+        scaled = self.rope_scaling and self.rope_scaling.get("rope_type", self.rope_scaling.get("type", "default")) != "default"
+        return not scaled and self.rotary_dim == self.head_dim and not self.rope_interleaved
 
     @classmethod
     def from_hf_config(cls, d: dict) -> "ModelConfig":
-        theta = d.get("rope_theta") or (d.get("rope_parameters") or {}).get("rope_theta")
+        params = d.get("rope_parameters") or {}
+        theta = d.get("rope_theta") or params.get("rope_theta")
+        scaling = d.get("rope_scaling") or (params if params.get("rope_type", "default") != "default" else None)
         return cls(vocab_size=d["vocab_size"], hidden_size=d["hidden_size"], n_layers=d["num_hidden_layers"],
                    n_heads=d["num_attention_heads"], n_kv_heads=d["num_key_value_heads"],
                    head_dim=d.get("head_dim") or d["hidden_size"] // d["num_attention_heads"],
                    intermediate_size=d["intermediate_size"], rope_theta=float(theta),
-                   rms_norm_eps=d["rms_norm_eps"], tie_word_embeddings=d.get("tie_word_embeddings", False))
+                   rms_norm_eps=d["rms_norm_eps"], tie_word_embeddings=d.get("tie_word_embeddings", False),
+                   rope_scaling=scaling, partial_rotary_factor=float(d.get("partial_rotary_factor") or params.get("partial_rotary_factor") or 1.0))
 
     def kv_bytes_per_token(self, dtype: torch.dtype) -> int:
         return self.n_layers * 2 * self.n_kv_heads * self.head_dim * torch.finfo(dtype).bits // 8
@@ -171,6 +187,13 @@ class Qwen2Model:
         # RoPE inverse frequencies in fp32, computed on the CPU like the reference (nanoserve/model.py:168)
         inv_freq = 1.0 / (cfg.rope_theta ** (torch.arange(0, cfg.head_dim, 2, dtype=torch.float) / cfg.head_dim))
         self.inv_freq = inv_freq.to(self.device)
+        # fp32 tables of the rotary kernels (kernels.rotary): positions that are scaled, partial or interleaved, and every step
+        # over an 8-bit cache
+        from nanoserve_b200.kernels.rotary import rotary_frequencies
+        self.rot_freq, self.rope_factor = None, 1.0
+        if not cfg.plain_rope or cfg.rope_theta > 1.0:               # (the 16-bit path never asked theta to exceed 1)
+            rot_freq, self.rope_factor = rotary_frequencies(cfg.rotary_dim, cfg.rope_theta, cfg.rope_scaling)
+            self.rot_freq = rot_freq.to(self.device)
 
     # ---- variants -----------------------------------------------------------------------------------------------
     def with_fused_ops(self) -> "Qwen2Model":
@@ -198,6 +221,9 @@ class Qwen2Model:
     # ---- token-wise pieces ------------------------------------------------------------------------------------
     def rope(self, positions: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """cos/sin [1, T, head_dim] in the model dtype for int64 positions [T]."""
+        if not self.cfg.plain_rope:
+            raise NotImplementedError("cos / sin of the model's dtype exist for unscaled half-layout positions of the whole head only: "
+                                      "rope_fp32 serves the others")
         if self.fused:
             from nanoserve_b200.kernels.fused import rope_cos_sin
             cos, sin = rope_cos_sin(positions.contiguous(), self.inv_freq, self.cfg.head_dim, self.dtype)
@@ -205,6 +231,24 @@ class Qwen2Model:
         freqs = positions[None, :, None].float() * self.inv_freq
         emb = torch.cat((freqs, freqs), dim=-1)
         return emb.cos().to(self.dtype), emb.sin().to(self.dtype)
+
+    def rope_fp32(self, positions: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """fp32 tables [T, rotary_dim / 2] of the model's positions, scaling included (kernels.rotary.rope_tables)."""
+        from nanoserve_b200.kernels.rotary import rope_tables
+        if self.rot_freq is None:
+            raise ValueError(f"rope theta {self.cfg.rope_theta} must be greater than 1")
+        return rope_tables(positions.contiguous(), self.rot_freq, self.rope_factor)
+
+    def _fp32_rope(self, paged) -> bool:
+        """Whether a step's rotation and KV store go through rope_append: an 8-bit pool, or positions rope_qkv does not cover."""
+        return not self.cfg.plain_rope or (paged is not None and paged.kv_dtype is not None)
+
+    def _rope_append(self, i: int, qkv: torch.Tensor, cos, sin, paged, slot_mapping, dense_kv: bool):
+        from nanoserve_b200.kernels.rotary import rope_append
+        cfg = self.cfg
+        pool = (None, None, None) if paged is None else (paged.k[i], paged.v[i], slot_mapping)
+        return rope_append(qkv, cos, sin, cfg.n_heads // self.tp_size, cfg.n_kv_heads // self.tp_size, cfg.head_dim, *pool,
+                           interleaved=cfg.rope_interleaved, dense_kv=dense_kv, **({} if paged is None else paged.scales(i)))
 
     def final_norm(self, x: torch.Tensor) -> torch.Tensor:
         if self.fused:
@@ -222,6 +266,10 @@ class Qwen2Model:
                                   dense_kv)
         h = rms_norm(x, layer.ln1, cfg.rms_norm_eps)
         N, hd = h.shape[1], cfg.head_dim
+        if self._fp32_rope(paged):
+            qkv = torch.cat([F.linear(h[0], w, b) for w, b in ((layer.q_w, layer.q_b), (layer.k_w, layer.k_b), (layer.v_w, layer.v_b))], dim=-1)
+            q, k, v = self._rope_append(i, qkv, cos, sin, paged, slot_mapping, True)
+            return q[None], k[None], v[None]
         q = F.linear(h, layer.q_w, layer.q_b).view(1, N, -1, hd)
         k = F.linear(h, layer.k_w, layer.k_b).view(1, N, -1, hd)
         v = F.linear(h, layer.v_w, layer.v_b).view(1, N, -1, hd)
@@ -236,6 +284,9 @@ class Qwen2Model:
         from nanoserve_b200.kernels.fused import rope_qkv
         layer, cfg = self.layers[i], self.cfg
         qkv = F.linear(h, layer.qkv_w, layer.qkv_b)[0]
+        if self._fp32_rope(paged):
+            q, k, v = self._rope_append(i, qkv, cos, sin, paged, slot_mapping, dense_kv)
+            return q[None], (k[None] if k is not None else None), (v[None] if v is not None else None)
         q, k, v = rope_qkv(qkv, cos[0], sin[0], cfg.n_heads // self.tp_size, cfg.n_kv_heads // self.tp_size,
                            cfg.head_dim, paged.k[i] if paged is not None else None,
                            paged.v[i] if paged is not None else None, slot_mapping, dense_kv=dense_kv)
@@ -292,7 +343,7 @@ class Qwen2Model:
         tables, lens, cu = _meta if _meta is not None else self._ragged_meta(seqs, paged, decode_meta)
         N, nh, hd = q.shape[1], q.shape[2], q.shape[3]
         o = None if out is None else out[0].view(N, nh, hd)
-        o = ragged_paged_attention(q[0], paged.k[i], paged.v[i], tables, lens, cu, hd ** -0.5, out=o)
+        o = ragged_paged_attention(q[0], paged.k[i], paged.v[i], tables, lens, cu, hd ** -0.5, out=o, **paged.scales(i))
         return o.view(1, N, nh * hd)
 
     @torch.inference_mode()
@@ -306,7 +357,7 @@ class Qwen2Model:
         assert sum(s.n_tokens for s in seqs) == token_ids.shape[0], "seqs must cover token_ids exactly"
         meta = self._ragged_meta(seqs, paged, decode_meta)
         x = F.embedding(token_ids, self.embed)[None]
-        cos, sin = self.rope(positions)
+        cos, sin = self.rope_fp32(positions) if self._fp32_rope(paged) else self.rope(positions)
         for i in range(self.cfg.n_layers):
             q, k, v = self._pre(i, x, cos, sin, paged, slot_mapping)
             x = self._post(i, x, self._attend(i, q, k, v, seqs, paged, decode_meta, _meta=meta))
@@ -396,9 +447,12 @@ class Qwen2Model:
         # GEMM (inside a capture this becomes a fork and a join in the graph).
         # tensor parallel, small steps: the two all-reduces of a layer are fused with the add + RMSNorm after them and
         # read the peers' partials over NVLink (tensor_parallel.PeerReduce); larger steps use the NCCL all-reduce
+        # An 8-bit pool, or positions rope_qkv does not cover: the QKV product is followed by rope_append (whose CTAs own whole
+        # blocks: a block's scale depends on all its rows), not by a GEMM epilogue that stores K and V row by row.
+        fp32_rope, kv8 = self._fp32_rope(paged), paged.kv_dtype is not None
         peer = self.tp_peer if (self.tp_peer is not None and self.tp_group is not None and T <= self.tp_peer.max_rows) else None
         plan_stream = None
-        if plan:
+        if plan and not (kv8 and cu is None):                         # (decode rows of an 8-bit pool need no plan)
             main = torch.cuda.current_stream()
             plan_stream = Qwen2Model._plan_streams.get(self.device)
             if plan_stream is None:
@@ -406,12 +460,16 @@ class Qwen2Model:
             plan_stream.wait_stream(main)
             with torch.cuda.stream(plan_stream):
                 meta.workspace.plan(meta.seq_lens, cu, meta.n_seqs, paged.block_size, meta.table_rows)
-        cos, sin = rope_cos_sin(meta.positions, self.inv_freq, hd, self.dtype)
+        cos, sin = self.rope_fp32(meta.positions) if fp32_rope else rope_cos_sin(meta.positions, self.inv_freq, hd, self.dtype)
         x = F.embedding(meta.tokens, self.embed)
         h = norm(x, self.layers[0].ln1, eps)
         scale = hd ** -0.5
         for i, layer in enumerate(self.layers):
-            if thin_qkv:
+            if fp32_rope:
+                # (thin_gemm where the fused form would have been taken: its weights are requested before its input is there)
+                qkv = thin_gemm(h, layer.qkv_w, layer.qkv_b) if thin_qkv else F.linear(h, layer.qkv_w, layer.qkv_b)
+                q, _, _ = self._rope_append(i, qkv, cos, sin, paged, meta.slot_mapping, False)
+            elif thin_qkv:
                 q = thin_gemm(h, layer.qkv_w, layer.qkv_b, epilogue=EPI_ROPE_KV, cos=cos, sin=sin, k_cache=paged.k[i],
                               v_cache=paged.v[i], slots=meta.slot_mapping, n_heads=nh, n_kv_heads=nkv)
             elif skinny_qkv:
@@ -425,7 +483,7 @@ class Qwen2Model:
                 plan_stream = None
             o = ragged_paged_attention(q, paged.k[i], paged.v[i], meta.block_tables, meta.seq_lens, cu, scale,
                                        n_seqs=meta.n_seqs, table_rows=meta.table_rows, workspace=meta.workspace,
-                                       planned=True)
+                                       planned=True, **paged.scales(i))
             o2 = o.view(T, nh * hd)
             if fold_norm:
                 x, ss = thin_gemm_residual(o2, layer.o_w, x)

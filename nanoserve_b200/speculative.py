@@ -122,7 +122,7 @@ class SpeculativeEngine:
     def __init__(self, target: Qwen2Model, draft: Qwen2Model, eos_token_ids: list[int], num_speculative_tokens: int = 4,
                  max_seq_len: int = 2048, max_num_seqs: int = 8, max_num_batched_tokens: int = 4096,
                  target_kv_tokens: int | None = None, draft_kv_tokens: int | None = None, block_size: int = 16,
-                 cuda_graphs: bool | None = None):
+                 cuda_graphs: bool | None = None, kv_cache_dtype=None):
         if target.cfg.vocab_size != draft.cfg.vocab_size:
             raise ValueError("draft and target must share a vocabulary")
         if target.device.type != "cuda":
@@ -139,8 +139,10 @@ class SpeculativeEngine:
         span = max_seq_len + self.k + 1
         t_tokens = target_kv_tokens or 8 * span
         d_tokens = draft_kv_tokens or t_tokens
-        self.tpool = PagedKVCache.from_token_budget(target.cfg, t_tokens + block_size, block_size, target.device, target.dtype)
-        self.dpool = PagedKVCache.from_token_budget(draft.cfg, d_tokens + block_size, block_size, draft.device, draft.dtype)
+        self.tpool = PagedKVCache.from_token_budget(target.cfg, t_tokens + block_size, block_size, target.device, target.dtype,
+                                                    kv_cache_dtype)
+        self.dpool = PagedKVCache.from_token_budget(draft.cfg, d_tokens + block_size, block_size, draft.device, draft.dtype,
+                                                    kv_cache_dtype)
         graphs = True if cuda_graphs is None else bool(cuda_graphs)
         step_tokens = self.max_num_batched_tokens + max_num_seqs * (self.k + 1)
         self._t = _Lane(target, self.tpool, max_num_seqs, step_tokens, span, graphs)

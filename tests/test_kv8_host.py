@@ -144,3 +144,47 @@ def test_frequencies_refusals(bad):
 def test_unknown_scaling_type():
     with pytest.raises(NotImplementedError):
         rotary_frequencies(64, 1e4, {"type": "other", "factor": 2.0})
+
+
+# ------------------------------------------------------------------------------------------------------ pool and configuration
+def tiny_cfg(**kw):
+    from nanoserve_b200.model import ModelConfig
+    return ModelConfig(**dict(dict(vocab_size=8, hidden_size=8, n_layers=3, n_heads=2, n_kv_heads=2, head_dim=64, intermediate_size=8,
+                                   rope_theta=1e4, rms_norm_eps=1e-6, tie_word_embeddings=True), **kw))
+
+
+def test_pool_of_8bit_codes():
+    from nanoserve_b200.kv_cache import PagedKVCache, kv_cache_bytes_per_block, resolve_kv_dtype
+    cfg = tiny_cfg()
+    for name, dt in (("int8", torch.int8), ("fp8_e4m3", torch.float8_e4m3fn), (torch.int8, torch.int8)):
+        pool = PagedKVCache(cfg, 5, 16, "cpu", torch.bfloat16, name)
+        assert pool.k.dtype == dt and pool.k.shape == (3, 5, 16, 2, 64) and pool.k_scale.shape == (3, 5, 2)
+        assert pool.reserved_bytes == pool.k.numel() * 2 + pool.k_scale.numel() * 8
+        assert pool.scales(1)["v_scale"].data_ptr() == pool.v_scale[1].data_ptr()
+    plain = PagedKVCache(cfg, 5, 16, "cpu", torch.bfloat16)
+    assert plain.kv_dtype is None and plain.scales(0) == {} and plain.reserved_bytes == plain.k.numel() * 4
+    per = kv_cache_bytes_per_block(cfg, 16, torch.bfloat16, "int8")
+    assert PagedKVCache.tokens_for_bytes(cfg, 10 * per + 5, torch.bfloat16, "int8") == 160
+    assert PagedKVCache.tokens_for_bytes(cfg, 10 * per, torch.bfloat16) == 10 * per // cfg.kv_bytes_per_token(torch.bfloat16)
+    assert resolve_kv_dtype("auto") is None
+    for bad in ("int4", torch.float16, 8):
+        with pytest.raises(ValueError):
+            resolve_kv_dtype(bad)
+    with pytest.raises(ValueError):
+        PagedKVCache(cfg, 5, 24, "cpu", torch.bfloat16, "int8")
+
+
+def test_configuration_of_rotary_positions():
+    from nanoserve_b200.model import ModelConfig
+    assert tiny_cfg().plain_rope and tiny_cfg().rotary_dim == 64
+    assert not tiny_cfg(partial_rotary_factor=0.5).plain_rope and tiny_cfg(partial_rotary_factor=0.4).rotary_dim == 24
+    assert not tiny_cfg(rope_interleaved=True).plain_rope and tiny_cfg(rope_scaling={"type": "default"}).plain_rope
+    hf = dict(vocab_size=8, hidden_size=128, num_hidden_layers=1, num_attention_heads=2, num_key_value_heads=1, intermediate_size=8,
+              rms_norm_eps=1e-6, rope_theta=1e6)
+    yarn = {"type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768}
+    assert ModelConfig.from_hf_config(hf).plain_rope
+    assert ModelConfig.from_hf_config(dict(hf, rope_scaling=yarn)).rope_scaling == yarn
+    new = ModelConfig.from_hf_config(dict({k: v for k, v in hf.items() if k != "rope_theta"},
+                                          rope_parameters=dict(rope_type="linear", factor=2.0, rope_theta=5e5, partial_rotary_factor=0.5)))
+    assert new.rope_theta == 5e5 and new.rotary_dim == 32 and new.rope_scaling["factor"] == 2.0
+    assert ModelConfig.from_hf_config(dict(hf, rope_parameters=dict(rope_type="default", rope_theta=1e6))).plain_rope
