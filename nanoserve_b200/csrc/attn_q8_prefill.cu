@@ -1,21 +1,22 @@
 // Prefill-chunk attention over 8-bit pools on the 5th-generation tensor cores (tcgen05), accumulators in tensor memory.
 //
-// Work item = (sequence, 16 query tokens, eight query heads of a KV head), from the plan: 128 rows of one UMMA tile (row r =
-// token r / 8, head r % 8) against key tiles of 64.
+// Work item = (sequence, 32 query tokens, eight query heads of a KV head): two UMMA tiles A and B of 128 rows (row r of a tile =
+// token r / 8, head r % 8) against the same key tiles of 64.
 //   S[128 x 64]  = Q[128 x HD] . K_tile[64 x HD]^T      f16 operands, fp32 accumulators
 //   O[128 x HD] += P[128 x 64] . V_tile[64 x HD]
-// The codes become f16 on their way into shared memory (exact for int8 and e4m3, so K and V are never rounded): three converting
+// The codes become f16 on their way into shared memory (exact for int8 and e4m3, so K and V are never rounded): six converting
 // warps read 16-byte pieces of the pool's rows, one tile ahead, and store them in the swizzled layout the UMMA descriptors
-// expect. Rows past the sequence and blocks outside the pool become zeros there. Scales stay out of the operands:
+// expect; both Q tiles use them. Rows past the sequence and blocks outside the pool become zeros there. Scales stay out of the
+// operands:
 //   x = s * (scale log2 e * 2^e_q * sk) + log2 sv,   P = 2^(x - m),   l += sum(P) / sv   per block of 16 keys
 // (Q is scaled by a power of two per row, P is relative to the row's largest contribution; see attn_q8_decode.cu.)
-// Two warpgroups, 256 threads, two CTAs per SM:
-//   warps 0-3  one softmax thread per row. 176 registers a thread
-//   warp 4     lane 0 issues every tcgen05.mma
-//   warps 5-7  convert K and V tiles. 80 registers a thread: (176 + 80) * 128 = 128 * 256, what the block was launched with
-// Pipeline over the key tiles as in the 16-bit kernel: S runs two tiles ahead, P double buffered, O stays in tensor memory and
-// is rescaled only when a row's reference has to move. Every mbarrier wait is bounded: on expiry the CTA counts an error in the
-// plan header (ns_collect_status), skips its stores, frees its tensor memory and returns.
+// Four warpgroups, 512 threads, one CTA per SM (all 512 columns of its tensor memory):
+//   warps 0-3, 4-7   one softmax thread per row of tile A, of tile B. 176 registers a thread
+//   warps 8, 9       lane 0 issues the tcgen05.mma of tile A, of tile B
+//   warps 10-15      convert K and V tiles. 80 registers a thread: 2 (176 + 80) 128 = 128 * 512, what the block was launched with
+// Pipeline per tile as in the 16-bit kernel: S runs two key tiles ahead, P double buffered, O stays in tensor memory and is
+// rescaled only when a row's reference has to move; A and B fill each other's gaps. Every mbarrier wait is bounded: on expiry the
+// CTA counts an error in the plan header (ns_collect_status), skips its stores, frees its tensor memory and returns.
 #include "attn_q8.cuh"
 #include "tc_common.cuh"
 
@@ -25,17 +26,18 @@ namespace q8p {
 
 using namespace tc;
 
-constexpr int kRows = 128, kKeys = 64, kThreads = 256, kConv = 96;     // softmax rows, keys per tile, threads, converting threads
+constexpr int kRows = 128, kKeys = 64, kThreads = 512, kConv = 192;    // rows of a Q tile, keys per tile, threads, converting threads
+constexpr int kTokens = 2 * kPrefillTileTokens;                        // query tokens per item
 constexpr int kConvWarps = kConv / 32;
 constexpr int kRegsSoftmax = 176, kRegsOther = 80;
 constexpr int kScaleRing = 8;       // a converter is at most five tiles ahead of the slowest softmax thread
 template <int HD> struct Depth {
-    static constexpr int K = HD == 64 ? 3 : 1, V = HD == 64 ? 4 : 2, P = 2;
-    // mbarriers: S0 S1 PV0 PV1 | K full | V full | K free | V free | P0 P1 ready | scales of a tile
-    static constexpr int BarS = 0, BarPV = 2, BarKFull = 4, BarVFull = BarKFull + K, BarKFree = BarVFull + V, BarVFree = BarKFree + K,
-                         BarPReady = BarVFree + V, BarScale = BarPReady + 2, Bars = BarScale + kScaleRing;
+    static constexpr int K = 3, V = HD == 64 ? 4 : 2, P = 2;
+    // mbarriers: S0 S1, PV0 PV1, P0 P1 ready of each Q tile | K full | V full | K free | V free | scales of a key tile
+    static constexpr int BarS = 0, BarPV = 4, BarPReady = 8, BarKFull = 12, BarVFull = BarKFull + K, BarKFree = BarVFull + V,
+                         BarVFree = BarKFree + K, BarScale = BarVFree + V, Bars = BarScale + kScaleRing;
 };
-constexpr int kTailBytes = 832;     // mbarriers, two words, the scale ring [8][3][4], the NaN-key ring [8][3]
+constexpr int kTailBytes = 1152;    // mbarriers, two words, the scale ring [8][3][4], the NaN-key ring [8][6]
 constexpr float kLazy = 8.f;
 constexpr float kMinScale = 7.8886090522101181e-31f;    // 2^-100
 
@@ -50,19 +52,19 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 __device__ __forceinline__ void st_shared16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-// Named barrier 1: the softmax threads and the issuing warp meet once, when Q is in place.
-__device__ __forceinline__ void q_ready_barrier() { asm volatile("bar.sync 1, %0;" ::"r"(kRows + 32) : "memory"); }
+// Named barriers 1 and 2: a tile's softmax threads and its issuing warp meet once, when Q is in place.
+__device__ __forceinline__ void q_ready_barrier(int tile) { asm volatile("bar.sync %0, %1;" ::"r"(1 + tile), "r"(kRows + 32) : "memory"); }
 
 }  // namespace q8p
 
 template <int HD, typename KV>
-__global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Params p) {
+__global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Params p) {
     using namespace q8p;
     using D = Depth<HD>;
     constexpr int kStagesK = D::K, kStagesV = D::V, kBufsP = D::P;
     constexpr int ATOMS = HD / 64;
     constexpr int Q_BYTES = kRows * 128 * ATOMS, KV_BYTES = kKeys * 128 * ATOMS, P_BYTES = kRows * 128;
-    constexpr uint32_t COL_S = 0, COL_O = 2 * kKeys, TMEM_COLS = 256;
+    constexpr uint32_t COL_TILE = 2 * kKeys + HD, COL_O = 2 * kKeys, TMEM_COLS = 512;      // per Q tile: S0, S1, O
     static_assert(D::Bars * 8 + 16 + kScaleRing * (48 + 8 * kConvWarps) <= kTailBytes, "the tail holds the barriers, two words and the rings");
     // V codes that are NaN (e4m3 only): 0 x NaN would reach rows that must not see the key, so the operand gets 0 there and the
     // key goes on a list: the score of a row that does see it becomes NaN (its whole output row then is).
@@ -73,14 +75,11 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
     const int sub = (p.group + 7) >> 3;
     int item_idx, vh;
     {
-        // the plan lists the items heaviest first; where they are one wave of two CTAs per SM, an SM's second CTA is light
+        // the plan lists tiles of 16 tokens, heaviest first: the even ones of a sequence stand for a pair, the odd ones for nothing
         const int n_items = hdr->n_prefill_items, n_kv = (int)gridDim.y;
-        const int units = n_items * n_kv, S = p.sm_count;
         const int lin = (int)(blockIdx.x + gridDim.x * blockIdx.y);
-        int r = lin;
-        if (S > 0 && units > S && units <= 2 * S && lin >= S) r = units - 1 - (lin - S);
-        item_idx = lin < units ? r / n_kv : n_items;
-        vh = r % n_kv;
+        item_idx = lin < n_items * n_kv ? lin / n_kv : n_items;
+        vh = lin % n_kv;
         if (item_idx >= n_items) {
             pdl_wait();                           // the grid must not complete before the decode kernel it overlaps
             return;
@@ -88,7 +87,7 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
     }
     const int2 item = reinterpret_cast<const int2*>(p.ws + p.L.prefill_items)[item_idx];
     const int s = item.x, q_start = item.y;
-    if (s < 0 || s >= p.n_seqs) {                 // a plan of another batch
+    if (s < 0 || s >= p.n_seqs || (q_start & kPrefillTileTokens)) {      // (s: a plan of another batch)
         pdl_wait();
         return;
     }
@@ -99,13 +98,14 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
     const int len = q8_len(p, s);
     const int ctx = len - T;
     const int32_t* table = p.block_tables + (int64_t)(p.table_rows ? p.table_rows[s] : s) * p.table_stride;
-    const int kv_end = min(len, ctx + q_start + kPrefillTileTokens);
+    const int kv_end = min(len, ctx + min(q_start + kTokens, T));
+    const int n_q = T - q_start > kPrefillTileTokens ? 2 : 1;                // Q tiles
     const int n_tiles = kv_end > 0 ? (kv_end + kKeys - 1) / kKeys : 0;
 
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
-    const uint32_t sQ = base, sK = sQ + Q_BYTES, sV = sK + kStagesK * KV_BYTES, sP = sV + kStagesV * KV_BYTES;
-    const uint32_t bar0 = sP + kBufsP * P_BYTES;
+    const uint32_t sQ0 = base, sK = sQ0 + 2 * Q_BYTES, sV = sK + kStagesK * KV_BYTES, sP0 = sV + kStagesV * KV_BYTES;
+    const uint32_t bar0 = sP0 + 2 * kBufsP * P_BYTES;
     auto bar = [&](int i) -> uint32_t { return bar0 + 8u * (uint32_t)i; };
     volatile uint32_t* tail_words = reinterpret_cast<volatile uint32_t*>(smem_raw + (bar0 - raw) + D::Bars * 8);
     volatile uint32_t& tmem_slot = tail_words[0];
@@ -122,7 +122,9 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
     if (tid == 0) {
 #pragma unroll
         for (int i = 0; i < D::Bars; ++i) {
-            const uint32_t count = i >= D::BarScale ? (kNanCodes ? kConvWarps : 1) : i >= D::BarPReady ? kRows : (i >= D::BarKFull && i < D::BarKFree) ? kConv : 1;
+            // K and V free: one commit per Q tile that read them
+            const uint32_t count = i >= D::BarScale ? (kNanCodes ? kConvWarps : 1) : i >= D::BarKFree ? n_q : i >= D::BarKFull ? kConv
+                                   : i >= D::BarPReady ? kRows : 1;
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar(i)), "r"(count) : "memory");
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -138,11 +140,13 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
     const uint32_t tmem = tmem_slot;
     bool ok = true;
 
-    if (warp >= 4) {
+    if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-        if (warp == 4) {
-            q_ready_barrier();
-            if (lane == 0) {
+        if (warp < 10) {
+            const int w = warp - 8;
+            q_ready_barrier(w);
+            if (lane == 0 && w < n_q) {
+                const uint32_t sQ = sQ0 + w * Q_BYTES, sP = sP0 + w * (kBufsP * P_BYTES), t_tile = tmem + w * COL_TILE;
                 constexpr uint32_t idesc_s = instr_desc(false, kKeys), idesc_pv = instr_desc(true, HD);
                 const uint64_t dQ = smem_desc(sQ, 16, 1024), dK = smem_desc(sK, 16, 1024), dP = smem_desc(sP, 16, 1024);
                 const uint64_t dV = smem_desc(sV, kKeys * 128, 1024);
@@ -151,14 +155,14 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
                     if (!mbar_wait_or_abort(bar(D::BarKFull + sk), (uint32_t)((kt / kStagesK) & 1), tail_words + 1)) { ok = false; return; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint64_t k0 = dK + (uint64_t)((sk * KV_BYTES) >> 4);
-                    const uint32_t d = tmem + COL_S + (uint32_t)((kt & 1) * kKeys);
+                    const uint32_t d = t_tile + (uint32_t)((kt & 1) * kKeys);
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; ++kk) {
                         const uint32_t a_off = (uint32_t)(((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4);
                         const uint32_t b_off = (uint32_t)(((kk >> 2) * (kKeys * 128) + (kk & 3) * 32) >> 4);
                         tc::mma_f16(d, dQ + a_off, k0 + b_off, idesc_s, kk > 0);
                     }
-                    mma_commit(bar(D::BarS + (kt & 1)));
+                    mma_commit(bar(D::BarS + 2 * w + (kt & 1)));
                     mma_commit(bar(D::BarKFree + sk));
                 };
                 auto issue_pv = [&](int kt) {
@@ -169,15 +173,15 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
                     const uint64_t v0 = dV + (uint64_t)((sv * KV_BYTES) >> 4);
 #pragma unroll
                     for (int kk = 0; kk < kKeys / 16; ++kk)
-                        tc::mma_f16(tmem + COL_O, p0 + (uint32_t)((kk * 32) >> 4), v0 + (uint32_t)((kk * 2048) >> 4), idesc_pv,
+                        tc::mma_f16(t_tile + COL_O, p0 + (uint32_t)((kk * 32) >> 4), v0 + (uint32_t)((kk * 2048) >> 4), idesc_pv,
                                     (kt > 0 || kk > 0) ? 1u : 0u);
-                    mma_commit(bar(D::BarPV + (kt & 1)));
+                    mma_commit(bar(D::BarPV + 2 * w + (kt & 1)));
                     mma_commit(bar(D::BarVFree + sv));
                 };
                 if (n_tiles > 0) issue_s(0);
                 if (n_tiles > 1) issue_s(1);
                 for (int kt = 0; kt < n_tiles && ok; ++kt) {
-                    if (!mbar_wait_or_abort(bar(D::BarPReady + (kt & 1)), (uint32_t)((kt >> 1) & 1), tail_words + 1)) { ok = false; break; }
+                    if (!mbar_wait_or_abort(bar(D::BarPReady + 2 * w + (kt & 1)), (uint32_t)((kt >> 1) & 1), tail_words + 1)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     issue_pv(kt);
                     if (kt + 2 < n_tiles) issue_s(kt + 2);
@@ -187,34 +191,39 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
         } else {
             // ---- converting warps. An item is 32 consecutive 16-code pieces of a tile: ROWS rows of it.
             constexpr int CPR = HD / 16, ROWS = 32 / CPR, ITEMS = kKeys / ROWS, MINE = (ITEMS + kConvWarps - 1) / kConvWarps;
-            const int cw = warp - 5, row_in = lane / CPR, piece = lane % CPR;
+            const int cw = warp - 10, row_in = lane / CPR, piece = lane % CPR;
             const uint8_t* kb = p.k_pool + g * p.head_stride + piece * 16;
             const uint8_t* vb = p.v_pool + g * p.head_stride + piece * 16;
             uint4 kr[MINE], vr[MINE];
-            auto fetch_ids = [&](int kt) -> int {              // lane b < 4: block of keys 16 b .. of the tile, -1: absent
+            // lane b & 3: where keys 16 b .. 16 b + 15 of the tile start in a pool, and their block; -1: absent
+            auto fetch_ids = [&](int kt, int64_t& off) -> int {
                 const int key = kt * kKeys + 16 * (lane & 3);
+                off = 0;
                 if (kt >= n_tiles || key >= kv_end) return -1;
-                const int id = table[key / p.block_size];
+                const int b = key / p.block_size, id = table[b];
+                off = (int64_t)id * p.blk_stride + (int64_t)(key - b * p.block_size) * p.pos_stride;
                 return (unsigned)id < (unsigned)p.num_blocks ? id : -1;
             };
             auto item_at = [&](int n, bool v) -> int { const int i = (v ? kConvWarps - 1 - cw : cw) + kConvWarps * n; return i < ITEMS ? i : -1; };
-            auto load_item = [&](int kt, int i, int ids, const uint8_t* pool) -> uint4 {
-                const int row = i * ROWS + row_in, key = kt * kKeys + row;
-                const int id = __shfl_sync(0xffffffffu, ids, row >> 4);
-                if (id < 0 || key >= len) return make_uint4(0u, 0u, 0u, 0u);
-                return __ldcg(reinterpret_cast<const uint4*>(pool + (int64_t)id * p.blk_stride + (int64_t)(key % p.block_size) * p.pos_stride));
+            // ROWS divides 16: an item lies inside one block
+            const int64_t lane_off = row_in * p.pos_stride, item_step = ROWS * p.pos_stride;
+            auto load_item = [&](int kt, int i, int id_all, int64_t off_all, const uint8_t* pool) -> uint4 {
+                const int b = i * ROWS >> 4;
+                const int id = __shfl_sync(0xffffffffu, id_all, b);
+                const int64_t off = __shfl_sync(0xffffffffu, off_all, b);
+                if (id < 0 || kt * kKeys + i * ROWS + row_in >= len) return make_uint4(0u, 0u, 0u, 0u);
+                return __ldcg(reinterpret_cast<const uint4*>(pool + off + lane_off + (i & (16 / ROWS - 1)) * item_step));
             };
+            const uint32_t piece_off = (uint32_t)((piece >> 2) * (kKeys * 128) + row_in * 128), chunk0 = (uint32_t)((piece & 3) * 2);
             auto store_item = [&](uint32_t tile, int i, const uint4& w) {      // 16 codes -> two 16-byte pieces of f16
-                const int row = i * ROWS + row_in;
-                const uint32_t dst = tile + (uint32_t)((piece >> 2) * (kKeys * 128) + row * 128);
+                const uint32_t dst = tile + piece_off + i * (ROWS * 128), r7 = (uint32_t)((i * ROWS + row_in) & 7);
                 uint32_t a, b, c, d;
-                const uint32_t c0 = (uint32_t)((piece & 3) * 2);
                 q8::expand<KV>(w.x, a, b);
                 q8::expand<KV>(w.y, c, d);
-                st_shared16(dst + (((c0) ^ (row & 7)) << 4), a, b, c, d);
+                st_shared16(dst + ((chunk0 ^ r7) << 4), a, b, c, d);
                 q8::expand<KV>(w.z, a, b);
                 q8::expand<KV>(w.w, c, d);
-                st_shared16(dst + (((c0 + 1) ^ (row & 7)) << 4), a, b, c, d);
+                st_shared16(dst + (((chunk0 + 1) ^ r7) << 4), a, b, c, d);
             };
             auto write_scales = [&](int kt, float sk, float sv, int id) {      // lanes 0..3 of the first converting warp
                 sv = sv < kMinScale ? kMinScale : sv;
@@ -223,7 +232,8 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
                 e[4] = id >= 0 ? log2f(sv) : -INFINITY;
                 e[8] = id >= 0 ? 1.f / sv : 0.f;
             };
-            int ids = fetch_ids(0);
+            int64_t off, off_next, off_after;
+            int ids = fetch_ids(0, off);
             float sk = 0.f, sv = 1.f;
             auto load_scales = [&](int id) {
                 if (cw == 0 && lane < 4 && id >= 0) {
@@ -236,13 +246,13 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
 #pragma unroll
             for (int n = 0; n < MINE; ++n) {
                 const int ik = item_at(n, false), iv = item_at(n, true);
-                if (n_tiles > 0 && ik >= 0) kr[n] = load_item(0, ik, ids, kb);
-                if (n_tiles > 0 && iv >= 0) vr[n] = load_item(0, iv, ids, vb);
+                if (n_tiles > 0 && ik >= 0) kr[n] = load_item(0, ik, ids, off, kb);
+                if (n_tiles > 0 && iv >= 0) vr[n] = load_item(0, iv, ids, off, vb);
             }
-            int ids_next = fetch_ids(1);
+            int ids_next = fetch_ids(1, off_next);
             for (int kt = 0; kt < n_tiles; ++kt) {
                 const int st_k = kt % kStagesK, st_v = kt % kStagesV;
-                const int ids_after = fetch_ids(kt + 2);
+                const int ids_after = fetch_ids(kt + 2, off_after);
                 if (kt >= kStagesK)
                     ok = mbar_wait_or_abort(bar(D::BarKFree + st_k), (uint32_t)((kt / kStagesK - 1) & 1), tail_words + 1);
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
@@ -276,7 +286,7 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
                     const int i = item_at(n, false);
                     if (i >= 0) {
                         store_item(sK + st_k * KV_BYTES, i, kr[n]);
-                        if (kt + 1 < n_tiles) kr[n] = load_item(kt + 1, i, ids_next, kb);
+                        if (kt + 1 < n_tiles) kr[n] = load_item(kt + 1, i, ids_next, off_next, kb);
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -289,21 +299,24 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
                     const int i = item_at(n, true);
                     if (i >= 0) {
                         store_item(sV + st_v * KV_BYTES, i, vr[n]);
-                        if (kt + 1 < n_tiles) vr[n] = load_item(kt + 1, i, ids_next, vb);
+                        if (kt + 1 < n_tiles) vr[n] = load_item(kt + 1, i, ids_next, off_next, vb);
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(bar(D::BarVFull + st_v));
                 ids = ids_next;
                 ids_next = ids_after;
+                off_next = off_after;
                 load_scales(ids);
             }
             if (!ok) abort_flag = 1;
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
-        const uint32_t t_lane = tmem + ((uint32_t)(32 * warp) << 16);     // this warp's 32 lanes; lane = row
-        const int tok = q_start + (tid >> 3), hh = tid & 7;
+        const int w = warp >> 2, row = tid & (kRows - 1);                  // Q tile, its row
+        const uint32_t sQ = sQ0 + w * Q_BYTES, sP = sP0 + w * (kBufsP * P_BYTES);
+        const uint32_t t_lane = tmem + w * COL_TILE + ((uint32_t)(32 * (warp & 3)) << 16);     // this warp's 32 lanes; lane = row
+        const int tok = q_start + w * kPrefillTileTokens + (row >> 3), hh = row & 7;
         const bool row_ok = tok < T && hh < heads && q0 + tok >= 0 && q0 + tok < p.n_tokens;
         // Q row: scaled by a power of two so that its largest element lies in [1, 2), as f16
         float f_row;
@@ -322,22 +335,23 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
             const float mult = __int_as_float((127 - e) << 23);
             f_row = p.scale_log2 * __int_as_float((127 + e) << 23);
             for (int c = 0; c < HD / 8; ++c) {
-                uint32_t w[4] = {0u, 0u, 0u, 0u};
+                uint32_t u[4] = {0u, 0u, 0u, 0u};
                 if (row_ok) {
                     const Vec16<__nv_bfloat16> v = load16(src + 8 * c);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = pack_f16x2(v.get(2 * i) * mult, v.get(2 * i + 1) * mult);
+                    for (int i = 0; i < 4; ++i) u[i] = pack_f16x2(v.get(2 * i) * mult, v.get(2 * i + 1) * mult);
                 }
-                st_shared16(sQ + (c >> 3) * (kRows * 128) + tid * 128 + (((c & 7) ^ (tid & 7)) << 4), w[0], w[1], w[2], w[3]);
+                st_shared16(sQ + (c >> 3) * (kRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4), u[0], u[1], u[2], u[3]);
             }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        q_ready_barrier();
+        q_ready_barrier(w);
         const int limit = ctx + tok;      // last key this row may see
         const uint32_t t_o = t_lane + COL_O;
         const volatile uint32_t* abort_now = tail_words + 1;
         float m_run = -INFINITY, l_run = 0.f;
-        for (int kt = 0; kt < n_tiles; ++kt) {
+        const int my_tiles = w < n_q ? n_tiles : 0;
+        for (int kt = 0; kt < my_tiles; ++kt) {
             // (a warp gives up as a whole: its tensor-memory accesses and votes are warp-wide)
             ok = __all_sync(0xffffffffu, mbar_wait_or_abort(bar(D::BarScale + kt % kScaleRing), (uint32_t)((kt / kScaleRing) & 1), abort_now) && !*abort_now);
             if (!ok) break;
@@ -346,12 +360,12 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
                          iv4 = *reinterpret_cast<const float4*>(ring + 8);
             const float fac[4] = {f_row * sk4.x, f_row * sk4.y, f_row * sk4.z, f_row * sk4.w};
             const float lv[4] = {lv4.x, lv4.y, lv4.z, lv4.w}, isv[4] = {iv4.x, iv4.y, iv4.z, iv4.w};
-            ok = __all_sync(0xffffffffu, mbar_wait_or_abort(bar(D::BarS + (kt & 1)), (uint32_t)((kt >> 1) & 1), abort_now));
+            ok = __all_sync(0xffffffffu, mbar_wait_or_abort(bar(D::BarS + 2 * w + (kt & 1)), (uint32_t)((kt >> 1) & 1), abort_now));
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t s_src = t_lane + COL_S + (uint32_t)((kt & 1) * kKeys);
+            const uint32_t s_src = t_lane + (uint32_t)((kt & 1) * kKeys);
             const int key_base = kt * kKeys;
-            const bool masked = key_base + kKeys - 1 > ctx + q_start;      // else every row sees every key of the tile
+            const bool masked = key_base + kKeys - 1 > ctx + q_start + w * kPrefillTileTokens;      // else every row sees every key of the tile
             uint32_t sr[2][32];
             tmem_ld32_issue(s_src, sr[0]);
             tmem_ld32_issue(s_src + 32, sr[1]);
@@ -370,7 +384,9 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
                 }
             if (kNanCodes) {
                 const uint64_t* nr = nan_ring + (kt % kScaleRing) * kConvWarps;
-                const uint64_t keys = nr[0] | nr[1] | nr[2];
+                uint64_t keys = 0;
+#pragma unroll
+                for (int i = 0; i < kConvWarps; ++i) keys |= nr[i];
                 if (keys != 0) {
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf)
@@ -394,7 +410,7 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
             const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
             const bool move = __any_sync(0xffffffffu, mx > m_run + kLazy);
             if (move && kt > 0) {                                          // the output is rewritten: PV(kt - 1) has to be over
-                ok = __all_sync(0xffffffffu, mbar_wait_or_abort(bar(D::BarPV + ((kt - 1) & 1)), (uint32_t)(((kt - 1) >> 1) & 1), abort_now));
+                ok = __all_sync(0xffffffffu, mbar_wait_or_abort(bar(D::BarPV + 2 * w + ((kt - 1) & 1)), (uint32_t)(((kt - 1) >> 1) & 1), abort_now));
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             }
             if (move) {
@@ -417,7 +433,7 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
             }
             const float m_ref = m_run == -INFINITY ? 0.f : m_run;
             const uint64_t neg_m2 = pack_f32x2(-m_ref, -m_ref);
-            const uint32_t p_dst = sP + (kt % kBufsP) * P_BYTES + tid * 128;
+            const uint32_t p_dst = sP + (kt % kBufsP) * P_BYTES + row * 128;
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
                 float v[32];
@@ -440,19 +456,19 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
                 }
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    st_shared16(p_dst + (((4 * hf + c) ^ (tid & 7)) << 4), pack_f16x2(v[8 * c + 0], v[8 * c + 1]), pack_f16x2(v[8 * c + 2], v[8 * c + 3]),
+                    st_shared16(p_dst + (((4 * hf + c) ^ (row & 7)) << 4), pack_f16x2(v[8 * c + 0], v[8 * c + 1]), pack_f16x2(v[8 * c + 2], v[8 * c + 3]),
                                 pack_f16x2(v[8 * c + 4], v[8 * c + 5]), pack_f16x2(v[8 * c + 6], v[8 * c + 7]));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (!ok) break;
-            mbar_arrive(bar(D::BarPReady + (kt & 1)));
+            mbar_arrive(bar(D::BarPReady + 2 * w + (kt & 1)));
         }
         if (!ok) abort_flag = 1;
         // ---- the row's output: after the last PV, 32 columns at a time
-        const bool have_o = n_tiles > 0 && ok;                             // (a wait of another role that ran out makes this one run out too)
+        const bool have_o = my_tiles > 0 && ok;                             // (a wait of another role that ran out makes this one run out too)
         if (have_o) {
-            ok = __all_sync(0xffffffffu, mbar_wait_or_abort(bar(D::BarPV + ((n_tiles - 1) & 1)), (uint32_t)(((n_tiles - 1) >> 1) & 1), abort_now));
+            ok = __all_sync(0xffffffffu, mbar_wait_or_abort(bar(D::BarPV + 2 * w + ((n_tiles - 1) & 1)), (uint32_t)(((n_tiles - 1) >> 1) & 1), abort_now));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
         const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
@@ -474,12 +490,12 @@ __global__ void __launch_bounds__(q8p::kThreads, 2) prefill_q8_kernel(const Q8Pa
             if (ok && row_ok) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    uint4 w;
-                    w.x = pack_bf16x2(v[8 * e + 0], v[8 * e + 1]);
-                    w.y = pack_bf16x2(v[8 * e + 2], v[8 * e + 3]);
-                    w.z = pack_bf16x2(v[8 * e + 4], v[8 * e + 5]);
-                    w.w = pack_bf16x2(v[8 * e + 6], v[8 * e + 7]);
-                    *reinterpret_cast<uint4*>(out_row + 32 * c + 8 * e) = w;
+                    uint4 o;
+                    o.x = pack_bf16x2(v[8 * e + 0], v[8 * e + 1]);
+                    o.y = pack_bf16x2(v[8 * e + 2], v[8 * e + 3]);
+                    o.z = pack_bf16x2(v[8 * e + 4], v[8 * e + 5]);
+                    o.w = pack_bf16x2(v[8 * e + 6], v[8 * e + 7]);
+                    *reinterpret_cast<uint4*>(out_row + 32 * c + 8 * e) = o;
                 }
             }
         }
@@ -503,15 +519,15 @@ template <int HD, typename KV> static int launch_prefill_q8_hd(const Q8Params& p
     constexpr int atoms = HD / 64;
     using D = q8p::Depth<HD>;
     // tiles + tail; 1 KB of slack for the 1024-byte alignment
-    constexpr int smem = q8p::kRows * 128 * atoms + (D::K + D::V) * q8p::kKeys * 128 * atoms + D::P * q8p::kRows * 128 + q8p::kTailBytes +
-                         (HD == 64 ? 1024 : 0);
+    constexpr int smem = 2 * q8p::kRows * 128 * atoms + (D::K + D::V) * q8p::kKeys * 128 * atoms + 2 * D::P * q8p::kRows * 128 + q8p::kTailBytes + 1024;
+    static_assert(smem <= 227 * 1024, "one CTA's shared memory");
     static SmemOptIn optin;
     if (optin.needs((size_t)smem)) {
         // setmaxnreg moves registers between the warpgroups within what the block was launched with: it must be all of 128 a thread
         cudaFuncAttributes attr;
         cudaError_t e = cudaFuncGetAttributes(&attr, prefill_q8_kernel<HD, KV>);
         if (e != cudaSuccess) return fail(NS_ERR_CUDA, "prefill_q8: cannot query the kernel: %s", cudaGetErrorString(e));
-        if (attr.numRegs * q8p::kThreads < (q8p::kRegsSoftmax + q8p::kRegsOther) * 128) return NS_ERR_UNSUPPORTED;
+        if (attr.numRegs * q8p::kThreads < 2 * (q8p::kRegsSoftmax + q8p::kRegsOther) * 128) return NS_ERR_UNSUPPORTED;
         e = cudaFuncSetAttribute(prefill_q8_kernel<HD, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return fail(NS_ERR_CUDA, "prefill_q8: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
         optin.done((size_t)smem);
