@@ -350,7 +350,7 @@ int ns_kv_values(const void* pool, const float* scale, void* out, int64_t num_bl
  * count as absent. A query that sees no key gets zeros; rows of no sequence are left as they were.
  * Sequences of one token need no plan; a call with cu_seqlens takes its prefill tiles from the plan in the workspace
  * (ns_attn_plan with the same seq_lens / cu_seqlens / table_rows). workspace as in ns_ragged_paged_attn; calls
- * that share one must not overlap. Tensor-core kernels: block_size a multiple of 16 (prefill chunks: 16), head_dim 64 / 128,
+ * that share one must not overlap. Tensor-core kernels: block_size a power of two from 16, head_dim 64 / 128,
  * 16-byte aligned pools; everything else runs ns_ragged_paged_attn_q8_simple, which needs no workspace (head_dim <= 256).
  * Replaces, for 8-bit pools: nanoserve/model.py:262-323 _attend and nanoserve/kernels/paged_attention.py:85-105. */
 int ns_ragged_paged_attn_q8(const void* q, const void* k_pool, const void* v_pool, const float* k_scale, const float* v_scale,

@@ -34,6 +34,7 @@ static int fill_params(Q8Params& p, const void* q, const void* k_pool, const voi
     p.sc_blk_stride = scale_block_stride; p.sc_head_stride = scale_head_stride;
     p.n_seqs = n_seqs; p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.group = n_heads / n_kv_heads; p.head_dim = head_dim;
     p.block_size = block_size; p.num_blocks = num_blocks; p.table_width = table_width;
+    p.block_shift = (block_size & (block_size - 1)) == 0 ? 31 - __builtin_clz((unsigned)block_size) : -1;
     p.scale = scale; p.scale_log2 = scale * 1.4426950408889634f;
     return NS_OK;
 }

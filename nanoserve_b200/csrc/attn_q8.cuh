@@ -18,6 +18,7 @@ struct Q8Params {
     WsLayout L;
     int64_t n_tokens, table_stride, q_stride, out_stride, blk_stride, pos_stride, head_stride, sc_blk_stride, sc_head_stride;
     int n_seqs, n_heads, n_kv_heads, group, head_dim, block_size, num_blocks, table_width;
+    int block_shift;                 // log2(block_size) where that is a power of two, else -1 (scalar kernel only)
     float scale, scale_log2;         // softmax scale, and times log2(e)
     int only_prefill;                // 1: sequences of one token are another launch's
     int overlap_prefill;             // 1: the prefill kernel runs beside the decode kernel launched just before it

@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
                 id_base = base;
                 const int j = base + lane;
                 id = -1;
-                if (j < j1) id = table[j * 16 / p.block_size];
+                if (j < j1) id = table[j * 16 >> p.block_shift];
                 if ((unsigned)id >= (unsigned)p.num_blocks) id = -1;
                 sk = id >= 0 ? ksc[(int64_t)id * p.sc_blk_stride] : 0.f;
                 float sv = id >= 0 ? vsc[(int64_t)id * p.sc_blk_stride] : 1.f;
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
                 T.lv = __shfl_sync(0xffffffffu, lv, src);
                 T.isv = __shfl_sync(0xffffffffu, isv, src);
                 T.valid = blk >= 0 ? min(16, len - 16 * j) : 0;
-                const int64_t off = (int64_t)max(blk, 0) * p.blk_stride + (int64_t)((j * 16) % p.block_size) * p.pos_stride;
+                const int64_t off = (int64_t)max(blk, 0) * p.blk_stride + (int64_t)((j * 16) & (p.block_size - 1)) * p.pos_stride;
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
 bool q8_decode_supported(const Q8Params& p, int dtype) {
     const int64_t qa = dtype == NS_F32 ? 4 : 8;
     if (p.head_dim != 64 && p.head_dim != 128) return false;
-    if (p.block_size % 16 != 0) return false;
+    if (p.block_size < 16 || p.block_shift < 0) return false;
     if (((uintptr_t)p.k_pool | (uintptr_t)p.v_pool | (uintptr_t)p.q) & 15) return false;
     if (((uintptr_t)p.out & (dtype == NS_F32 ? 15 : 7)) || p.out_stride % 4 || p.q_stride % qa) return false;
     if (p.blk_stride % 16 || p.pos_stride % 16 || p.head_stride % 16) return false;

@@ -50,7 +50,14 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ void st_shared16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+    // (no memory clobber: only the fence before the barrier arrival orders these stores, and loads may move across them)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d));
+}
+// Every lane's generic-proxy stores become visible to the tensor cores, then one arrival for the warp.
+__device__ __forceinline__ void warp_arrive(uint32_t mbar_saddr) {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(mbar_saddr);
 }
 // Named barriers 1 and 2: a tile's softmax threads and its issuing warp meet once, when Q is in place.
 __device__ __forceinline__ void q_ready_barrier(int tile) { asm volatile("bar.sync %0, %1;" ::"r"(1 + tile), "r"(kRows + 32) : "memory"); }
@@ -123,8 +130,8 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
 #pragma unroll
         for (int i = 0; i < D::Bars; ++i) {
             // K and V free: one commit per Q tile that read them
-            const uint32_t count = i >= D::BarScale ? (kNanCodes ? kConvWarps : 1) : i >= D::BarKFree ? n_q : i >= D::BarKFull ? kConv
-                                   : i >= D::BarPReady ? kRows : 1;
+            const uint32_t count = i >= D::BarScale ? (kNanCodes ? kConvWarps : 4) : i >= D::BarKFree ? n_q : i >= D::BarVFull ? kConvWarps : i >= D::BarKFull ? 4
+                                   : i >= D::BarPReady ? kRows / 32 : 1;
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar(i)), "r"(count) : "memory");
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -189,125 +196,149 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
                 if (!ok) abort_flag = 1;
             }
         } else {
-            // ---- converting warps. An item is 32 consecutive 16-code pieces of a tile: ROWS rows of it.
-            constexpr int CPR = HD / 16, ROWS = 32 / CPR, ITEMS = kKeys / ROWS, MINE = (ITEMS + kConvWarps - 1) / kConvWarps;
+            // ---- converting warps. A piece is 16 codes of a row (one lane), an item 32 consecutive pieces: ROWS rows of one block. The
+            // first four warps take a block of the tile each: its K items and its last V item; the other two the remaining V
+            // items of two blocks each. A warp's addresses are then a base per block and constant steps: what bounds these warps is
+            // the number of their instructions (they share the issue slots with the softmax).
+            constexpr int CPR = HD / 16, ROWS = 32 / CPR, PER = 16 / ROWS;       // pieces per row, rows per item, items per block
             const int cw = warp - 10, row_in = lane / CPR, piece = lane % CPR;
-            const uint8_t* kb = p.k_pool + g * p.head_stride + piece * 16;
-            const uint8_t* vb = p.v_pool + g * p.head_stride + piece * 16;
-            uint4 kr[MINE], vr[MINE];
-            // lane b & 3: where keys 16 b .. 16 b + 15 of the tile start in a pool, and their block; -1: absent
-            auto fetch_ids = [&](int kt, int64_t& off) -> int {
-                const int key = kt * kKeys + 16 * (lane & 3);
-                off = 0;
-                if (kt >= n_tiles || key >= kv_end) return -1;
-                const int b = key / p.block_size, id = table[b];
-                off = (int64_t)id * p.blk_stride + (int64_t)(key - b * p.block_size) * p.pos_stride;
-                return (unsigned)id < (unsigned)p.num_blocks ? id : -1;
-            };
-            auto item_at = [&](int n, bool v) -> int { const int i = (v ? kConvWarps - 1 - cw : cw) + kConvWarps * n; return i < ITEMS ? i : -1; };
-            // ROWS divides 16: an item lies inside one block
-            const int64_t lane_off = row_in * p.pos_stride, item_step = ROWS * p.pos_stride;
-            auto load_item = [&](int kt, int i, int id_all, int64_t off_all, const uint8_t* pool) -> uint4 {
-                const int b = i * ROWS >> 4;
-                const int id = __shfl_sync(0xffffffffu, id_all, b);
-                const int64_t off = __shfl_sync(0xffffffffu, off_all, b);
-                if (id < 0 || kt * kKeys + i * ROWS + row_in >= len) return make_uint4(0u, 0u, 0u, 0u);
-                return __ldcg(reinterpret_cast<const uint4*>(pool + off + lane_off + (i & (16 / ROWS - 1)) * item_step));
-            };
+            const bool k_warp = cw < 4;
+            const int b0 = k_warp ? cw : 2 * (cw - 4);                           // this warp's (first) block
+            constexpr int NV = 2 * (PER - 1);                                    // V items of a warp, at most
+            const uint8_t* kb = p.k_pool + g * p.head_stride + piece * 16 + row_in * p.pos_stride;
+            const uint8_t* vb = p.v_pool + g * p.head_stride + piece * 16 + row_in * p.pos_stride;
+            const int64_t step = ROWS * p.pos_stride;
             const uint32_t piece_off = (uint32_t)((piece >> 2) * (kKeys * 128) + row_in * 128), chunk0 = (uint32_t)((piece & 3) * 2);
-            auto store_item = [&](uint32_t tile, int i, const uint4& w) {      // 16 codes -> two 16-byte pieces of f16
-                const uint32_t dst = tile + piece_off + i * (ROWS * 128), r7 = (uint32_t)((i * ROWS + row_in) & 7);
-                uint32_t a, b, c, d;
-                q8::expand<KV>(w.x, a, b);
-                q8::expand<KV>(w.y, c, d);
-                st_shared16(dst + ((chunk0 ^ r7) << 4), a, b, c, d);
-                q8::expand<KV>(w.z, a, b);
-                q8::expand<KV>(w.w, c, d);
-                st_shared16(dst + (((chunk0 + 1) ^ r7) << 4), a, b, c, d);
+            uint4 kr[PER], vr[NV];
+            // the table entry of keys 16 b .. of a tile, -1 past the last visible key; it is requested a whole tile before it is looked at
+            auto fetch_raw = [&](int kt, int b) -> int {
+                const int key = kt * kKeys + 16 * b;
+                return kt < n_tiles && key < kv_end ? table[key >> p.block_shift] : -1;
             };
-            auto write_scales = [&](int kt, float sk, float sv, int id) {      // lanes 0..3 of the first converting warp
-                sv = sv < kMinScale ? kMinScale : sv;
-                float* e = scale_ring + (kt % kScaleRing) * 12 + lane;
-                e[0] = id >= 0 ? sk : 0.f;
-                e[4] = id >= 0 ? log2f(sv) : -INFINITY;
-                e[8] = id >= 0 ? 1.f / sv : 0.f;
+            auto locate = [&](int kt, int b, int& raw) -> int64_t {              // offset of the block's first key in a pool; raw -1: absent
+                int64_t off = (int64_t)raw * p.blk_stride;
+                if (p.block_size != 16) off += (int64_t)((kt * kKeys + 16 * b) & (p.block_size - 1)) * p.pos_stride;
+                if ((unsigned)raw >= (unsigned)p.num_blocks) raw = -1;
+                return off;
             };
-            int64_t off, off_next, off_after;
-            int ids = fetch_ids(0, off);
+            // items n0 .. of a block into r: a block that is there and full takes plain loads (the usual case, and warp-uniform)
+            auto load_items = [&](const uint8_t* pool, int64_t off, int id, int kt, int b, int n0, auto count, uint4* r) {
+                const uint8_t* src = pool + off;
+                const int left = len - (kt * kKeys + 16 * b);                    // keys of the block
+                if (id >= 0 && left >= 16) {
+#pragma unroll
+                    for (int n = 0; n < decltype(count)::value; ++n) r[n] = __ldcg(reinterpret_cast<const uint4*>(src + (n0 + n) * step));
+                } else {
+#pragma unroll
+                    for (int n = 0; n < decltype(count)::value; ++n)
+                        r[n] = id >= 0 && (n0 + n) * ROWS + row_in < left ? __ldcg(reinterpret_cast<const uint4*>(src + (n0 + n) * step))
+                                                                         : make_uint4(0u, 0u, 0u, 0u);
+                }
+            };
+            auto store_item = [&](uint32_t tile, int b, int n, const uint4& w) { // 16 codes -> two 16-byte pieces of f16
+                const uint32_t dst = tile + piece_off + b * (16 * 128) + n * (ROWS * 128), r7 = (uint32_t)((n * ROWS + row_in) & 7);
+                uint32_t x, y, z, u;
+                q8::expand<KV>(w.x, x, y);
+                q8::expand<KV>(w.y, z, u);
+                st_shared16(dst + ((chunk0 ^ r7) << 4), x, y, z, u);
+                q8::expand<KV>(w.z, x, y);
+                q8::expand<KV>(w.w, z, u);
+                st_shared16(dst + (((chunk0 + 1) ^ r7) << 4), x, y, z, u);
+            };
+            // V item m of this warp: block and item inside it
+            auto v_block = [&](int m) -> int { return k_warp ? b0 : b0 + m / (PER - 1); };
+            auto v_item = [&](int m) -> int { return k_warp ? PER - 1 : m % (PER - 1); };
+            const int n_v = k_warp ? 1 : NV;
+            int id0 = fetch_raw(0, b0), id1 = k_warp ? -1 : fetch_raw(0, b0 + 1);
+            int raw0 = fetch_raw(1, b0), raw1 = k_warp ? -1 : fetch_raw(1, b0 + 1);
             float sk = 0.f, sv = 1.f;
-            auto load_scales = [&](int id) {
-                if (cw == 0 && lane < 4 && id >= 0) {
-                    const int64_t o = (int64_t)id * p.sc_blk_stride + (int64_t)g * p.sc_head_stride;
+            using std::integral_constant;
+            auto load_tile_k = [&](int kt, int64_t off0) { load_items(kb, off0, id0, kt, b0, 0, integral_constant<int, PER>(), kr); };
+            auto load_tile_v = [&](int kt, int64_t off0, int64_t off1) {
+                if (k_warp) {
+                    load_items(vb, off0, id0, kt, b0, PER - 1, integral_constant<int, 1>(), vr);
+                } else {
+                    load_items(vb, off0, id0, kt, b0, 0, integral_constant<int, PER - 1>(), vr);
+                    load_items(vb, off1, id1, kt, b0 + 1, 0, integral_constant<int, PER - 1>(), vr + PER - 1);
+                }
+            };
+            auto load_scales = [&]() {
+                if (k_warp && id0 >= 0) {
+                    const int64_t o = (int64_t)id0 * p.sc_blk_stride + (int64_t)g * p.sc_head_stride;
                     sk = p.k_scale[o];
                     sv = p.v_scale[o];
                 }
             };
-            load_scales(ids);
-#pragma unroll
-            for (int n = 0; n < MINE; ++n) {
-                const int ik = item_at(n, false), iv = item_at(n, true);
-                if (n_tiles > 0 && ik >= 0) kr[n] = load_item(0, ik, ids, off, kb);
-                if (n_tiles > 0 && iv >= 0) vr[n] = load_item(0, iv, ids, off, vb);
+            {
+                const int64_t off0 = locate(0, b0, id0), off1 = locate(0, b0 + 1, id1);
+                if (n_tiles > 0) {
+                    if (k_warp) load_tile_k(0, off0);
+                    load_tile_v(0, off0, off1);
+                    load_scales();
+                }
             }
-            int ids_next = fetch_ids(1, off_next);
             for (int kt = 0; kt < n_tiles; ++kt) {
                 const int st_k = kt % kStagesK, st_v = kt % kStagesV;
-                const int ids_after = fetch_ids(kt + 2, off_after);
-                if (kt >= kStagesK)
-                    ok = mbar_wait_or_abort(bar(D::BarKFree + st_k), (uint32_t)((kt / kStagesK - 1) & 1), tail_words + 1);
+                const int here = id0;                                            // this tile's block (scales)
+                int64_t off0 = 0, off1 = 0;
+                if (k_warp) {
+                    if (kt >= kStagesK)
+                        ok = mbar_wait_or_abort(bar(D::BarKFree + st_k), (uint32_t)((kt / kStagesK - 1) & 1), tail_words + 1);
+                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+#pragma unroll
+                    for (int n = 0; n < PER; ++n) store_item(sK + st_k * KV_BYTES, b0, n, kr[n]);
+                    warp_arrive(bar(D::BarKFull + st_k));
+                    // scales of the block: log2 and reciprocal by the approximate instructions (2^-22, far below P's 11 bits)
+                    const float svf = sv < kMinScale ? kMinScale : sv;
+                    if (lane == 0) {
+                        float* e = scale_ring + (kt % kScaleRing) * 12 + b0;
+                        e[0] = here >= 0 ? sk : 0.f;
+                        e[4] = here >= 0 ? __log2f(svf) : -INFINITY;
+                        e[8] = here >= 0 ? __fdividef(1.f, svf) : 0.f;
+                    }
+                }
+                id0 = raw0;
+                id1 = raw1;
+                off0 = locate(kt + 1, b0, id0);
+                off1 = locate(kt + 1, b0 + 1, id1);
+                raw0 = fetch_raw(kt + 2, b0);
+                raw1 = k_warp ? -1 : fetch_raw(kt + 2, b0 + 1);
+                if (k_warp) {
+                    load_tile_k(kt + 1, off0);
+                    load_scales();
+                }
+                if (kt >= kStagesV)
+                    ok = mbar_wait_or_abort(bar(D::BarVFree + st_v), (uint32_t)((kt / kStagesV - 1) & 1), tail_words + 1);
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 if (kNanCodes) {
-                    uint64_t keys = 0;
+                    auto nan_of = [](uint32_t w) -> uint32_t { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };   // bit 7 of a NaN byte
+                    uint32_t any = 0;
 #pragma unroll
-                    for (int n = 0; n < MINE; ++n) {
-                        const int i = item_at(n, true);
-                        if (i < 0) continue;
-                        auto nan_of = [](uint32_t w) -> uint32_t { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };   // bit 7 of a NaN byte
-                        const uint32_t fx = nan_of(vr[n].x), fy = nan_of(vr[n].y), fz = nan_of(vr[n].z), fw = nan_of(vr[n].w);
-                        const uint32_t lanes = __ballot_sync(0xffffffffu, (fx | fy | fz | fw) != 0);
-                        if (lanes != 0) {
-                            vr[n].x &= ~((fx >> 7) * 0xffu);
-                            vr[n].y &= ~((fy >> 7) * 0xffu);
-                            vr[n].z &= ~((fz >> 7) * 0xffu);
-                            vr[n].w &= ~((fw >> 7) * 0xffu);
+                    for (int m = 0; m < NV; ++m)
+                        if (m < n_v) any |= nan_of(vr[m].x) | nan_of(vr[m].y) | nan_of(vr[m].z) | nan_of(vr[m].w);
+                    uint64_t keys = 0;
+                    if (__any_sync(0xffffffffu, any != 0)) {
+#pragma unroll
+                        for (int m = 0; m < NV; ++m) {
+                            if (m >= n_v) continue;
+                            const uint32_t fx = nan_of(vr[m].x), fy = nan_of(vr[m].y), fz = nan_of(vr[m].z), fw = nan_of(vr[m].w);
+                            const uint32_t lanes = __ballot_sync(0xffffffffu, (fx | fy | fz | fw) != 0);
+                            vr[m].x &= ~((fx >> 7) * 0xffu);
+                            vr[m].y &= ~((fy >> 7) * 0xffu);
+                            vr[m].z &= ~((fz >> 7) * 0xffu);
+                            vr[m].w &= ~((fw >> 7) * 0xffu);
                             for (int r = 0; r < ROWS; ++r)
-                                if ((lanes >> (r * CPR)) & ((1u << CPR) - 1u)) keys |= 1ull << (i * ROWS + r);
+                                if ((lanes >> (r * CPR)) & ((1u << CPR) - 1u)) keys |= 1ull << (16 * v_block(m) + v_item(m) * ROWS + r);
                         }
                     }
                     if (lane == 0) nan_ring[(kt % kScaleRing) * kConvWarps + cw] = keys;
                 }
-                if (cw == 0 && lane < 4) write_scales(kt, sk, sv, ids);
-                if (cw == 0 || kNanCodes) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(bar(D::BarScale + kt % kScaleRing));
-                }
+                if (lane == 0 && (k_warp || kNanCodes)) mbar_arrive(bar(D::BarScale + kt % kScaleRing));
 #pragma unroll
-                for (int n = 0; n < MINE; ++n) {
-                    const int i = item_at(n, false);
-                    if (i >= 0) {
-                        store_item(sK + st_k * KV_BYTES, i, kr[n]);
-                        if (kt + 1 < n_tiles) kr[n] = load_item(kt + 1, i, ids_next, off_next, kb);
-                    }
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(bar(D::BarKFull + st_k));
-                if (kt >= kStagesV)
-                    ok = mbar_wait_or_abort(bar(D::BarVFree + st_v), (uint32_t)((kt / kStagesV - 1) & 1), tail_words + 1);
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-#pragma unroll
-                for (int n = 0; n < MINE; ++n) {
-                    const int i = item_at(n, true);
-                    if (i >= 0) {
-                        store_item(sV + st_v * KV_BYTES, i, vr[n]);
-                        if (kt + 1 < n_tiles) vr[n] = load_item(kt + 1, i, ids_next, off_next, vb);
-                    }
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(bar(D::BarVFull + st_v));
-                ids = ids_next;
-                ids_next = ids_after;
-                off_next = off_after;
-                load_scales(ids);
+                for (int m = 0; m < NV; ++m)
+                    if (m < n_v) store_item(sV + st_v * KV_BYTES, v_block(m), v_item(m), vr[m]);
+                warp_arrive(bar(D::BarVFull + st_v));
+                load_tile_v(kt + 1, off0, off1);
             }
             if (!ok) abort_flag = 1;
         }
@@ -459,10 +490,9 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
                     st_shared16(p_dst + (((4 * hf + c) ^ (row & 7)) << 4), pack_f16x2(v[8 * c + 0], v[8 * c + 1]), pack_f16x2(v[8 * c + 2], v[8 * c + 3]),
                                 pack_f16x2(v[8 * c + 4], v[8 * c + 5]), pack_f16x2(v[8 * c + 6], v[8 * c + 7]));
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (!ok) break;
-            mbar_arrive(bar(D::BarPReady + 2 * w + (kt & 1)));
+            warp_arrive(bar(D::BarPReady + 2 * w + (kt & 1)));
         }
         if (!ok) abort_flag = 1;
         // ---- the row's output: after the last PV, 32 columns at a time
