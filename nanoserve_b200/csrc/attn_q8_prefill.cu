@@ -53,6 +53,12 @@ __device__ __forceinline__ void st_shared16(uint32_t dst, uint32_t a, uint32_t b
     // (no memory clobber: only the fence before the barrier arrival orders these stores, and loads may move across them)
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d));
 }
+// Largest of three (NaN operands are passed over, as by fmaxf).
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 // Every lane's generic-proxy stores become visible to the tensor cores, then one arrival for the warp.
 __device__ __forceinline__ void warp_arrive(uint32_t mbar_saddr) {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -383,15 +389,11 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
         float m_run = -INFINITY, l_run = 0.f;
         const int my_tiles = w < n_q ? n_tiles : 0;
         for (int kt = 0; kt < my_tiles; ++kt) {
-            // (a warp gives up as a whole: its tensor-memory accesses and votes are warp-wide)
-            ok = __all_sync(0xffffffffu, mbar_wait_or_abort(bar(D::BarScale + kt % kScaleRing), (uint32_t)((kt / kScaleRing) & 1), abort_now) && !*abort_now);
-            if (!ok) break;
-            const float* ring = scale_ring + (kt % kScaleRing) * 12;
-            const float4 sk4 = *reinterpret_cast<const float4*>(ring), lv4 = *reinterpret_cast<const float4*>(ring + 4),
-                         iv4 = *reinterpret_cast<const float4*>(ring + 8);
-            const float fac[4] = {f_row * sk4.x, f_row * sk4.y, f_row * sk4.z, f_row * sk4.w};
-            const float lv[4] = {lv4.x, lv4.y, lv4.z, lv4.w}, isv[4] = {iv4.x, iv4.y, iv4.z, iv4.w};
-            ok = __all_sync(0xffffffffu, mbar_wait_or_abort(bar(D::BarS + 2 * w + (kt & 1)), (uint32_t)((kt >> 1) & 1), abort_now));
+            // The scales of tile kt were written before its S was issued: their barrier is only looked at. (A warp gives up as a whole:
+            // its tensor-memory accesses and votes are warp-wide.)
+            ok = mbar_wait_or_abort(bar(D::BarS + 2 * w + (kt & 1)), (uint32_t)((kt >> 1) & 1), abort_now) &&
+                 mbar_wait_or_abort(bar(D::BarScale + kt % kScaleRing), (uint32_t)((kt / kScaleRing) & 1), abort_now);
+            ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t s_src = t_lane + (uint32_t)((kt & 1) * kKeys);
@@ -400,6 +402,11 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
             uint32_t sr[2][32];
             tmem_ld32_issue(s_src, sr[0]);
             tmem_ld32_issue(s_src + 32, sr[1]);
+            const float* ring = scale_ring + (kt % kScaleRing) * 12;
+            const float4 sk4 = *reinterpret_cast<const float4*>(ring), lv4 = *reinterpret_cast<const float4*>(ring + 4),
+                         iv4 = *reinterpret_cast<const float4*>(ring + 8);
+            const float fac[4] = {f_row * sk4.x, f_row * sk4.y, f_row * sk4.z, f_row * sk4.w};
+            const float lv[4] = {lv4.x, lv4.y, lv4.z, lv4.w}, isv[4] = {iv4.x, iv4.y, iv4.z, iv4.w};
             tmem_ld_wait();
             // x = s * factor + log2(sv), two at a time
 #pragma unroll
@@ -437,7 +444,8 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-                for (int i = 0; i < 32; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], __uint_as_float(sr[hf][i]));
+                for (int i = 0; i < 32; i += 2)
+                    mx4[(i >> 1) & 3] = max3(mx4[(i >> 1) & 3], __uint_as_float(sr[hf][i]), __uint_as_float(sr[hf][i + 1]));
             const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
             const bool move = __any_sync(0xffffffffu, mx > m_run + kLazy);
             if (move && kt > 0) {                                          // the output is rewritten: PV(kt - 1) has to be over
