@@ -59,8 +59,6 @@ template <int HD> struct Tile {
     static constexpr int KW = HD / 64, VW = HD / 32;        // 16-byte pieces per K row, words per V row
     uint4 k[2][KW];
     uint32_t v[4][VW];
-    float sk, lv, isv;
-    int valid;
 };
 
 // Streaming loads past L1: every byte is used once. (Not the read-only path: with programmatic launches the kernel before
@@ -76,80 +74,80 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
     constexpr int NW = Cfg<HD>::kWarps, D = Cfg<HD>::kDepth, KW = HD / 64, VW = HD / 32, RS = HD + 4, THREADS = NW * 32;
     constexpr int QN = F32 ? 2 : 1;                          // f16 terms of q and of P
     extern __shared__ __align__(16) uint8_t smem_q8[];
-    float* const slots = reinterpret_cast<float*>(smem_q8);              // [NW][2][8][RS]
-    int* const prefix = reinterpret_cast<int*>(slots + NW * 2 * 8 * RS); // [n_rows + 1] tiles (per unit of the row) before row r
+    float* const slots = reinterpret_cast<float*>(smem_q8);              // [NW][2][8][RS] pieces of units
+    float4* const tile_info = reinterpret_cast<float4*>(slots + NW * 2 * 8 * RS);   // [NW][2][32] {sk, log2 sv, 1 / sv, present}
+    int* const prefix = reinterpret_cast<int*>(tile_info + NW * 64);     // [n_rows + 1] tiles (per unit of the row) before row r
     int* const row_len = prefix + n_rows + 1;                            // keys; -1: not a decode row
     int* const row_tab = row_len + n_rows;
-    __shared__ int warp_sum_sm[NW + 1];
-    __shared__ int cuts[2];
-    __shared__ int4 chain[2 * NW];         // pieces of one unit in this CTA: {row, vhead, first warp | slot << 8 | last warp << 16, kind}
-    __shared__ int join_of[2];             // chain index of a unit this CTA is the last to deliver, by piece: head, tail
-    __shared__ float join_w[8][2];         // not used by the main loop: per head {max, 1 / sum} of a join
+    __shared__ int warp_total[NW], has_empty, n_chain, n_open;
+    __shared__ int4 chain[2 * NW];         // units with pieces in this CTA: {row, vhead, first warp | slot << 8 | last warp << 16, kind}
+    __shared__ int4 open_unit[2];          // units over several CTAs: [0] began in an earlier one, [1] begins here {row, vhead, first CTA, parts}
+    __shared__ int open_last[2];
 
     // A mixed call's prefill kernel, launched next, does not wait for this one (it reads the same inputs and writes other rows):
     // it may start only once the inputs exist, that is after this kernel's own wait.
     if (!p.overlap_prefill) pdl_launch_dependents();
-    pdl_wait();
-    if (p.overlap_prefill) pdl_launch_dependents();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int G = gridDim.x, cta = blockIdx.x;
     const int sub = (p.group + 7) >> 3, VH = p.n_kv_heads * sub;
+    if (tid == 0) has_empty = n_chain = n_open = 0;
+    if (tid < 2) {
+        open_unit[tid].w = 0;
+        open_last[tid] = 0;
+    }
+    pdl_wait();
+    if (p.overlap_prefill) pdl_launch_dependents();
 
     // ---- tiles before each row
-    {
-        int total = 0;
-        for (int base = 0; base < n_rows; base += THREADS) {
-            const int r = base + tid, s = s_begin + r;
-            int nt = 0;
-            if (r < n_rows) {
-                int T = 1, q0 = s;
-                if (p.cu_seqlens != nullptr) {
-                    q0 = p.cu_seqlens[s];
-                    T = p.cu_seqlens[s + 1] - q0;
-                }
-                const int len = (T == 1 && q0 >= 0 && q0 < p.n_tokens) ? q8_len(p, s) : -1;
-                nt = len > 0 ? (len + 15) >> 4 : 0;
-                row_len[r] = len;
-                row_tab[r] = p.table_rows != nullptr ? p.table_rows[s] : s;
+    int total = 0;
+    for (int base = 0; base < n_rows; base += THREADS) {
+        const int r = base + tid, s = s_begin + r;
+        int nt = 0, len = -1;
+        if (r < n_rows) {
+            int T = 1, q0 = s;
+            if (p.cu_seqlens != nullptr) {
+                q0 = p.cu_seqlens[s];
+                T = p.cu_seqlens[s + 1] - q0;
             }
-            int inc = nt;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int n = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += n;
-            }
-            if (lane == 31) warp_sum_sm[warp] = inc;
-            __syncthreads();
-            if (warp == 0) {
-                int v = lane < NW ? warp_sum_sm[lane] : 0, w = v;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int n = __shfl_up_sync(0xffffffffu, w, o);
-                    if (lane >= o) w += n;
-                }
-                if (lane < NW) warp_sum_sm[lane] = w - v;
-                if (lane == NW - 1) warp_sum_sm[NW] = w;
-            }
-            __syncthreads();
-            if (r < n_rows) prefix[r] = total + warp_sum_sm[warp] + inc - nt;
-            total += warp_sum_sm[NW];
-            __syncthreads();
+            const int tab = p.table_rows != nullptr ? p.table_rows[s] : s;
+            len = q8_len(p, s);
+            if (T != 1 || q0 < 0 || q0 >= p.n_tokens) len = -1;
+            nt = len > 0 ? (len + 15) >> 4 : 0;
+            row_len[r] = len;
+            row_tab[r] = tab;
         }
-        if (tid == 0) prefix[n_rows] = total;
-        if (tid < 2 * NW) chain[tid].w = 0;
-        if (tid < 2) join_of[tid] = -1;
+        int inc = nt;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int n = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += n;
+        }
+        if (base > 0) __syncthreads();                    // warp_total has been read
+        if (lane == 31) warp_total[warp] = inc;
+        __syncthreads();
+        int before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const int v = warp_total[w];
+            before += w < warp ? v : 0;
+            all += v;
+        }
+        if (r < n_rows) prefix[r] = total + before + inc - nt;
+        if (len == 0) has_empty = 1;
+        total += all;
     }
+    if (tid == 0) prefix[n_rows] = total;
     __syncthreads();
-    const int W = prefix[n_rows] * VH;
-    // rows without keys: zeros
-    for (int r = cta; r < n_rows; r += G)
-        if (row_len[r] == 0) {
-            const int64_t q0 = p.cu_seqlens != nullptr ? p.cu_seqlens[s_begin + r] : s_begin + r;
-            for (int e = tid; e < p.n_heads * HD; e += THREADS) {
-                if (F32) reinterpret_cast<float*>(p.out)[q0 * p.out_stride + e] = 0.f;
-                else reinterpret_cast<__nv_bfloat16*>(p.out)[q0 * p.out_stride + e] = __float2bfloat16_rn(0.f);
+    const int W = total * VH;
+    if (has_empty)                                        // rows without keys: zeros
+        for (int r = cta; r < n_rows; r += G)
+            if (row_len[r] == 0) {
+                const int64_t q0 = p.cu_seqlens != nullptr ? p.cu_seqlens[s_begin + r] : s_begin + r;
+                for (int e = tid; e < p.n_heads * HD; e += THREADS) {
+                    if (F32) reinterpret_cast<float*>(p.out)[q0 * p.out_stride + e] = 0.f;
+                    else reinterpret_cast<__nv_bfloat16*>(p.out)[q0 * p.out_stride + e] = __float2bfloat16_rn(0.f);
+                }
             }
-        }
     if (W == 0) return;
     // row that holds tile x of the list: the last r with prefix[r] * VH <= x (empty rows share their successor's prefix)
     auto row_of = [&](int x) -> int {
@@ -160,31 +158,34 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
         }
         return lo;
     };
-    const int per = max((W + G - 1) / G, min_tiles);
-    if (tid < 2) {
-        const long long want = (long long)(cta + tid) * per;
+    // First tile of CTA c: an even cut, moved onto the end or the start of a unit that is near (no cross-CTA join then).
+    const int per = max((W + G - 1) / G, min_tiles), slack = per >> 2;
+    auto cta_cut = [&](int c) -> int {
+        const long long want = (long long)c * per;
         int x = want >= W ? W : (int)want;
         if (x > 0 && x < W) {
             const int r = row_of(x), nt = prefix[r + 1] - prefix[r], start = prefix[r] * VH;
-            const int lo = start + (x - start) / nt * nt, hi = lo + nt, slack = per >> 2;
+            const int lo = start + (int)((unsigned)(x - start) / (unsigned)nt) * nt, hi = lo + nt;
             if (x - lo <= hi - x) {
                 if (x - lo <= slack) x = lo;
             } else if (hi - x <= slack) {
                 x = hi;
             }
         }
-        cuts[tid] = x;
-    }
-    __syncthreads();
-    const int c0 = cuts[0], c1 = cuts[1], n_mine = c1 - c0;
+        return x;
+    };
+    int c0 = cta_cut(cta + (lane & 1));                   // every warp for itself: lane 0 the CTA's first tile, lane 1 the next CTA's
+    const int c1 = __shfl_sync(0xffffffffu, c0, 1);
+    c0 = __shfl_sync(0xffffffffu, c0, 0);
+    const int n_mine = c1 - c0;
     if (n_mine <= 0) return;
-    auto warp_cut = [&](int w) -> int { return c0 + (int)((long long)n_mine * w / NW); };
+    auto warp_cut = [&](int w) -> int { return c0 + (int)((unsigned)(n_mine * w) / (unsigned)NW); };
     const int a = warp_cut(warp), b = warp_cut(warp + 1);
 
     // ---- this warp's tiles
     if (a < b) {
         int r = row_of(a), nt = prefix[r + 1] - prefix[r], us = prefix[r] * VH;
-        int vh = (a - us) / nt;
+        int vh = (int)((unsigned)(a - us) / (unsigned)nt);
         us += vh * nt;
         int x = a;
         while (x < b) {
@@ -197,38 +198,55 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
             const float* ksc = p.k_scale + kvh * p.sc_head_stride;
             const float* vsc = p.v_scale + kvh * p.sc_head_stride;
 
-            // block id and scales of 32 tiles at a time, one per lane
-            int id_base = j0, id = -1;
-            float sk = 0.f, lv = 0.f, isv = 0.f;
-            auto fetch_ids = [&](int base) {
-                id_base = base;
-                const int j = base + lane;
-                id = -1;
-                if (j < j1) id = table[j * 16 >> p.block_shift];
-                if ((unsigned)id >= (unsigned)p.num_blocks) id = -1;
+            // Q's raw rows and the first block ids are requested together; K, V and the scales follow as soon as the ids are there, and
+            // Q is converted while they travel. Lane (g, t) holds head g, dims 64 w + 16 t .. + 15, as B fragments.
+            constexpr int QV = F32 ? 4 : 2;                   // 16-byte pieces per 16 dims
+            uint4 qraw[KW * QV];
+#pragma unroll
+            for (int w = 0; w < KW; ++w)
+#pragma unroll
+                for (int c = 0; c < QV; ++c) {
+                    const int64_t o = q0 * p.q_stride + (int64_t)(kvh * p.group + h0 + min(g, heads - 1)) * HD + 64 * w + 16 * t;
+                    qraw[w * QV + c] = F32 ? *reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p.q) + o + 4 * c)
+                                           : *reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) + o + 8 * c);
+                }
+            // block ids of 32 tiles at a time, one per lane, the next 32 requested a batch ahead; their scales go to shared memory
+            auto raw_id = [&](int base) -> int { return base + lane < j1 ? table[(base + lane) * 16 >> p.block_shift] : -1; };
+            float4* const info = tile_info + warp * 64;
+            int id_base = j0, id = raw_id(j0), id_next = raw_id(j0 + 32);
+            if ((unsigned)id >= (unsigned)p.num_blocks) id = -1;
+            float sk, sv;
+            auto load_scales = [&]() {
                 sk = id >= 0 ? ksc[(int64_t)id * p.sc_blk_stride] : 0.f;
-                float sv = id >= 0 ? vsc[(int64_t)id * p.sc_blk_stride] : 1.f;
-                sv = sv < kMinScale ? kMinScale : sv;
-                lv = log2f(sv);
-                isv = 1.f / sv;
+                sv = id >= 0 ? vsc[(int64_t)id * p.sc_blk_stride] : 1.f;
             };
-            fetch_ids(j0);
+            auto put_scales = [&]() {                         // (the older batch of the two in `info` may still be read)
+                const float svf = sv < kMinScale ? kMinScale : sv;
+                info[(((id_base - j0) >> 5) & 1) * 32 + lane] = make_float4(sk, log2f(svf), 1.f / svf, id >= 0 ? 1.f : 0.f);
+                __syncwarp();
+            };
             Tile<HD> ring[D];
+            const int64_t row_k = g * p.pos_stride, row_k8 = 8 * p.pos_stride, row_v = 2 * t * p.pos_stride;
             auto load = [&](Tile<HD>& T, int j) {
-                if (j - id_base >= 32) fetch_ids(j);
-                const int src = j - id_base, blk = __shfl_sync(0xffffffffu, id, src);
-                T.sk = __shfl_sync(0xffffffffu, sk, src);
-                T.lv = __shfl_sync(0xffffffffu, lv, src);
-                T.isv = __shfl_sync(0xffffffffu, isv, src);
-                T.valid = blk >= 0 ? min(16, len - 16 * j) : 0;
-                const int64_t off = (int64_t)max(blk, 0) * p.blk_stride + (int64_t)((j * 16) & (p.block_size - 1)) * p.pos_stride;
+                if (j - id_base >= 32) {
+                    id_base = j;
+                    id = (unsigned)id_next >= (unsigned)p.num_blocks ? -1 : id_next;
+                    id_next = raw_id(j + 32);
+                    load_scales();
+                    put_scales();
+                }
+                const int blk = __shfl_sync(0xffffffffu, id, j - id_base);
+                int64_t off = (int64_t)max(blk, 0) * p.blk_stride;
+                if (p.block_size != 16) off += (int64_t)((j * 16) & (p.block_size - 1)) * p.pos_stride;
+                const uint8_t* ks = kb + off + row_k;
+                const uint8_t* vs = vb + off + row_v;
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
-                    for (int w = 0; w < KW; ++w) T.k[e][w] = ld16(kb + off + (g + 8 * e) * p.pos_stride + 64 * w);
+                    for (int w = 0; w < KW; ++w) T.k[e][w] = ld16(ks + e * row_k8 + 64 * w);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint8_t* src_v = vb + off + (2 * t + (e & 1) + 8 * (e >> 1)) * p.pos_stride;
+                    const uint8_t* src_v = vs + (e & 1) * p.pos_stride + (e >> 1) * row_k8;
                     if constexpr (HD == 64) {
                         const uint2 v = __ldcg(reinterpret_cast<const uint2*>(src_v));
                         T.v[e][0] = v.x;
@@ -245,32 +263,24 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
 #pragma unroll
             for (int d = 0; d < D; ++d)
                 if (j0 + d < j1) load(ring[d], j0 + d);
+            load_scales();
 
-            // Q: lane (g, t) holds head g, dims 64 w + 16 t .. + 15, as B fragments
             uint32_t qf[QN][4 * KW][2];
             float f0, f1;                                     // score factors of heads 2t and 2t + 1
             {
                 float qx[16 * KW];
-                float top = 0.f;
 #pragma unroll
-                for (int w = 0; w < KW; ++w) {
-                    const int64_t o = q0 * p.q_stride + (int64_t)(kvh * p.group + h0 + min(g, heads - 1)) * HD + 64 * w + 16 * t;
-                    if (F32) {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const Vec16<float> v = load16(reinterpret_cast<const float*>(p.q) + o + 4 * c);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) qx[16 * w + 4 * c + i] = v.get(i);
-                        }
+                for (int i = 0; i < 16 * KW; ++i) {
+                    if constexpr (F32) {
+                        const uint4 u = qraw[i >> 2];
+                        qx[i] = __uint_as_float((i & 3) == 0 ? u.x : (i & 3) == 1 ? u.y : (i & 3) == 2 ? u.z : u.w);
                     } else {
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const Vec16<__nv_bfloat16> v = load16(reinterpret_cast<const __nv_bfloat16*>(p.q) + o + 8 * c);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) qx[16 * w + 8 * c + i] = v.get(i);
-                        }
+                        const uint4 u = qraw[i >> 3];
+                        const uint32_t word = ((i >> 1) & 3) == 0 ? u.x : ((i >> 1) & 3) == 1 ? u.y : ((i >> 1) & 3) == 2 ? u.z : u.w;
+                        qx[i] = __uint_as_float((i & 1) ? (word & 0xffff0000u) : (word << 16));
                     }
                 }
+                float top = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16 * KW; ++i) top = fmaxf(top, fabsf(qx[i]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -295,13 +305,16 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
                 f0 = p.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * t);
                 f1 = p.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * t + 4);
             }
+            put_scales();
 
             float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
             float o[HD / 16][4];
 #pragma unroll
             for (int i = 0; i < HD / 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
 
-            auto compute = [&](Tile<HD>& T) {
+            auto compute = [&](Tile<HD>& T, int j) {
+                const float4 ti = info[(j - j0) & 63];
+                const int valid = ti.w != 0.f ? min(16, len - 16 * j) : 0;
                 float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int w = 0; w < KW; ++w) {
@@ -316,14 +329,14 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
                         for (int n = 0; n < QN; ++n) mma_f16(s, a0, a1, a2, a3, qf[n][4 * w + i][0], qf[n][4 * w + i][1]);
                     }
                 }
-                const float k0 = f0 * T.sk, k1 = f1 * T.sk;
-                float x0 = fmaf(s[0], k0, T.lv), x1 = fmaf(s[1], k1, T.lv), x2 = fmaf(s[2], k0, T.lv), x3 = fmaf(s[3], k1, T.lv);
-                if (T.valid < 16) {                           // the row's last tile, or a block that is not there
-                    if (g >= T.valid) x0 = x1 = -INFINITY;
-                    if (g + 8 >= T.valid) x2 = x3 = -INFINITY;
+                const float k0 = f0 * ti.x, k1 = f1 * ti.x;
+                float x0 = fmaf(s[0], k0, ti.y), x1 = fmaf(s[1], k1, ti.y), x2 = fmaf(s[2], k0, ti.y), x3 = fmaf(s[3], k1, ti.y);
+                if (valid < 16) {                           // the row's last tile, or a block that is not there
+                    if (g >= valid) x0 = x1 = -INFINITY;
+                    if (g + 8 >= valid) x2 = x3 = -INFINITY;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (2 * t + (e & 1) + 8 * (e >> 1) >= T.valid) {
+                        if (2 * t + (e & 1) + 8 * (e >> 1) >= valid) {
 #pragma unroll
                             for (int w = 0; w < VW; ++w) T.v[e][w] = 0u;      // 0 x NaN must not reach the sum
                         }
@@ -352,8 +365,8 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
                 }
                 const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
                 const float p0 = ex2(x0 - r0), p1 = ex2(x1 - r1), p2 = ex2(x2 - r0), p3 = ex2(x3 - r1);
-                l0 = fmaf(p0 + p2, T.isv, l0);
-                l1 = fmaf(p1 + p3, T.isv, l1);
+                l0 = fmaf(p0 + p2, ti.z, l0);
+                l1 = fmaf(p1 + p3, ti.z, l1);
                 uint32_t pb[QN][2];
                 {
                     const uint32_t u = pack_f16x2(p0, p1), v = pack_f16x2(p2, p3);
@@ -384,7 +397,7 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
 #pragma unroll
                 for (int d = 0; d < D; ++d)
                     if (j + d < j1) {
-                        compute(ring[d]);
+                        compute(ring[d], j + d);
                         if (j + d + D < j1) load(ring[d], j + d + D);
                     }
             }
@@ -425,8 +438,12 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
                     int last = warp;
                     const int end = min(us + nt, c1);
                     while (warp_cut(last + 1) < end) ++last;
-                    const int kind = us >= c0 ? (us + nt <= c1 ? 1 : 3) : 2;      // 1 whole, 2 began in an earlier CTA, 3 begins here
-                    chain[warp * 2 + slot] = make_int4(r, vh, warp | slot << 8 | last << 16, kind);
+                    const int kind = us >= c0 ? (us + nt <= c1 ? 1 : 3) : 2;      // 1 whole, 2 began in an earlier CTA, 3 begins here and ends in a later one
+                    chain[atomicAdd(&n_chain, 1)] = make_int4(r, vh, warp | slot << 8 | last << 16, kind);
+                    if (kind >= 2) {
+                        open_unit[kind - 2] = make_int4(r, vh, 0, 1);
+                        atomicAdd(&n_open, 1);
+                    }
                 }
             }
             x = us + j1;
@@ -440,147 +457,150 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
     }
     __syncthreads();
 
-    // ---- join the pieces of this CTA's warps: (unit, head) items over the warps, a lane HD / 32 columns
+    // ---- join the pieces of this CTA's warps: (unit, head) items over the warps; a lane is a piece for the weights and HD / 32
+    // columns for the sums
     constexpr int C = HD / 32;
     float* const partials = reinterpret_cast<float*>(p.ws + p.L.partials);       // [CTA][2][8][RS]
-    for (int item = warp; item < 2 * NW * 8; item += NW) {
+    for (int item = warp; item < n_chain * 8; item += NW) {
         const int4 ch = chain[item >> 3];
-        const int h = item & 7;
-        if (ch.w == 0) continue;
-        const int kvh = ch.y / sub, h0 = (ch.y - kvh * sub) * 8;
+        const int h = item & 7, kvh = ch.y / sub, h0 = (ch.y - kvh * sub) * 8;
         if (h >= min(8, p.group - h0)) continue;
         const int w0 = ch.z & 0xff, slot = (ch.z >> 8) & 0xff, w1 = ch.z >> 16;
-        auto piece = [&](int w) -> const float* { return slots + ((w * 2 + (w == w0 ? slot : 0)) * 8 + h) * RS; };
-        float m = -INFINITY;
-        for (int w = w0; w <= w1; ++w)
-            if (warp_cut(w) < warp_cut(w + 1)) m = fmaxf(m, piece(w)[HD]);
-        const float ref = m == -INFINITY ? 0.f : m;
-        float l = 0.f, acc[C];
+        const float* const piece0 = slots + ((w0 * 2 + slot) * 8 + h) * RS;      // of the first warp; the others' are their slot 0
+        auto piece = [&](int w) -> const float* { return w == w0 ? piece0 : slots + (w * 16 + h) * RS; };
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (w0 + lane <= w1 && warp_cut(w0 + lane) < warp_cut(w0 + lane + 1)) ml = *reinterpret_cast<const float2*>(piece(w0 + lane) + HD);
+        const float m = warp_max(ml.x);
+        const float wt = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+        const float l = warp_sum(ml.y == 0.f ? 0.f : wt * ml.y);
+        float acc[C];
 #pragma unroll
         for (int i = 0; i < C; ++i) acc[i] = 0.f;
+#pragma unroll 4
         for (int w = w0; w <= w1; ++w) {
-            if (warp_cut(w) >= warp_cut(w + 1)) continue;
-            const float* src = piece(w);
-            const float wt = ex2(src[HD] - ref);
-            l = fmaf(wt, src[HD + 1], l);
-#pragma unroll
-            for (int i = 0; i < C; ++i) acc[i] = fmaf(wt, src[C * lane + i], acc[i]);
+            const float f = __shfl_sync(0xffffffffu, wt, w - w0);
+            if (f == 0.f) continue;                          // (a warp without tiles, or a piece that weighs nothing)
+            const float* src = piece(w) + C * lane;
+            if constexpr (C == 4) {
+                const float4 v = *reinterpret_cast<const float4*>(src);
+                acc[0] = fmaf(f, v.x, acc[0]);
+                acc[1] = fmaf(f, v.y, acc[1]);
+                acc[2] = fmaf(f, v.z, acc[2]);
+                acc[3] = fmaf(f, v.w, acc[3]);
+            } else {
+                const float2 v = *reinterpret_cast<const float2*>(src);
+                acc[0] = fmaf(f, v.x, acc[0]);
+                acc[1] = fmaf(f, v.y, acc[1]);
+            }
         }
         if (ch.w == 1) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const int64_t q0 = p.cu_seqlens != nullptr ? p.cu_seqlens[s_begin + ch.x] : s_begin + ch.x;
             const int64_t at = q0 * p.out_stride + (int64_t)(kvh * p.group + h0 + h) * HD + C * lane;
 #pragma unroll
-            for (int i = 0; i < C; ++i) {
-                if (F32) reinterpret_cast<float*>(p.out)[at + i] = acc[i] * inv;
-                else reinterpret_cast<__nv_bfloat16*>(p.out)[at + i] = __float2bfloat16_rn(acc[i] * inv);
+            for (int i = 0; i < C; i += 2) {
+                if (F32) *reinterpret_cast<float2*>(reinterpret_cast<float*>(p.out) + at + i) = make_float2(acc[i] * inv, acc[i + 1] * inv);
+                else *reinterpret_cast<uint32_t*>(reinterpret_cast<__nv_bfloat16*>(p.out) + at + i) = pack_bf16x2(acc[i] * inv, acc[i + 1] * inv);
             }
         } else {
             float* dst = partials + ((size_t)(cta * 2 + (ch.w == 3)) * 8 + h) * RS;
 #pragma unroll
-            for (int i = 0; i < C; ++i) __stcg(dst + C * lane + i, acc[i]);
+            for (int i = 0; i < C; i += 2) __stcg(reinterpret_cast<float2*>(dst + C * lane + i), make_float2(acc[i], acc[i + 1]));
             if (lane == 0) __stcg(reinterpret_cast<float2*>(dst + HD), make_float2(m, l));
         }
     }
 
-    // ---- units over several CTAs: the last one to arrive joins the pieces in CTA order
-    bool open = false;
-    for (int k = 0; k < 2 * NW; ++k) open |= chain[k].w >= 2;
-    if (!open) return;
-    __threadfence();
+    // ---- units over several CTAs: the last one to arrive joins the pieces in CTA order. Warps 0 and 1 count the arrivals (the
+    // barrier orders the CTA's partials before them, the atomic releases them and acquires the others').
+    if (n_open == 0) return;
     __syncthreads();
     int* const counters = reinterpret_cast<int*>(p.ws + p.L.q8_counters);
-    // CTA cut c of the list, as above
-    auto cta_cut = [&](int c) -> int {
-        const long long want = (long long)c * per;
-        int x = want >= W ? W : (int)want;
-        if (x > 0 && x < W) {
-            const int r = row_of(x), nt = prefix[r + 1] - prefix[r], start = prefix[r] * VH;
-            const int lo = start + (x - start) / nt * nt, hi = lo + nt, slack = per >> 2;
-            if (x - lo <= hi - x) {
-                if (x - lo <= slack) x = lo;
-            } else if (hi - x <= slack) {
-                x = hi;
+    if (warp < 2 && open_unit[warp].w != 0) {
+        const int4 u = open_unit[warp];
+        const int nt = prefix[u.x + 1] - prefix[u.x], us = prefix[u.x] * VH + u.y * nt, ue = us + nt;
+        // CTAs that hold the unit's first and last tile: a cut moves by less than half a share, so they are among the neighbours of
+        // the even ones (lanes 0..3 try the first, 4..7 the last)
+        const int c = min((lane < 4 ? us : ue - 1) / per - 1 + (lane & 3), G);
+        const int cut = lane < 8 && c >= 0 ? cta_cut(c) : 0;
+        const unsigned first = __ballot_sync(0xffffffffu, lane < 4 && (c < 0 || cut <= us)), last = __ballot_sync(0xffffffffu, lane >= 4 && lane < 8 && (c < 0 || cut < ue));
+        const int f = us / per - 1 + __popc(first) - 1, l = (ue - 1) / per - 1 + __popc(last) - 1;
+        if (lane == 0) {
+            int before;
+            asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(&counters[f]) : "memory");
+            if (before == l - f) {
+                counters[f] = 0;
+                open_unit[warp] = make_int4(u.x, u.y, f, l - f + 1);
+                open_last[warp] = 1;
             }
-        }
-        return x;
-    };
-    __shared__ int join_span[2][2];
-    if (tid < 2 * NW && chain[tid].w >= 2) {
-        const int4 ch = chain[tid];
-        const int nt = prefix[ch.x + 1] - prefix[ch.x], us = prefix[ch.x] * VH + ch.y * nt, ue = us + nt;
-        int f = us / per, l = (ue - 1) / per;                 // CTAs of the unit's first and last tile, up to the snapping
-        f = min(f + 1, G - 1);
-        while (cta_cut(f) > us) --f;
-        l = min(l + 1, G - 1);
-        while (cta_cut(l) >= ue) --l;
-        const int k = ch.w == 3;
-        const int before = atomicAdd(&counters[f], 1);
-        if (before == l - f) {
-            counters[f] = 0;
-            join_of[k] = tid;
-            join_span[k][0] = f;
-            join_span[k][1] = l;
         }
     }
     __syncthreads();
+#pragma unroll 1
     for (int k = 0; k < 2; ++k) {
-        if (join_of[k] < 0) continue;
-        __threadfence();
-        const int4 ch = chain[join_of[k]];
-        const int f = join_span[k][0], l = join_span[k][1], parts = l - f + 1;
-        const int kvh = ch.y / sub, h0 = (ch.y - kvh * sub) * 8, heads = min(8, p.group - h0);
-        // piece i lies in CTA f + i: the first CTA's is its "begins here" piece
-        auto piece = [&](int i, int h) -> const float* { return partials + ((size_t)((f + i) * 2 + (i == 0)) * 8 + h) * RS; };
-        float* const red = slots;                             // [THREADS] float4 of column sums, then nothing else lives here
-        if (warp < heads) {
-            float m = -INFINITY;
-            for (int i = lane; i < parts; i += 32) m = fmaxf(m, __ldcg(piece(i, warp) + HD));
-            m = warp_max(m);
-            float s = 0.f;
-            for (int i = lane; i < parts; i += 32) {
-                const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece(i, warp) + HD));
-                s = fmaf(ex2(ml.x - (m == -INFINITY ? 0.f : m)), ml.y, s);
-            }
-            s = warp_sum(s);
-            if (lane == 0) {
-                join_w[warp][0] = m == -INFINITY ? 0.f : m;
-                join_w[warp][1] = s == 0.f ? 0.f : 1.f / s;
-            }
-        }
-        __syncthreads();
-        constexpr int E4 = 8 * HD / 4, GR = THREADS / E4 > 0 ? THREADS / E4 : 1;      // float4 columns; groups that share the pieces
-        static_assert(THREADS >= E4, "one float4 column per thread at least");
+        if (!open_last[k]) continue;
+        const int4 u = open_unit[k];
+        const int f = u.z, parts = u.w;
+        const int kvh = u.y / sub, h0 = (u.y - kvh * sub) * 8, heads = min(8, p.group - h0);
+        // thread = (share of the pieces, head, four columns); piece i lies in CTA f + i, the first CTA's is its "begins here" piece.
+        // Eight pieces' statistics and columns are requested at once.
+        constexpr int E4 = 8 * HD / 4, GR = THREADS / E4;
+        static_assert(GR >= 1, "one float4 column per thread at least");
         const int e = tid % E4, gr = tid / E4, h = e / (HD / 4), c4 = e % (HD / 4);
+        float m = -INFINITY, l = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (gr < GR && h < heads) {
-            const float ref = join_w[h][0];
-#pragma unroll 4
-            for (int i = gr; i < parts; i += GR) {
-                const float* src = piece(i, h);
-                const float wt = ex2(__ldcg(src + HD) - ref);
-                const float4 v = __ldcg(reinterpret_cast<const float4*>(src) + c4);
-                acc.x = fmaf(wt, v.x, acc.x);
-                acc.y = fmaf(wt, v.y, acc.y);
-                acc.z = fmaf(wt, v.z, acc.z);
-                acc.w = fmaf(wt, v.w, acc.w);
+        if (gr < GR && h < heads)
+            for (int i0 = gr; i0 < parts; i0 += 8 * GR) {
+                float2 ml[8];
+                float4 v[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int q = i0 + i * GR;
+                    const float* src = partials + ((size_t)((f + q) * 2 + (q == 0)) * 8 + h) * RS;
+                    ml[i] = q < parts ? __ldcg(reinterpret_cast<const float2*>(src + HD)) : make_float2(-INFINITY, 0.f);
+                    v[i] = q < parts ? __ldcg(reinterpret_cast<const float4*>(src) + c4) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+                float mn = m;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) mn = fmaxf(mn, ml[i].x);
+                const float ref = mn == -INFINITY ? 0.f : mn, al = ex2(m - ref);
+                m = mn;
+                l *= al;
+                acc.x *= al;
+                acc.y *= al;
+                acc.z *= al;
+                acc.w *= al;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float wt = ml[i].x == -INFINITY ? 0.f : ex2(ml[i].x - ref);
+                    l = fmaf(wt, ml[i].y, l);
+                    acc.x = fmaf(wt, v[i].x, acc.x);
+                    acc.y = fmaf(wt, v[i].y, acc.y);
+                    acc.z = fmaf(wt, v[i].z, acc.z);
+                    acc.w = fmaf(wt, v[i].w, acc.w);
+                }
             }
-        }
-        if (GR > 1) {
-            reinterpret_cast<float4*>(red)[tid] = acc;
+        if (GR > 1) {                                        // the shares meet in shared memory, in order
+            float* const red = slots;                        // [THREADS][6]: nothing else lives there any more
+            if (gr > 0) {
+                float* mine = red + tid * 6;
+                mine[0] = acc.x, mine[1] = acc.y, mine[2] = acc.z, mine[3] = acc.w, mine[4] = m, mine[5] = l;
+            }
             __syncthreads();
             if (gr == 0)
                 for (int i = 1; i < GR; ++i) {
-                    const float4 v = reinterpret_cast<float4*>(red)[tid + i * E4];
-                    acc.x += v.x;
-                    acc.y += v.y;
-                    acc.z += v.z;
-                    acc.w += v.w;
+                    const float* o = red + (tid + i * E4) * 6;
+                    const float mn = fmaxf(m, o[4]), ref = mn == -INFINITY ? 0.f : mn, wa = ex2(m - ref), wb = ex2(o[4] - ref);
+                    acc.x = acc.x * wa + o[0] * wb;
+                    acc.y = acc.y * wa + o[1] * wb;
+                    acc.z = acc.z * wa + o[2] * wb;
+                    acc.w = acc.w * wa + o[3] * wb;
+                    l = l * wa + o[5] * wb;
+                    m = mn;
                 }
         }
         if (gr == 0 && h < heads) {
-            const float inv = join_w[h][1];
-            const int64_t q0 = p.cu_seqlens != nullptr ? p.cu_seqlens[s_begin + ch.x] : s_begin + ch.x;
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const int64_t q0 = p.cu_seqlens != nullptr ? p.cu_seqlens[s_begin + u.x] : s_begin + u.x;
             const int64_t at = q0 * p.out_stride + (int64_t)(kvh * p.group + h0 + h) * HD + 4 * c4;
             if (F32) *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.out) + at) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
             else *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(p.out) + at) =
@@ -610,7 +630,7 @@ template <int HD, typename KV, bool F32> static int launch_decode_q8(const Q8Par
     if (grid > kMaxDecodeCtas) grid = kMaxDecodeCtas;
     for (int s0 = 0; s0 < p.n_seqs; s0 += q8::kMaxSeqs) {
         const int n = p.n_seqs - s0 < q8::kMaxSeqs ? p.n_seqs - s0 : q8::kMaxSeqs;
-        const size_t smem = (size_t)NW * 2 * 8 * (HD + 4) * 4 + (size_t)(3 * n + 1) * 4;
+        const size_t smem = (size_t)NW * 2 * 8 * (HD + 4) * 4 + (size_t)NW * 64 * 16 + (size_t)(3 * n + 1) * 4;
         static SmemOptIn optin;
         if (optin.needs(smem)) {
             cudaError_t e = cudaFuncSetAttribute(decode_q8_kernel<HD, KV, F32>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
