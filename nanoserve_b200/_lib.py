@@ -108,7 +108,7 @@ def load() -> ctypes.CDLL:
 def call(name: str, *args) -> None:
     """Invoke a status-returning entry point; raise with the library's message on failure."""
     global launch_count
-    lib = load()
+    lib = _lib or load()
     status = getattr(lib, name)(*args)
     launch_count += _LAUNCHES_PER_CALL.get(name, 1)
     if status != 0:
@@ -130,13 +130,17 @@ def note_launches(n: int) -> None:
     launch_count += n
 
 
+_DTYPE_CODES: dict = {}
+
+
 def dtype_code(dtype) -> int:
-    import torch
-    if dtype == torch.bfloat16:
-        return NS_BF16
-    if dtype == torch.float32:
-        return NS_F32
-    raise NotImplementedError(f"nanoserve_b200 kernels handle bfloat16 and float32, not {dtype}")
+    if not _DTYPE_CODES:
+        import torch
+        _DTYPE_CODES.update({torch.bfloat16: NS_BF16, torch.float32: NS_F32})
+    code = _DTYPE_CODES.get(dtype)
+    if code is None:
+        raise NotImplementedError(f"nanoserve_b200 kernels handle bfloat16 and float32, not {dtype}")
+    return code
 
 
 _KV8_CODES: dict = {}
@@ -181,11 +185,18 @@ def same_device(*tensors) -> int:
     return dev
 
 
+_cuda_state = None
+
+
 def call_on(device: int, name: str, *args) -> None:
     """call() with CUDA device `device` current (a launch needs that) and its current stream as the last argument."""
-    import torch
-    if device == torch._C._cuda_getDevice():
-        call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+    global _cuda_state
+    if _cuda_state is None:
+        import torch
+        _cuda_state = (torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.cuda.device)
+    current, raw_stream, guard = _cuda_state
+    if device == current():
+        call(name, *args, raw_stream(device))
         return
-    with torch.cuda.device(device):
-        call(name, *args, torch._C._cuda_getCurrentRawStream(device))
+    with guard(device):
+        call(name, *args, raw_stream(device))

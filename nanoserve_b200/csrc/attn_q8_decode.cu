@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
             };
             auto put_scales = [&]() {                         // (the older batch of the two in `info` may still be read)
                 const float svf = sv < kMinScale ? kMinScale : sv;
-                info[(((id_base - j0) >> 5) & 1) * 32 + lane] = make_float4(sk, log2f(svf), 1.f / svf, id >= 0 ? 1.f : 0.f);
+                info[(((id_base - j0) >> 5) & 1) * 32 + lane] = make_float4(sk, __log2f(svf), __fdividef(1.f, svf), id >= 0 ? 1.f : 0.f);
                 __syncwarp();
             };
             Tile<HD> ring[D];
@@ -467,31 +467,34 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
         if (h >= min(8, p.group - h0)) continue;
         const int w0 = ch.z & 0xff, slot = (ch.z >> 8) & 0xff, w1 = ch.z >> 16;
         const float* const piece0 = slots + ((w0 * 2 + slot) * 8 + h) * RS;      // of the first warp; the others' are their slot 0
-        auto piece = [&](int w) -> const float* { return w == w0 ? piece0 : slots + (w * 16 + h) * RS; };
         float2 ml = make_float2(-INFINITY, 0.f);
-        if (w0 + lane <= w1 && warp_cut(w0 + lane) < warp_cut(w0 + lane + 1)) ml = *reinterpret_cast<const float2*>(piece(w0 + lane) + HD);
+        if (w0 + lane <= w1 && warp_cut(w0 + lane) < warp_cut(w0 + lane + 1)) 
+            ml = *reinterpret_cast<const float2*>((lane == 0 ? piece0 : slots + ((w0 + lane) * 16 + h) * RS) + HD);
         const float m = warp_max(ml.x);
         const float wt = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
         const float l = warp_sum(ml.y == 0.f ? 0.f : wt * ml.y);
         float acc[C];
 #pragma unroll
         for (int i = 0; i < C; ++i) acc[i] = 0.f;
-#pragma unroll 4
-        for (int w = w0; w <= w1; ++w) {
-            const float f = __shfl_sync(0xffffffffu, wt, w - w0);
-            if (f == 0.f) continue;                          // (a warp without tiles, or a piece that weighs nothing)
-            const float* src = piece(w) + C * lane;
-            if constexpr (C == 4) {
-                const float4 v = *reinterpret_cast<const float4*>(src);
-                acc[0] = fmaf(f, v.x, acc[0]);
-                acc[1] = fmaf(f, v.y, acc[1]);
-                acc[2] = fmaf(f, v.z, acc[2]);
-                acc[3] = fmaf(f, v.w, acc[3]);
-            } else {
-                const float2 v = *reinterpret_cast<const float2*>(src);
-                acc[0] = fmaf(f, v.x, acc[0]);
-                acc[1] = fmaf(f, v.y, acc[1]);
+        // all pieces' columns are requested before the first is used (a piece without tiles, or one that weighs nothing, is skipped:
+        // its slot may hold anything)
+        float v[NW][C];
+#pragma unroll
+        for (int k = 0; k < NW; ++k) {
+            const bool on = w0 + k <= w1 && __shfl_sync(0xffffffffu, wt, k) != 0.f;
+            const float* src = (k == 0 ? piece0 : slots + ((w0 + k) * 16 + h) * RS) + C * lane;
+#pragma unroll
+            for (int i = 0; i < C; i += 2) {
+                const float2 u = on ? *reinterpret_cast<const float2*>(src + i) : make_float2(0.f, 0.f);
+                v[k][i] = u.x;
+                v[k][i + 1] = u.y;
             }
+        }
+#pragma unroll
+        for (int k = 0; k < NW; ++k) {
+            const float f = __shfl_sync(0xffffffffu, wt, k);
+#pragma unroll
+            for (int i = 0; i < C; ++i) acc[i] = fmaf(f, v[k][i], acc[i]);
         }
         if (ch.w == 1) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -542,18 +545,18 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
         const int f = u.z, parts = u.w;
         const int kvh = u.y / sub, h0 = (u.y - kvh * sub) * 8, heads = min(8, p.group - h0);
         // thread = (share of the pieces, head, four columns); piece i lies in CTA f + i, the first CTA's is its "begins here" piece.
-        // Eight pieces' statistics and columns are requested at once.
-        constexpr int E4 = 8 * HD / 4, GR = THREADS / E4;
+        // B pieces' statistics and columns are requested at once.
+        constexpr int E4 = 8 * HD / 4, GR = THREADS / E4, B = GR > 1 ? 8 : 16;
         static_assert(GR >= 1, "one float4 column per thread at least");
         const int e = tid % E4, gr = tid / E4, h = e / (HD / 4), c4 = e % (HD / 4);
         float m = -INFINITY, l = 0.f;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         if (gr < GR && h < heads)
-            for (int i0 = gr; i0 < parts; i0 += 8 * GR) {
-                float2 ml[8];
-                float4 v[8];
+            for (int i0 = gr; i0 < parts; i0 += B * GR) {
+                float2 ml[B];
+                float4 v[B];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < B; ++i) {
                     const int q = i0 + i * GR;
                     const float* src = partials + ((size_t)((f + q) * 2 + (q == 0)) * 8 + h) * RS;
                     ml[i] = q < parts ? __ldcg(reinterpret_cast<const float2*>(src + HD)) : make_float2(-INFINITY, 0.f);
@@ -561,7 +564,7 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
                 }
                 float mn = m;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) mn = fmaxf(mn, ml[i].x);
+                for (int i = 0; i < B; ++i) mn = fmaxf(mn, ml[i].x);
                 const float ref = mn == -INFINITY ? 0.f : mn, al = ex2(m - ref);
                 m = mn;
                 l *= al;
@@ -570,7 +573,7 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
                 acc.z *= al;
                 acc.w *= al;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < B; ++i) {
                     const float wt = ml[i].x == -INFINITY ? 0.f : ex2(ml[i].x - ref);
                     l = fmaf(wt, ml[i].y, l);
                     acc.x = fmaf(wt, v[i].x, acc.x);

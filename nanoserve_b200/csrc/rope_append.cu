@@ -25,6 +25,17 @@ __global__ void __launch_bounds__(256) rope_tables_kernel(const int64_t* pos, co
 }
 
 // ------------------------------------------------------------------------------------------------ rotation
+// Quotient of a 31-bit number by a fixed divisor: a multiplication and a shift instead of a division per item.
+struct FastDiv {
+    uint32_t mul = 0, shift = 0, div = 1;
+    FastDiv() = default;
+    explicit FastDiv(uint32_t d) : div(d) {
+        while ((1ull << shift) < d) ++shift;
+        mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t quot(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+
 struct RopeAppendParams {
     const void *q, *k, *v;                    // rows of heads, head stride = head_dim
     int64_t q_stride, k_stride, v_stride;     // elements between tokens
@@ -37,7 +48,9 @@ struct RopeAppendParams {
     int64_t n_tokens, n_slots;
     int n_heads, n_kv_heads, head_dim, block_size, block_shift;
     int64_t blk_stride, pos_stride, head_stride, sc_blk_stride, sc_head_stride;
-    int kv_ctas, planes, chunk;               // 8-bit pools: CTAs of the append role, (head, K or V) planes, tokens per CTA
+    int kv_ctas, planes;                      // 8-bit pools: CTAs of the append role, (head, K or V) planes
+    FastDiv by_cpr, by_groups;                // items of the other role: pieces per head, groups of heads per token
+    int h0, h1, heads_per_item, pairs;        // heads [h0, h1) of q | k | v have work there; pairs: rotate_pairs takes them
 };
 
 template <typename T, int V> __device__ __forceinline__ void load_vec(const T* p, float (&x)[V]) {
@@ -126,59 +139,37 @@ __device__ __forceinline__ void rotate_vec(const T* head, int rot, int interleav
 }
 
 // ------------------------------------------------------------------------------------------------ append, 8-bit pools
-// A block's scale depends on every row of it that the call writes, so a block has ONE owner: the warp that holds the first
-// token of the call which lands in it (the leader), whatever order the tokens come in and however often a slot is named.
-// A CTA takes `chunk` tokens and one (head, K or V) plane: it finds the leaders among its tokens, scans all slots of the
-// call for the members of their blocks (the last token that names a slot wins, a block with an earlier token elsewhere
-// is left to that token's CTA), and each warp then takes one leader: largest magnitude, scale, codes.
-constexpr int kAppendChunk = 64;              // most tokens per CTA
+// A block's scale depends on every row of it that the call writes, so a block has ONE owner per plane (KV head, K or V): the
+// warp of the first token of the call which lands in it (the leader), whatever order the tokens come in and however often a
+// slot is named. The owner needs the block's members: for each row, the last token of the call that names it.
+//   steps of up to kSmallStep tokens: a warp per (token, plane) looks through all slots itself; nothing is shared, no barrier.
+//   larger steps: a CTA takes kAppendChunk tokens of a plane, finds the leaders among them, and its threads look through all
+//     slots once for all of its leaders' blocks. (256 tokens / one layer of the 14-head shape: 3.4 us against 5.4 for the CTA form;
+//     4096 tokens: a scan per leader and plane would read every slot 2,000 times.)
+constexpr int kSmallStep = 256;
+constexpr int kAppendChunk = 64;              // tokens per CTA of a large step
 constexpr int kAppendMaxBlock = 64;           // largest block size
 constexpr int kAppendWarps = 8;
 
-template <typename T, typename KV, int V>
-__device__ void append_kv8(const RopeAppendParams& p, int cta) {
-    __shared__ int member[kAppendChunk * kAppendMaxBlock];
-    __shared__ int cand_block[kAppendChunk], cand_tok[kAppendChunk], cand_dead[kAppendChunk];
-    __shared__ int n_cand;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int plane = cta % p.planes, bs = p.block_size, mask = bs - 1;
-    const int64_t t0 = (int64_t)(cta / p.planes) * p.chunk;
-    const int n_here = (int)(p.n_tokens - t0 < p.chunk ? p.n_tokens - t0 : p.chunk);
-    const int n_tok = (int)p.n_tokens;
-    if (tid == 0) n_cand = 0;
-    for (int i = tid; i < p.chunk * bs; i += blockDim.x) member[i] = -1;
-    __syncthreads();
-    auto block_of = [&](int64_t slot) -> int { return (slot >= 0 && slot < p.n_slots) ? (int)(slot >> p.block_shift) : -1; };
-    if (tid < n_here) {
-        const int t = (int)t0 + tid;
-        const int b = block_of(p.slots[t]);
-        if (b >= 0 && (t == 0 || block_of(p.slots[t - 1]) != b)) {
-            const int c = atomicAdd(&n_cand, 1);
-            cand_block[c] = b;
-            cand_tok[c] = t;
-            cand_dead[c] = 0;
-        }
-    }
-    __syncthreads();
-    const int nc = n_cand;
-    for (int t = tid; t < n_tok; t += blockDim.x) {
-        const int64_t slot = p.slots[t];
-        const int b = block_of(slot);
-        if (b < 0) continue;
-        for (int c = 0; c < nc; ++c)
-            if (cand_block[c] == b) {
-                if (t < cand_tok[c]) cand_dead[c] = 1;
-                else atomicMax(&member[c * bs + ((int)slot & mask)], t);
-            }
-    }
-    __syncthreads();
+template <typename KV> __device__ __forceinline__ uint2 encode8(const float (&x)[8]) {
+    uint2 w = make_uint2(0u, 0u);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) (j < 4 ? w.x : w.y) |= KV::encode(x[j]) << (8 * (j & 3));
+    return w;
+}
 
-    const int head = plane >> 1, is_v = plane & 1, hd = p.head_dim;
+// One block of one plane by one warp. mem[row]: the token that writes the row, or -1. NI > 0: the block has NI * 32 pieces of V
+// dims, CPR per row, and the rotated values wait in registers for the scale; NI == 0: any sizes, the values are computed twice.
+template <typename T, typename KV, int V, int NI, int CPR>
+__device__ __forceinline__ void append_block(const RopeAppendParams& p, int plane, int64_t blk, const int* mem) {
+    const int lane = threadIdx.x & 31, head = plane >> 1, is_v = plane & 1, hd = p.head_dim, half = p.rot / 2;
     const T* src = reinterpret_cast<const T*>(is_v ? p.v : p.k) + (int64_t)head * hd;
     const int64_t src_stride = is_v ? p.v_stride : p.k_stride;
-    uint8_t* pool = reinterpret_cast<uint8_t*>(is_v ? p.v_pool : p.k_pool) + head * p.head_stride;
-    float* scales = (is_v ? p.v_scale : p.k_scale) + head * p.sc_head_stride;
-    const int cpr = hd / V, items = bs * cpr, half = p.rot / 2;
+    uint8_t* pool = reinterpret_cast<uint8_t*>(is_v ? p.v_pool : p.k_pool) + head * p.head_stride + blk * p.blk_stride;
+    float* sc = (is_v ? p.v_scale : p.k_scale) + head * p.sc_head_stride + blk * p.sc_blk_stride;
+    const float old = *sc;
+    const bool fresh = mem[0] >= 0;
+    const int cpr = NI > 0 ? CPR : hd / V, items = NI > 0 ? NI * 32 : p.block_size * cpr;
     auto values = [&](int t, int d0, float (&x)[V]) {
         const T* row = src + t * src_stride;
         if (!is_v && d0 < p.rot) {
@@ -190,105 +181,278 @@ __device__ void append_kv8(const RopeAppendParams& p, int cta) {
             load_vec<T, V>(row + d0, x);
         }
     };
-    for (int c = warp; c < nc; c += kAppendWarps) {
-        if (cand_dead[c]) continue;
-        const int* mem = member + c * bs;
-        const int64_t blk = cand_block[c];
-        uint32_t amax = 0;
+    float kept[NI > 0 ? NI : 1][V];
+    uint32_t amax = 0;
+    if constexpr (NI > 0) {
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+            const int i = n * 32 + lane, t = mem[i / CPR];
+            if (t >= 0) values(t, (i % CPR) * V, kept[n]);
+            if (n & 1) asm volatile("" ::: "memory");            // two rows' loads at a time: all of them would not fit the registers
+        }
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+            if (mem[(n * 32 + lane) / CPR] < 0) continue;
+#pragma unroll
+            for (int j = 0; j < V; ++j) amax = max(amax, (uint32_t)__float_as_int(kept[n][j]) & 0x7fffffffu);
+        }
+    } else {
         for (int i = lane; i < items; i += 32) {
             const int off = i / cpr, t = mem[off];
             if (t < 0) continue;
-            float x[V];
-            values(t, (i - off * cpr) * V, x);
+            values(t, (i - off * cpr) * V, kept[0]);
 #pragma unroll
-            for (int j = 0; j < V; ++j) amax = max(amax, (uint32_t)__float_as_int(x[j]) & 0x7fffffffu);
-        }
-        amax = __reduce_max_sync(0xffffffffu, amax);
-        const float s_new = pow2_scale<KV>(amax);
-        float* sc = scales + blk * p.sc_blk_stride;
-        const float old = *sc;
-        const bool fresh = mem[0] >= 0;
-        const float now = fresh ? s_new : (old != old || s_new != s_new) ? __int_as_float(0x7fffffff) : fmaxf(old, s_new);
-        const float inv = 1.0f / now, ratio = old / now;
-        __syncwarp();
-        if (lane == 0) *sc = now;
-        for (int i = lane; i < items; i += 32) {
-            const int off = i / cpr, t = mem[off], d0 = (i - off * cpr) * V;
-            uint8_t* dst = pool + blk * p.blk_stride + (int64_t)off * p.pos_stride + d0;
-            float x[V];
-            if (t >= 0) {
-                values(t, d0, x);
-#pragma unroll
-                for (int j = 0; j < V; ++j) x[j] = __fmul_rn(x[j], inv);
-            } else if (fresh) {
-#pragma unroll
-                for (int j = 0; j < V; ++j) x[j] = 0.f;
-            } else if (now == old) {
-                continue;
-            } else {
-                if constexpr (V == 1) {
-                    x[0] = __fmul_rn(KV::decode(dst[0]), ratio);
-                } else {
-                    const uint2 w = *reinterpret_cast<const uint2*>(dst);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(KV::decode(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 0xffu), ratio);
-                }
-            }
-            if constexpr (V == 1) {
-                dst[0] = (uint8_t)KV::encode(x[0]);
-            } else {
-                uint2 w = make_uint2(0u, 0u);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) (j < 4 ? w.x : w.y) |= KV::encode(x[j]) << (8 * (j & 3));
-                *reinterpret_cast<uint2*>(dst) = w;
-            }
+            for (int j = 0; j < V; ++j) amax = max(amax, (uint32_t)__float_as_int(kept[0][j]) & 0x7fffffffu);
         }
     }
+    amax = __reduce_max_sync(0xffffffffu, amax);
+    const float s_new = pow2_scale<KV>(amax);
+    const float now = fresh ? s_new : (old != old || s_new != s_new) ? __int_as_float(0x7fffffff) : fmaxf(old, s_new);
+    const float inv = 1.0f / now, ratio = old / now;
+    __syncwarp();
+    if (lane == 0 && now != old) *sc = now;
+    auto put = [&](int off, int d0, int t, float (&x)[V]) {      // x: the row's values if a token writes it
+        uint8_t* dst = pool + (int64_t)off * p.pos_stride + d0;
+        if (t >= 0) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[j] = __fmul_rn(x[j], inv);
+        } else if (fresh) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[j] = 0.f;
+        } else if (now == old) {
+            return;
+        } else if constexpr (V == 1) {
+            x[0] = __fmul_rn(KV::decode(dst[0]), ratio);
+        } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(dst);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(KV::decode(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 0xffu), ratio);
+        }
+        if constexpr (V == 1) dst[0] = (uint8_t)KV::encode(x[0]);
+        else *reinterpret_cast<uint2*>(dst) = encode8<KV>(x);
+    };
+    if constexpr (NI > 0) {
+#pragma unroll
+        for (int n = 0; n < NI; ++n) {
+            const int i = n * 32 + lane;
+            put(i / CPR, (i % CPR) * V, mem[i / CPR], kept[n]);
+        }
+    } else {
+        for (int i = lane; i < items; i += 32) {
+            const int off = i / cpr, t = mem[off], d0 = (i - off * cpr) * V;
+            if (t >= 0) values(t, d0, kept[0]);
+            put(off, d0, t, kept[0]);
+        }
+    }
+}
+
+template <typename T, typename KV, int V>
+__device__ __forceinline__ void append_any(const RopeAppendParams& p, int plane, int64_t blk, const int* mem) {
+    if constexpr (V == 8) {                      // the layouts of the framework's models; the others by the loop
+        if (p.block_size == 16 && p.head_dim == 64) return append_block<T, KV, V, 4, 8>(p, plane, blk, mem);
+        if (p.block_size == 16 && p.head_dim == 128) return append_block<T, KV, V, 8, 16>(p, plane, blk, mem);
+    }
+    append_block<T, KV, V, 0, 1>(p, plane, blk, mem);
+}
+
+__device__ __forceinline__ int block_of(const RopeAppendParams& p, int64_t slot) {
+    return (slot >= 0 && slot < p.n_slots) ? (int)(slot >> p.block_shift) : -1;
+}
+
+// A warp per (token, plane).
+template <typename T, typename KV, int V> __device__ void append_small(const RopeAppendParams& p, int cta) {
+    __shared__ int member[kAppendWarps][kAppendMaxBlock];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, mask = p.block_size - 1;
+    const int unit = cta * kAppendWarps + warp, n_tok = (int)p.n_tokens;
+    const int t = unit / p.planes, plane = unit - t * p.planes;
+    if (t >= n_tok) return;
+    int blk[kSmallStep / 32], off[kSmallStep / 32];
+#pragma unroll
+    for (int k = 0; k < kSmallStep / 32; ++k) {
+        const int i = k * 32 + lane;
+        const int64_t slot = i < n_tok ? p.slots[i] : -1;
+        blk[k] = block_of(p, slot);
+        off[k] = (int)slot & mask;
+    }
+    int b = -1;
+#pragma unroll
+    for (int k = 0; k < kSmallStep / 32; ++k)
+        if (k == t >> 5) b = blk[k];
+    b = __shfl_sync(0xffffffffu, b, t & 31);
+    if (b < 0) return;
+    int* mem = member[warp];
+    for (int i = lane; i < p.block_size; i += 32) mem[i] = -1;
+    __syncwarp();
+    bool first = true;
+#pragma unroll
+    for (int k = 0; k < kSmallStep / 32; ++k) {
+        unsigned hit = __ballot_sync(0xffffffffu, blk[k] == b);
+        if (hit == 0) continue;
+        if (k * 32 + __ffs(hit) - 1 < t) first = false;        // an earlier token owns the block
+        if (!first) break;
+        if ((hit >> lane) & 1u) atomicMax(&mem[off[k]], k * 32 + lane);
+    }
+    if (!first) return;
+    __syncwarp();
+    append_any<T, KV, V>(p, plane, b, mem);
+}
+
+// A CTA per (chunk of tokens, plane).
+template <typename T, typename KV, int V> __device__ void append_large(const RopeAppendParams& p, int cta) {
+    __shared__ int member[kAppendChunk * kAppendMaxBlock];
+    __shared__ int cand_block[kAppendChunk], cand_tok[kAppendChunk], cand_dead[kAppendChunk];
+    __shared__ int n_cand;
+    const int tid = threadIdx.x, warp = tid >> 5;
+    const int plane = cta % p.planes, bs = p.block_size, mask = bs - 1;
+    const int t0 = (cta / p.planes) * kAppendChunk, n_tok = (int)p.n_tokens;
+    if (tid == 0) n_cand = 0;
+    for (int i = tid; i < kAppendChunk * bs; i += blockDim.x) member[i] = -1;
+    __syncthreads();
+    if (tid < kAppendChunk && t0 + tid < n_tok) {
+        const int t = t0 + tid, b = block_of(p, p.slots[t]);
+        if (b >= 0 && (t == 0 || block_of(p, p.slots[t - 1]) != b)) {
+            const int c = atomicAdd(&n_cand, 1);
+            cand_block[c] = b;
+            cand_tok[c] = t;
+            cand_dead[c] = 0;
+        }
+    }
+    __syncthreads();
+    const int nc = n_cand;
+    for (int base = tid; base < n_tok; base += 4 * blockDim.x) {          // four slots in flight
+        int64_t slot[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) slot[k] = base + k * (int)blockDim.x < n_tok ? p.slots[base + k * (int)blockDim.x] : -1;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int t = base + k * (int)blockDim.x, b = block_of(p, slot[k]);
+            if (b < 0) continue;
+            for (int c = 0; c < nc; ++c)
+                if (cand_block[c] == b) {
+                    if (t < cand_tok[c]) cand_dead[c] = 1;
+                    else atomicMax(&member[c * bs + ((int)slot[k] & mask)], t);
+                }
+        }
+    }
+    __syncthreads();
+    for (int c = warp; c < nc; c += kAppendWarps)
+        if (!cand_dead[c]) append_any<T, KV, V>(p, plane, cand_block[c], member + c * bs);
 }
 
 // ------------------------------------------------------------------------------------------------ the kernel
 struct NoKv8 {};
 
-// CTAs [0, kv_ctas): the append role (8-bit pools). The others walk (token, V dims, group of heads): the angles of the V
-// dims are loaded once for kHeadsPerItem heads.
-constexpr int kHeadsPerItem = 4;
+// Offset of a token's row in a 16/32-bit pool, -1 if its slot is outside.
+__device__ __forceinline__ int64_t pool_row(const RopeAppendParams& p, int64_t slot) {
+    if (slot < 0 || slot >= p.n_slots) return -1;
+    const int64_t b = p.block_shift >= 0 ? slot >> p.block_shift : slot / p.block_size;
+    return b * p.blk_stride + (slot - b * p.block_size) * p.pos_stride;
+}
 
+// Half layout, whole head: a thread takes 8 dims of the low half and their partners for several heads, so each row is read once
+// and the angles once per group of heads; all of its loads are in flight before the first is used.
+template <typename T, bool kv8> __device__ __forceinline__ void rotate_pairs(const RopeAppendParams& p, int cta, int ctas) {
+    constexpr int H = sizeof(T) == 2 ? 4 : 2, W = 8 / Vec16<T>::N;        // heads per item; 16-byte words per 8 dims
+    const int hd = p.head_dim, half = hd / 2, NH = p.n_heads, NKV = p.n_kv_heads;
+    const bool pool16 = !kv8 && p.k_pool != nullptr;
+    const uint32_t cpr = p.by_cpr.div, total = (uint32_t)p.n_tokens * p.by_groups.div * cpr;
+    for (uint32_t i = cta * blockDim.x + threadIdx.x; i < total; i += ctas * blockDim.x) {
+        const uint32_t tg = p.by_cpr.quot(i);
+        const int d0 = (int)(i - tg * cpr) * 8;
+        const int64_t t = p.by_groups.quot(tg);
+        const int first = p.h0 + (int)(tg - (uint32_t)t * p.by_groups.div) * H;
+        Vec16<T> lo[H][W], hi[H][W];
+#pragma unroll
+        for (int e = 0; e < H; ++e) {
+            const int h = first + e;
+            if (h >= p.h1) continue;
+            const T* head = (h < NH         ? reinterpret_cast<const T*>(p.q) + t * p.q_stride + (int64_t)h * hd
+                             : h < NH + NKV ? reinterpret_cast<const T*>(p.k) + t * p.k_stride + (int64_t)(h - NH) * hd
+                                            : reinterpret_cast<const T*>(p.v) + t * p.v_stride + (int64_t)(h - NH - NKV) * hd) + d0;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                lo[e][w] = load16(head + w * Vec16<T>::N);
+                hi[e][w] = load16(head + half + w * Vec16<T>::N);
+            }
+        }
+        float c[8], s[8];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            *reinterpret_cast<float4*>(&c[4 * w]) = *reinterpret_cast<const float4*>(p.cos + t * half + d0 + 4 * w);
+            *reinterpret_cast<float4*>(&s[4 * w]) = *reinterpret_cast<const float4*>(p.sin + t * half + d0 + 4 * w);
+        }
+        const int64_t row_off = pool16 ? pool_row(p, p.slots[t]) : -1;
+#pragma unroll
+        for (int e = 0; e < H; ++e) {
+            const int h = first + e;
+            if (h >= p.h1) continue;
+            const bool is_q = h < NH, is_v = h >= NH + NKV;
+            const int g = is_q ? h : is_v ? h - NH - NKV : h - NH;
+            if (!is_v) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int w = j / Vec16<T>::N, k = j % Vec16<T>::N;
+                    const float a = lo[e][w].get(k), b = hi[e][w].get(k);
+                    lo[e][w].set(k, __fsub_rn(__fmul_rn(a, c[j]), __fmul_rn(b, s[j])));
+                    hi[e][w].set(k, __fadd_rn(__fmul_rn(b, c[j]), __fmul_rn(a, s[j])));
+                }
+            }
+            T* dense = reinterpret_cast<T*>(is_q ? p.q_out : is_v ? p.v_out : p.k_out);
+            T* pool = !is_q && row_off >= 0 ? reinterpret_cast<T*>(is_v ? p.v_pool : p.k_pool) + row_off + g * p.head_stride + d0 : nullptr;
+            if (dense != nullptr) dense += (t * (is_q ? NH : NKV) + g) * hd + d0;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                if (dense != nullptr) {
+                    store16(dense + w * Vec16<T>::N, lo[e][w]);
+                    store16(dense + half + w * Vec16<T>::N, hi[e][w]);
+                }
+                if (pool != nullptr) {
+                    store16(pool + w * Vec16<T>::N, lo[e][w]);
+                    store16(pool + half + w * Vec16<T>::N, hi[e][w]);
+                }
+            }
+        }
+    }
+}
+
+// CTAs [0, kv_ctas): the append role (8-bit pools). The others walk (token, V dims, group of heads): the angles of the V dims are
+// loaded once per group.
 template <typename T, typename KV, int V>
-__global__ void __launch_bounds__(kAppendWarps * 32) rope_append_kernel(const RopeAppendParams p) {
+__global__ void __launch_bounds__(kAppendWarps * 32, 2) rope_append_kernel(const RopeAppendParams p) {
     constexpr bool kv8 = !std::is_same<KV, NoKv8>::value;
     pdl_launch_dependents();
     pdl_wait();
     if constexpr (kv8) {
         if ((int)blockIdx.x < p.kv_ctas) {
-            append_kv8<T, KV, V>(p, blockIdx.x);
+            if (p.n_tokens <= kSmallStep) append_small<T, KV, V>(p, blockIdx.x);
+            else append_large<T, KV, V>(p, blockIdx.x);
+            return;
+        }
+    }
+    if constexpr (V == 8) {
+        if (p.pairs) {
+            rotate_pairs<T, kv8>(p, blockIdx.x - p.kv_ctas, gridDim.x - p.kv_ctas);
             return;
         }
     }
     const int hd = p.head_dim, cpr = hd / V, half = p.rot / 2, NH = p.n_heads, NKV = p.n_kv_heads;
-    const bool dense_k = p.k_out != nullptr, dense_v = p.v_out != nullptr, pool16 = !kv8 && p.k_pool != nullptr;
-    const int h0 = p.q_out != nullptr ? 0 : NH;                                       // heads [h0, h1) of q | k | v have work here
-    const int h1 = (dense_v || pool16) ? NH + 2 * NKV : dense_k ? NH + NKV : NH;
-    const int groups = (h1 - h0 + kHeadsPerItem - 1) / kHeadsPerItem;
-    const int64_t total = p.n_tokens * groups * cpr;
-    for (int64_t i = (blockIdx.x - p.kv_ctas) * (int64_t)blockDim.x + threadIdx.x; i < total;
-         i += (int64_t)(gridDim.x - p.kv_ctas) * blockDim.x) {
-        const int64_t tg = i / cpr;
+    const bool pool16 = !kv8 && p.k_pool != nullptr;
+    const uint32_t total = (uint32_t)p.n_tokens * p.by_groups.div * cpr;
+    for (uint32_t i = (blockIdx.x - p.kv_ctas) * blockDim.x + threadIdx.x; i < total; i += (gridDim.x - p.kv_ctas) * blockDim.x) {
+        const uint32_t tg = p.by_cpr.quot(i);
         const int d0 = (int)(i - tg * cpr) * V;
-        const int64_t t = tg / groups;
-        const int grp = (int)(tg - t * groups);
+        const int64_t t = p.by_groups.quot(tg);
+        const int first = p.h0 + (int)(tg - (uint32_t)t * p.by_groups.div) * p.heads_per_item;
         float c[V], s[V];
         const bool rotated = d0 < p.rot;
         if (rotated) {
             load_angles<V>(p.cos + t * half, p.rot, p.interleaved, d0, c);
             load_angles<V>(p.sin + t * half, p.rot, p.interleaved, d0, s);
         }
-        const int64_t slot = pool16 ? p.slots[t] : -1;
-        const bool stored = pool16 && slot >= 0 && slot < p.n_slots;
-        const int64_t row_off = stored ? (slot / p.block_size) * p.blk_stride + (slot % p.block_size) * p.pos_stride : 0;
-#pragma unroll
-        for (int e = 0; e < kHeadsPerItem; ++e) {
-            const int h = h0 + grp * kHeadsPerItem + e;
-            if (h >= h1) break;
+        const int64_t row_off = pool16 ? pool_row(p, p.slots[t]) : -1;
+        for (int e = 0; e < p.heads_per_item; ++e) {
+            const int h = first + e;
+            if (h >= p.h1) break;
             const bool is_q = h < NH, is_v = h >= NH + NKV;
             const int g = is_q ? h : is_v ? h - NH - NKV : h - NH;
             const T* head = (is_q   ? reinterpret_cast<const T*>(p.q) + t * p.q_stride
@@ -299,7 +463,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) rope_append_kernel(const Ro
             else load_vec<T, V>(head + d0, x);
             T* dense = reinterpret_cast<T*>(is_q ? p.q_out : is_v ? p.v_out : p.k_out);
             if (dense != nullptr) store_vec<T, V>(dense + (t * (is_q ? NH : NKV) + g) * hd + d0, x);
-            if (stored && !is_q) {
+            if (!is_q && row_off >= 0) {
                 T* pool = reinterpret_cast<T*>(is_v ? p.v_pool : p.k_pool);
                 store_vec<T, V>(pool + row_off + g * p.head_stride + d0, x);
             }
@@ -312,16 +476,27 @@ template <typename T, typename KV, int V> static int launch_rope_append(RopeAppe
     const int threads = kAppendWarps * 32;
     int sms = device_sm_count();
     if (sms <= 0) sms = 148;
-    p.kv_ctas = 0;
     p.planes = 2 * p.n_kv_heads;
-    // Tokens per append CTA: few where the step is small (a decode step's tokens are one leader each: more CTAs), 64 where
-    // the scan of all slots, which every CTA repeats, would otherwise dominate.
-    p.chunk = p.n_tokens <= 1024 ? 16 : kAppendChunk;
-    if (kv8) p.kv_ctas = (int)((p.n_tokens + p.chunk - 1) / p.chunk) * p.planes;
-    const int heads = (p.q_out != nullptr ? p.n_heads : 0) + ((p.v_out || (!kv8 && p.k_pool)) ? 2 * p.n_kv_heads : p.k_out ? p.n_kv_heads : 0);
-    const int64_t items = p.n_tokens * ((heads + kHeadsPerItem - 1) / kHeadsPerItem) * (p.head_dim / V);
+    p.h0 = p.q_out != nullptr ? 0 : p.n_heads;
+    p.h1 = (p.v_out || (!kv8 && p.k_pool)) ? p.n_heads + 2 * p.n_kv_heads : p.k_out ? p.n_heads + p.n_kv_heads : p.n_heads;
+    p.pairs = V == 8 && !p.interleaved && p.rot == p.head_dim;
+    p.heads_per_item = p.pairs && sizeof(T) == 4 ? 2 : 4;
+    const int64_t groups = p.h1 > p.h0 ? (p.h1 - p.h0 + p.heads_per_item - 1) / p.heads_per_item : 0, cpr = p.head_dim / (p.pairs ? 2 * V : V);
+    p.kv_ctas = 0;
+    if (kv8) {
+        const int64_t n = p.n_tokens <= kSmallStep ? (p.n_tokens * p.planes + kAppendWarps - 1) / kAppendWarps
+                                                   : (p.n_tokens + kAppendChunk - 1) / kAppendChunk * p.planes;
+        NS_REQUIRE(n < (1 << 30), NS_ERR_UNSUPPORTED, "rope_append: %lld tokens", (long long)p.n_tokens);
+        p.kv_ctas = (int)n;
+    }
+    const int64_t items = p.n_tokens * groups * cpr;
+    NS_REQUIRE(items < ((int64_t)1 << 31), NS_ERR_UNSUPPORTED, "rope_append: %lld tokens", (long long)p.n_tokens);
+    if (groups > 0) {
+        p.by_cpr = FastDiv((uint32_t)cpr);
+        p.by_groups = FastDiv((uint32_t)groups);
+    }
     int64_t ctas = (items + threads - 1) / threads;
-    if (ctas > sms * 8) ctas = sms * 8;
+    if (ctas > sms * 16) ctas = sms * 16;
     if (ctas + p.kv_ctas == 0) return NS_OK;
     cudaError_t e = launch_pdl(rope_append_kernel<T, KV, V>, dim3((unsigned)(ctas + p.kv_ctas)), dim3(threads), 0, st, p);
     if (e != cudaSuccess) return fail(NS_ERR_CUDA, "rope_append: launch failed: %s", cudaGetErrorString(e));
@@ -427,6 +602,7 @@ extern "C" int ns_rope_append(const void* q, const void* k, const void* v, int64
     p.k_scale = k_scale; p.v_scale = v_scale; p.slots = slots; p.n_tokens = n_tokens; p.n_slots = n_slots;
     p.n_heads = n_heads; p.n_kv_heads = n_kv_heads; p.head_dim = head_dim; p.block_size = block_size > 0 ? block_size : 1;
     while ((1 << p.block_shift) < p.block_size) ++p.block_shift;
+    if ((1 << p.block_shift) != p.block_size) p.block_shift = -1;         // (16/32-bit pools only)
     p.blk_stride = pool_block_stride; p.pos_stride = pool_pos_stride; p.head_stride = pool_head_stride;
     p.sc_blk_stride = scale_block_stride; p.sc_head_stride = scale_head_stride;
     const int kind = k_pool == nullptr ? dtype : pool_dtype;

@@ -31,6 +31,7 @@ class AttnWorkspace:
         self._raw = torch.zeros(self.nbytes + 256, dtype=torch.uint8, device=device)
         off = (-self._raw.data_ptr()) % 256
         self.buf = self._raw[off:off + self.nbytes]
+        self.ptr = self.buf.data_ptr()
 
     def fits(self, n_seqs: int, n_tokens: int, n_heads: int, head_dim: int) -> bool:
         return (n_seqs <= self.max_seqs and n_tokens <= self.max_tokens and n_heads == self.n_heads
@@ -51,12 +52,12 @@ _cached_q8: dict[tuple, AttnWorkspace] = {}
 def _workspace_q8(device, n_seqs: int, n_tokens: int, n_heads: int, head_dim: int) -> AttnWorkspace:
     """The workspace of a call over an 8-bit pool that brings none: one per device and stream, so that calls on two streams
     never share one; inside a graph capture a new one, which belongs to the graph."""
-    cap_s, cap_t = max(256, 1 << (max(n_seqs, 1) - 1).bit_length()), max(4096, 1 << (max(n_tokens, 1) - 1).bit_length())
     if torch.cuda.is_current_stream_capturing():
         return AttnWorkspace(max(n_seqs, 1), max(n_tokens, 1), n_heads, head_dim, device)
-    key = (device.index, torch.cuda.current_stream(device).cuda_stream, n_heads, head_dim)
+    key = (device.index, torch._C._cuda_getCurrentRawStream(device.index), n_heads, head_dim)
     ws = _cached_q8.get(key)
-    if ws is None or not ws.fits(n_seqs, n_tokens, n_heads, head_dim):
+    if ws is None or n_seqs > ws.max_seqs or n_tokens > ws.max_tokens:
+        cap_s, cap_t = max(256, 1 << (max(n_seqs, 1) - 1).bit_length()), max(4096, 1 << (max(n_tokens, 1) - 1).bit_length())
         ws = _cached_q8[key] = AttnWorkspace(cap_s, cap_t, n_heads, head_dim, device)
     return ws
 
@@ -78,58 +79,64 @@ def _check_pool(q, k_pool, v_pool):
     assert k_pool.dtype == q.dtype and v_pool.dtype == q.dtype
 
 
-def _attend_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, seq_lens, cu_seqlens, scale, n_seqs, workspace, planned, out,
+def _attend_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, seq_lens, cu_seqlens, scale, n_seqs, ws, planned, out,
                simple) -> torch.Tensor:
-    """Ragged attention over an int8 / float8_e4m3fn pool (ns_ragged_paged_attn_q8)."""
+    """Ragged attention over an int8 / float8_e4m3fn pool (ns_ragged_paged_attn_q8). (A decode step makes one such call per layer:
+    the checks look at every tensor once.)"""
     N, n_heads, head_dim = q.shape
-    num_blocks, block_size, n_kv_heads, hd = k_pool.shape
+    pool_shape = num_blocks, block_size, n_kv_heads, hd = k_pool.shape
     rows, width = block_tables.shape
-    qs, ps, ts, i32 = q.stride(), k_pool.stride(), block_tables.stride(), torch.int32
+    q0, q1, q2 = q.stride()
+    ps = p0, p1, p2, p3 = k_pool.stride()
+    t0, t1 = block_tables.stride()
+    i32, kv_dtype, q_dtype = torch.int32, k_pool.dtype, q.dtype
     if v_scale is None:
-        raise ValueError(f"a {k_pool.dtype} pool needs k_scale and v_scale (fp32 [num_blocks, n_kv_heads])")
-    ss = check_kv8_scales(k_pool, k_scale, v_scale)
-    assert hd == head_dim and v_pool.shape == k_pool.shape and v_pool.stride() == ps and v_pool.dtype is k_pool.dtype and ps[3] == 1
-    assert qs[2] == 1 and (qs[1] == head_dim or n_heads == 1), "query heads must be adjacent (head stride == head_dim)"
-    assert block_tables.dtype is i32 and (ts[1] == 1 or width <= 1)
+        raise ValueError(f"a {kv_dtype} pool needs k_scale and v_scale (fp32 [num_blocks, n_kv_heads])")
+    s0, s1 = check_kv8_scales(k_pool, k_scale, v_scale)
+    assert hd == head_dim and p3 == 1 and v_pool.shape == pool_shape and v_pool.stride() == ps and v_pool.dtype is kv_dtype
+    assert q2 == 1 and (q1 == head_dim or n_heads == 1), "query heads must be adjacent (head stride == head_dim)"
+    assert block_tables.dtype is i32 and (t1 == 1 or width <= 1)
     assert seq_lens.dtype is i32 and seq_lens.is_contiguous() and seq_lens.shape[0] >= n_seqs
+    dev = _lib.same_device(q, k_pool, v_pool, k_scale, v_scale, block_tables, seq_lens)
+    cu = rows_ptr = None
     if cu_seqlens is None:
         assert N == n_seqs, "without cu_seqlens every sequence has one token"
     else:
         assert cu_seqlens.dtype is i32 and cu_seqlens.is_contiguous() and cu_seqlens.shape[0] > n_seqs
+        cu = cu_seqlens.data_ptr()
+        _lib.same_device(q, cu_seqlens)
     if table_rows is None:
         assert rows >= n_seqs, "block_tables has a row per sequence"
     else:
         assert table_rows.dtype is i32 and table_rows.is_contiguous() and table_rows.shape[0] >= n_seqs
-    dev = _lib.same_device(q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, seq_lens, cu_seqlens, out)
+        rows_ptr = table_rows.data_ptr()
+        _lib.same_device(q, table_rows)
     if out is None:
-        out = torch.empty((N, n_heads, head_dim), device=q.device, dtype=q.dtype)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        o0 = n_heads * head_dim
     else:
-        assert out.shape == q.shape and out.stride(2) == 1 and (out.stride(1) == head_dim or n_heads == 1) and out.dtype is q.dtype
-    common = (q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(),
-              None if table_rows is None else table_rows.data_ptr(), seq_lens.data_ptr(),
-              None if cu_seqlens is None else cu_seqlens.data_ptr(), out.data_ptr(), n_seqs, N, n_heads, n_kv_heads, head_dim, block_size,
-              num_blocks, width, ts[0], qs[0], out.stride(0), *ps[:3], *ss, scale, _lib.dtype_code(q.dtype), _lib.kv8_code(k_pool.dtype))
-    if simple:
-        _lib.call_on(dev, "ns_ragged_paged_attn_q8_simple", *common)
-        return out
+        o0, o1, o2 = out.stride()
+        assert out.shape == q.shape and o2 == 1 and (o1 == head_dim or n_heads == 1) and out.dtype is q_dtype
+        _lib.same_device(q, out)
     if dev != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            _launch_q8(common, dev, q.device, workspace, planned, seq_lens, cu_seqlens, table_rows)
-    else:
-        _launch_q8(common, dev, q.device, workspace, planned, seq_lens, cu_seqlens, table_rows)
-    return out
-
-
-def _launch_q8(common, dev, device, ws, planned, seq_lens, cu_seqlens, table_rows) -> None:
-    n_seqs, N, n_heads, _, head_dim, block_size = common[10:16]
+        with torch.cuda.device(dev):                       # a launch needs its device current
+            return _attend_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, seq_lens, cu_seqlens, scale, n_seqs, ws, planned,
+                              out, simple)
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    args = (q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(), rows_ptr,
+            seq_lens.data_ptr(), cu, out.data_ptr(), n_seqs, N, n_heads, n_kv_heads, head_dim, block_size, num_blocks, width, t0, q0, o0, p0, p1,
+            p2, s0, s1, scale, _lib.dtype_code(q_dtype), _lib.kv8_code(kv_dtype))
+    if simple:
+        _lib.call("ns_ragged_paged_attn_q8_simple", *args, stream)
+        return out
     if ws is None:
-        ws = _workspace_q8(device, n_seqs, N, n_heads, head_dim)
-    mixed = cu_seqlens is not None and N > 1
-    if mixed and not planned:
-        ws.plan(seq_lens, cu_seqlens, n_seqs, block_size, table_rows)
-    _lib.call_on(dev, "ns_ragged_paged_attn_q8", *common, ws.buf.data_ptr(), ws.nbytes, ws.max_seqs, ws.max_tokens)
-    if mixed:
+        ws = _workspace_q8(q.device, n_seqs, N, n_heads, head_dim)
+    if cu is not None and N > 1:
+        if not planned:
+            ws.plan(seq_lens, cu_seqlens, n_seqs, block_size, table_rows)
         _lib.note_launches(1)          # the prefill-tile kernel is launched next to the decode kernel
+    _lib.call("ns_ragged_paged_attn_q8", *args, ws.ptr, ws.nbytes, ws.max_seqs, ws.max_tokens, stream)
+    return out
 
 
 def paged_attention_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Tensor,

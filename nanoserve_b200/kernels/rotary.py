@@ -67,7 +67,7 @@ def rope_tables(positions: torch.Tensor, inv_freq: torch.Tensor, factor: float =
     assert positions.dtype is torch.int64 and positions.dim() == 1 and positions.is_contiguous()
     assert inv_freq.dtype is torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous()
     t, half = positions.shape[0], inv_freq.shape[0]
-    cos = torch.empty((t, half), device=positions.device, dtype=torch.float32)
+    cos = inv_freq.new_empty((t, half))
     sin = torch.empty_like(cos)
     _lib.call_on(dev, "ns_rope_tables", positions.data_ptr(), inv_freq.data_ptr(), float(factor), cos.data_ptr(), sin.data_ptr(), t, half)
     return cos, sin
@@ -133,7 +133,7 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_heads
     assert cos.is_contiguous() and sin.is_contiguous() and 2 * half <= head_dim
     pool, n_slots, block_size, strides, code = _pool_args(dtype, n, n_kv_heads, head_dim, k_cache, v_cache, slots, k_scale, v_scale)
     dev = _lib.same_device(qkv, cos, sin, k_cache, v_cache, slots, k_scale, v_scale)
-    q = torch.empty((n, n_heads, head_dim), device=qkv.device, dtype=dtype)
+    q = qkv.new_empty((n, n_heads, head_dim))
     k = torch.empty((n, n_kv_heads, head_dim), device=qkv.device, dtype=dtype) if dense_kv else None
     v = torch.empty_like(k) if dense_kv else None
     base, size = qkv.data_ptr(), 2 if dtype is torch.bfloat16 else 4
