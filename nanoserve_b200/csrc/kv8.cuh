@@ -8,14 +8,21 @@
 
 namespace ns {
 
-// Storage kinds of a pool element. kOrd: bits of the largest code's mantissa and its exponent (127 = 1.984375 * 2^6,
+// Storage kinds of a pool element. kMaxMant / kMaxExp: the largest code's mantissa bits and exponent (127 = 1.984375 * 2^6,
 // 448 = 1.75 * 2^8), from which the smallest power-of-two scale that holds a magnitude follows without a division.
+// encode: nearest code, ties to even, saturating; NaN gives code 0. encode4: four finite values within the code range, packed.
 struct KvInt8 {
     static constexpr uint32_t kMaxMant = 0x7E0000u;
     static constexpr int kMaxExp = 6;
-    // Nearest code, ties to even; NaN gives code 0 (its block's scale is NaN then and says so).
     static __device__ __forceinline__ uint32_t encode(float x) {
         return x == x ? (uint32_t)__float2int_rn(fminf(fmaxf(x, -127.f), 127.f)) & 0xffu : 0u;
+    }
+    static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+        // adding 1.5 * 2^23 rounds to an integer (to even) and leaves its two's complement in the low byte
+        const float r = 12582912.f;
+        const uint32_t x = __float_as_uint(__fadd_rn(a, r)), y = __float_as_uint(__fadd_rn(b, r)), z = __float_as_uint(__fadd_rn(c, r)),
+                       w = __float_as_uint(__fadd_rn(d, r));
+        return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
     }
     static __device__ __forceinline__ float decode(uint32_t byte) { return (float)(int8_t)byte; }
 };
@@ -24,6 +31,13 @@ struct KvE4m3 {
     static constexpr int kMaxExp = 8;
     static __device__ __forceinline__ uint32_t encode(float x) {
         return x == x ? (uint32_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3) : 0u;
+    }
+    static __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+        uint32_t w;
+        asm("{.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\tmov.b32 %0, {l, h};}"
+            : "=r"(w)
+            : "f"(a), "f"(b), "f"(c), "f"(d));
+        return w;
     }
     static __device__ __forceinline__ float decode(uint32_t byte) {
         return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));

@@ -48,7 +48,8 @@ struct RopeAppendParams {
     int64_t n_tokens, n_slots;
     int n_heads, n_kv_heads, head_dim, block_size, block_shift;
     int64_t blk_stride, pos_stride, head_stride, sc_blk_stride, sc_head_stride;
-    int kv_ctas, planes;                      // 8-bit pools: CTAs of the append role, (head, K or V) planes
+    int kv_ctas, planes, chunk, overlap;      // 8-bit pools: CTAs of the append role, (head, K or V) planes, tokens per CTA of a
+                                              // large step; two kernels side by side
     FastDiv by_cpr, by_groups;                // items of the other role: pieces per head, groups of heads per token
     int h0, h1, heads_per_item, pairs;        // heads [h0, h1) of q | k | v have work there; pairs: rotate_pairs takes them
 };
@@ -143,24 +144,70 @@ __device__ __forceinline__ void rotate_vec(const T* head, int rot, int interleav
 // warp of the first token of the call which lands in it (the leader), whatever order the tokens come in and however often a
 // slot is named. The owner needs the block's members: for each row, the last token of the call that names it.
 //   steps of up to kSmallStep tokens: a warp per (token, plane) looks through all slots itself; nothing is shared, no barrier.
-//   larger steps: a CTA takes kAppendChunk tokens of a plane, finds the leaders among them, and its threads look through all
+//   larger steps: a CTA takes kAppendChunk tokens of a KV head, finds the leaders among them, and its threads look through all
 //     slots once for all of its leaders' blocks. (256 tokens / one layer of the 14-head shape: 3.4 us against 5.4 for the CTA form;
 //     4096 tokens: a scan per leader and plane would read every slot 2,000 times.)
 constexpr int kSmallStep = 256;
 constexpr int kAppendChunk = 64;              // tokens per CTA of a large step
 constexpr int kAppendMaxBlock = 64;           // largest block size
-constexpr int kAppendWarps = 8;
+constexpr int kMembers = 4096;
+constexpr int kAppendWarps = 8, kLargeThreads = 512;
 
-template <typename KV> __device__ __forceinline__ uint2 encode8(const float (&x)[8]) {
+// What the owner of a block does with its scale: the magnitude of the written rows, the old scale and whether the call writes the
+// block's first row give the new one.
+struct Rescale {
+    float now, old, inv, ratio;
+    bool fresh, dead;                          // dead: the scale is NaN, every written code is 0
+    __device__ __forceinline__ bool grown() const { return !fresh && !(now == old); }
+};
+template <typename KV> __device__ __forceinline__ Rescale rescale(uint32_t amax, float old, bool fresh) {
+    Rescale r;
+    const float s_new = pow2_scale<KV>(amax);
+    r.old = old;
+    r.fresh = fresh;
+    r.now = fresh ? s_new : (old != old || s_new != s_new) ? __int_as_float(0x7fffffff) : fmaxf(old, s_new);
+    r.inv = 1.0f / r.now;
+    r.ratio = old / r.now;
+    r.dead = r.now != r.now;
+    return r;
+}
+__device__ __forceinline__ void note_max(uint32_t& amax, float x) { amax = max(amax, (uint32_t)__float_as_int(x) & 0x7fffffffu); }
+
+// Codes of 8 dims at dst: of a written row (x: its values), of a row the call does not write in a block it starts afresh, or of an
+// older row under a scale that grew (was: its codes, requested before any of the block's stores).
+__device__ __forceinline__ void old_codes(const uint8_t* src, int partner, uint2 (&was)[2]) {
+    was[0] = *reinterpret_cast<const uint2*>(src);
+    was[1] = *reinterpret_cast<const uint2*>(src + partner);
+}
+template <typename KV> __device__ __forceinline__ void put_codes8(uint8_t* dst, const Rescale& r, bool written, const float* x, uint2 was) {
+    if (!written && !r.fresh && !r.grown()) return;
     uint2 w = make_uint2(0u, 0u);
+    if (written) {
+        if (!r.dead) {
+            float y[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) (j < 4 ? w.x : w.y) |= KV::encode(x[j]) << (8 * (j & 3));
-    return w;
+            for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(x[j], r.inv);
+            w = make_uint2(KV::encode4(y[0], y[1], y[2], y[3]), KV::encode4(y[4], y[5], y[6], y[7]));
+        }
+    } else if (!r.fresh) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            (j < 4 ? w.x : w.y) |= KV::encode(__fmul_rn(KV::decode(((j < 4 ? was.x : was.y) >> (8 * (j & 3))) & 0xffu), r.ratio)) << (8 * (j & 3));
+    }
+    *reinterpret_cast<uint2*>(dst) = w;
+}
+template <typename KV, int V> __device__ __forceinline__ void put_codes(uint8_t* dst, const Rescale& r, bool written, const float* x) {
+    if constexpr (V == 8) {
+        put_codes8<KV>(dst, r, written, x, !written && r.grown() ? *reinterpret_cast<const uint2*>(dst) : make_uint2(0u, 0u));
+    } else {
+        if (!written && !r.fresh && !r.grown()) return;
+        *dst = (uint8_t)(written ? KV::encode(__fmul_rn(x[0], r.inv)) : r.fresh ? 0u : KV::encode(__fmul_rn(KV::decode(*dst), r.ratio)));
+    }
 }
 
-// One block of one plane by one warp. mem[row]: the token that writes the row, or -1. NI > 0: the block has NI * 32 pieces of V
-// dims, CPR per row, and the rotated values wait in registers for the scale; NI == 0: any sizes, the values are computed twice.
-template <typename T, typename KV, int V, int NI, int CPR>
+// One block of one plane by one warp, any sizes. mem[row]: the token that writes the row, or -1. The rotated values are computed
+// twice, for the magnitude and for the codes, from rows that the first pass left in the caches.
+template <typename T, typename KV, int V>
 __device__ __forceinline__ void append_block(const RopeAppendParams& p, int plane, int64_t blk, const int* mem) {
     const int lane = threadIdx.x & 31, head = plane >> 1, is_v = plane & 1, hd = p.head_dim, half = p.rot / 2;
     const T* src = reinterpret_cast<const T*>(is_v ? p.v : p.k) + (int64_t)head * hd;
@@ -168,8 +215,7 @@ __device__ __forceinline__ void append_block(const RopeAppendParams& p, int plan
     uint8_t* pool = reinterpret_cast<uint8_t*>(is_v ? p.v_pool : p.k_pool) + head * p.head_stride + blk * p.blk_stride;
     float* sc = (is_v ? p.v_scale : p.k_scale) + head * p.sc_head_stride + blk * p.sc_blk_stride;
     const float old = *sc;
-    const bool fresh = mem[0] >= 0;
-    const int cpr = NI > 0 ? CPR : hd / V, items = NI > 0 ? NI * 32 : p.block_size * cpr;
+    const int cpr = hd / V, items = p.block_size * cpr;
     auto values = [&](int t, int d0, float (&x)[V]) {
         const T* row = src + t * src_stride;
         if (!is_v && d0 < p.rot) {
@@ -181,78 +227,97 @@ __device__ __forceinline__ void append_block(const RopeAppendParams& p, int plan
             load_vec<T, V>(row + d0, x);
         }
     };
-    float kept[NI > 0 ? NI : 1][V];
     uint32_t amax = 0;
-    if constexpr (NI > 0) {
+#pragma unroll 2
+    for (int i = lane; i < items; i += 32) {
+        const int off = i / cpr, t = mem[off];
+        if (t < 0) continue;
+        float x[V];
+        values(t, (i - off * cpr) * V, x);
 #pragma unroll
-        for (int n = 0; n < NI; ++n) {
-            const int i = n * 32 + lane, t = mem[i / CPR];
-            if (t >= 0) values(t, (i % CPR) * V, kept[n]);
-            if (n & 1) asm volatile("" ::: "memory");            // two rows' loads at a time: all of them would not fit the registers
-        }
-#pragma unroll
-        for (int n = 0; n < NI; ++n) {
-            if (mem[(n * 32 + lane) / CPR] < 0) continue;
-#pragma unroll
-            for (int j = 0; j < V; ++j) amax = max(amax, (uint32_t)__float_as_int(kept[n][j]) & 0x7fffffffu);
-        }
-    } else {
-        for (int i = lane; i < items; i += 32) {
-            const int off = i / cpr, t = mem[off];
-            if (t < 0) continue;
-            values(t, (i - off * cpr) * V, kept[0]);
-#pragma unroll
-            for (int j = 0; j < V; ++j) amax = max(amax, (uint32_t)__float_as_int(kept[0][j]) & 0x7fffffffu);
-        }
+        for (int j = 0; j < V; ++j) note_max(amax, x[j]);
     }
-    amax = __reduce_max_sync(0xffffffffu, amax);
-    const float s_new = pow2_scale<KV>(amax);
-    const float now = fresh ? s_new : (old != old || s_new != s_new) ? __int_as_float(0x7fffffff) : fmaxf(old, s_new);
-    const float inv = 1.0f / now, ratio = old / now;
+    const Rescale r = rescale<KV>(__reduce_max_sync(0xffffffffu, amax), old, mem[0] >= 0);
     __syncwarp();
-    if (lane == 0 && now != old) *sc = now;
-    auto put = [&](int off, int d0, int t, float (&x)[V]) {      // x: the row's values if a token writes it
-        uint8_t* dst = pool + (int64_t)off * p.pos_stride + d0;
+    if (lane == 0 && !(r.now == old)) *sc = r.now;
+#pragma unroll 2
+    for (int i = lane; i < items; i += 32) {
+        const int off = i / cpr, t = mem[off], d0 = (i - off * cpr) * V;
+        float x[V];
+        if (t >= 0) values(t, d0, x);
+        put_codes<KV, V>(pool + (int64_t)off * p.pos_stride + d0, r, t >= 0, x);
+    }
+}
+
+// The same for blocks of 16 rows of 64 or 128 dims, half layout, whole head rotated (the framework's models): a lane takes 8 dims of
+// the low half of a row together with their partners, so each row is read once, and keeps the values for the codes.
+template <typename T, typename KV, int HD>
+__device__ __forceinline__ void append_block_pairs(const RopeAppendParams& p, int plane, int64_t blk, const int* mem) {
+    constexpr int CPR = HD / 16, NI = 16 * CPR / 32;          // pairs of pieces per row, per lane
+    const int lane = threadIdx.x & 31, head = plane >> 1, is_v = plane & 1;
+    const T* src = reinterpret_cast<const T*>(is_v ? p.v : p.k) + (int64_t)head * HD;
+    const int64_t src_stride = is_v ? p.v_stride : p.k_stride;
+    uint8_t* pool = reinterpret_cast<uint8_t*>(is_v ? p.v_pool : p.k_pool) + head * p.head_stride + blk * p.blk_stride;
+    float* sc = (is_v ? p.v_scale : p.k_scale) + head * p.sc_head_stride + blk * p.sc_blk_stride;
+    const float old = *sc;
+    const int row0 = lane / CPR, d0 = (lane % CPR) * 8;                            // row n * (32 / CPR) + row0 of item n
+    float lo[NI][8], hi[NI][8];
+    uint32_t amax = 0;
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+        const int t = mem[n * (32 / CPR) + row0];
         if (t >= 0) {
+            const T* row = src + t * src_stride + d0;
+            load_vec<T, 8>(row, lo[n]);
+            load_vec<T, 8>(row + HD / 2, hi[n]);
+            if (!is_v) {
+                const float* cr = p.cos + (int64_t)t * (HD / 2) + d0;
+                const float* sr = p.sin + (int64_t)t * (HD / 2) + d0;
 #pragma unroll
-            for (int j = 0; j < V; ++j) x[j] = __fmul_rn(x[j], inv);
-        } else if (fresh) {
+                for (int w = 0; w < 2; ++w) {
+                    const float4 c4 = *reinterpret_cast<const float4*>(cr + 4 * w), s4 = *reinterpret_cast<const float4*>(sr + 4 * w);
+                    const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-            for (int j = 0; j < V; ++j) x[j] = 0.f;
-        } else if (now == old) {
-            return;
-        } else if constexpr (V == 1) {
-            x[0] = __fmul_rn(KV::decode(dst[0]), ratio);
-        } else {
-            const uint2 w = *reinterpret_cast<const uint2*>(dst);
+                    for (int j = 0; j < 4; ++j) {
+                        const float a = lo[n][4 * w + j], b = hi[n][4 * w + j];
+                        lo[n][4 * w + j] = __fsub_rn(__fmul_rn(a, c[j]), __fmul_rn(b, s[j]));
+                        hi[n][4 * w + j] = __fadd_rn(__fmul_rn(b, c[j]), __fmul_rn(a, s[j]));
+                    }
+                }
+            }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(KV::decode(((j < 4 ? w.x : w.y) >> (8 * (j & 3))) & 0xffu), ratio);
+            for (int j = 0; j < 8; ++j) {
+                note_max(amax, lo[n][j]);
+                note_max(amax, hi[n][j]);
+            }
         }
-        if constexpr (V == 1) dst[0] = (uint8_t)KV::encode(x[0]);
-        else *reinterpret_cast<uint2*>(dst) = encode8<KV>(x);
-    };
-    if constexpr (NI > 0) {
+        if (n & 1) asm volatile("" ::: "memory");            // two rows' loads at a time: all of them would not fit the registers
+    }
+    const Rescale r = rescale<KV>(__reduce_max_sync(0xffffffffu, amax), old, mem[0] >= 0);
+    __syncwarp();
+    if (lane == 0 && !(r.now == old)) *sc = r.now;
+    uint2 was[NI][2];
+    if (r.grown()) {
 #pragma unroll
-        for (int n = 0; n < NI; ++n) {
-            const int i = n * 32 + lane;
-            put(i / CPR, (i % CPR) * V, mem[i / CPR], kept[n]);
-        }
-    } else {
-        for (int i = lane; i < items; i += 32) {
-            const int off = i / cpr, t = mem[off], d0 = (i - off * cpr) * V;
-            if (t >= 0) values(t, d0, kept[0]);
-            put(off, d0, t, kept[0]);
-        }
+        for (int n = 0; n < NI; ++n) old_codes(pool + (int64_t)(n * (32 / CPR) + row0) * p.pos_stride + d0, HD / 2, was[n]);
+    }
+#pragma unroll
+    for (int n = 0; n < NI; ++n) {
+        const int off = n * (32 / CPR) + row0;
+        uint8_t* dst = pool + (int64_t)off * p.pos_stride + d0;
+        const bool written = mem[off] >= 0;
+        put_codes8<KV>(dst, r, written, lo[n], was[n][0]);
+        put_codes8<KV>(dst + HD / 2, r, written, hi[n], was[n][1]);
     }
 }
 
 template <typename T, typename KV, int V>
 __device__ __forceinline__ void append_any(const RopeAppendParams& p, int plane, int64_t blk, const int* mem) {
-    if constexpr (V == 8) {                      // the layouts of the framework's models; the others by the loop
-        if (p.block_size == 16 && p.head_dim == 64) return append_block<T, KV, V, 4, 8>(p, plane, blk, mem);
-        if (p.block_size == 16 && p.head_dim == 128) return append_block<T, KV, V, 8, 16>(p, plane, blk, mem);
+    if constexpr (V == 8) {
+        if (p.pairs && p.block_size == 16 && p.head_dim == 64) return append_block_pairs<T, KV, 64>(p, plane, blk, mem);
+        if (p.pairs && p.block_size == 16 && p.head_dim == 128) return append_block_pairs<T, KV, 128>(p, plane, blk, mem);
     }
-    append_block<T, KV, V, 0, 1>(p, plane, blk, mem);
+    append_block<T, KV, V>(p, plane, blk, mem);
 }
 
 __device__ __forceinline__ int block_of(const RopeAppendParams& p, int64_t slot) {
@@ -297,18 +362,111 @@ template <typename T, typename KV, int V> __device__ void append_small(const Rop
     append_any<T, KV, V>(p, plane, b, mem);
 }
 
-// A CTA per (chunk of tokens, plane).
-template <typename T, typename KV, int V> __device__ void append_large(const RopeAppendParams& p, int cta) {
-    __shared__ int member[kAppendChunk * kAppendMaxBlock];
-    __shared__ int cand_block[kAppendChunk], cand_tok[kAppendChunk], cand_dead[kAppendChunk];
-    __shared__ int n_cand;
-    const int tid = threadIdx.x, warp = tid >> 5;
-    const int plane = cta % p.planes, bs = p.block_size, mask = bs - 1;
-    const int t0 = (cta / p.planes) * kAppendChunk, n_tok = (int)p.n_tokens;
-    if (tid == 0) n_cand = 0;
-    for (int i = tid; i < kAppendChunk * bs; i += blockDim.x) member[i] = -1;
+// The blocks of a CTA's candidates, K and V, by all of its warps: the layouts of append_block_pairs. A step is a warp's share of a
+// unit (candidate, K or V): 32 pairs of pieces. First the magnitudes, then the scales, then the codes (the rotated values are
+// computed again, from rows that the first pass left in the caches).
+template <typename T, typename KV, int HD>
+__device__ __forceinline__ void append_units(const RopeAppendParams& p, int head, int nc, const int* cand_block, const int* cand_dead, const int* member,
+                                             uint32_t* unit_max, Rescale* unit_scale) {
+    constexpr int CPR = HD / 16, NI = 16 * CPR / 32, B = 4, NW = kLargeThreads / 32;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int row0 = lane / CPR, d0 = (lane % CPR) * 8;
+    const int units = 2 * nc, steps = units * NI;
+    float old = 0.f;
+    auto scale_of = [&](int u) -> float* {
+        return ((u & 1) ? p.v_scale : p.k_scale) + head * p.sc_head_stride + (int64_t)cand_block[u >> 1] * p.sc_blk_stride;
+    };
+    for (int u = tid; u < units; u += kLargeThreads) unit_max[u] = 0;
+    if (tid < units) old = *scale_of(tid);
     __syncthreads();
-    if (tid < kAppendChunk && t0 + tid < n_tok) {
+    auto pair_values = [&](int t, bool is_v, float (&lo)[8], float (&hi)[8]) {
+        const T* row = reinterpret_cast<const T*>(is_v ? p.v : p.k) + (int64_t)head * HD + t * (is_v ? p.v_stride : p.k_stride) + d0;
+        load_vec<T, 8>(row, lo);
+        load_vec<T, 8>(row + HD / 2, hi);
+        if (is_v) return;
+        const float* cr = p.cos + (int64_t)t * (HD / 2) + d0;
+        const float* sr = p.sin + (int64_t)t * (HD / 2) + d0;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const float4 c4 = *reinterpret_cast<const float4*>(cr + 4 * w), s4 = *reinterpret_cast<const float4*>(sr + 4 * w);
+            const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float a = lo[4 * w + j], b = hi[4 * w + j];
+                lo[4 * w + j] = __fsub_rn(__fmul_rn(a, c[j]), __fmul_rn(b, s[j]));
+                hi[4 * w + j] = __fadd_rn(__fmul_rn(b, c[j]), __fmul_rn(a, s[j]));
+            }
+        }
+    };
+#pragma unroll 2
+    for (int st = warp; st < steps; st += NW) {
+        const int u = st / NI, c = u >> 1, t = member[c * 16 + (st % NI) * (32 / CPR) + row0];
+        if (cand_dead[c] || !__any_sync(0xffffffffu, t >= 0)) continue;
+        uint32_t amax = 0;
+        if (t >= 0) {
+            float lo[8], hi[8];
+            pair_values(t, u & 1, lo, hi);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                note_max(amax, lo[j]);
+                note_max(amax, hi[j]);
+            }
+        }
+        amax = __reduce_max_sync(0xffffffffu, amax);
+        if (lane == 0) atomicMax(&unit_max[u], amax);
+    }
+    __syncthreads();
+    for (int u = tid; u < units; u += kLargeThreads) {
+        if (cand_dead[u >> 1]) continue;
+        const float was = u == tid ? old : *scale_of(u);
+        const Rescale r = rescale<KV>(unit_max[u], was, member[(u >> 1) * 16] >= 0);
+        unit_scale[u] = r;
+        if (!(r.now == was)) *scale_of(u) = r.now;
+    }
+    __syncthreads();
+    for (int st0 = warp; st0 < steps; st0 += B * NW) {
+        uint2 was[B][2];
+#pragma unroll
+        for (int k = 0; k < B; ++k) {
+            const int st = st0 + k * NW, u = st / NI, c = u >> 1, off = (st % NI) * (32 / CPR) + row0;
+            if (st >= steps || cand_dead[c] || !unit_scale[u].grown() || member[c * 16 + off] >= 0) continue;
+            old_codes(reinterpret_cast<const uint8_t*>((u & 1) ? p.v_pool : p.k_pool) + head * p.head_stride + cand_block[c] * p.blk_stride +
+                          off * p.pos_stride + d0, HD / 2, was[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < B; ++k) {
+            const int st = st0 + k * NW, u = st / NI, c = u >> 1, off = (st % NI) * (32 / CPR) + row0;
+            if (st >= steps || cand_dead[c]) continue;
+            const Rescale r = unit_scale[u];
+            const int t = member[c * 16 + off];
+            float lo[8], hi[8];
+            if (t >= 0) pair_values(t, u & 1, lo, hi);
+            uint8_t* dst = reinterpret_cast<uint8_t*>((u & 1) ? p.v_pool : p.k_pool) + head * p.head_stride + cand_block[c] * p.blk_stride +
+                           off * p.pos_stride + d0;
+            put_codes8<KV>(dst, r, t >= 0, lo, was[k][0]);
+            put_codes8<KV>(dst + HD / 2, r, t >= 0, hi, was[k][1]);
+        }
+    }
+}
+
+// A CTA per (chunk of tokens, KV head): K and V share the search for the members.
+template <typename T, typename KV, int V> __device__ void append_large(const RopeAppendParams& p, int cta) {
+    __shared__ int member[kMembers];
+    __shared__ int cand_block[kAppendChunk], cand_tok[kAppendChunk], cand_dead[kAppendChunk];
+    __shared__ int key[4 * kAppendChunk], val[4 * kAppendChunk];          // block -> candidate, open addressing, a quarter full at most
+    __shared__ int n_cand;
+    __shared__ uint32_t unit_max[2 * kAppendChunk];
+    __shared__ Rescale unit_scale[2 * kAppendChunk];
+    constexpr int kSlotsOfTable = 4 * kAppendChunk;
+    const int tid = threadIdx.x, warp = tid >> 5;
+    const int head = cta % p.n_kv_heads, bs = p.block_size, mask = bs - 1;
+    const int t0 = (cta / p.n_kv_heads) * p.chunk, n_tok = (int)p.n_tokens;
+    auto hash = [](int b) -> int { return (int)(((uint32_t)b * 2654435761u) >> 16) & (kSlotsOfTable - 1); };
+    if (tid == 0) n_cand = 0;
+    for (int i = tid; i < p.chunk * bs; i += blockDim.x) member[i] = -1;
+    for (int i = tid; i < kSlotsOfTable; i += blockDim.x) key[i] = -1;
+    __syncthreads();
+    if (tid < p.chunk && t0 + tid < n_tok) {
         const int t = t0 + tid, b = block_of(p, p.slots[t]);
         if (b >= 0 && (t == 0 || block_of(p, p.slots[t - 1]) != b)) {
             const int c = atomicAdd(&n_cand, 1);
@@ -319,24 +477,50 @@ template <typename T, typename KV, int V> __device__ void append_large(const Rop
     }
     __syncthreads();
     const int nc = n_cand;
-    for (int base = tid; base < n_tok; base += 4 * blockDim.x) {          // four slots in flight
+    // Of two candidates with one block the earlier token's is the owner; the table keeps that one (ends: fewer entries than places).
+    if (tid < nc) {
+        const int b = cand_block[tid];
+        for (int h = hash(b);; h = (h + 1) & (kSlotsOfTable - 1)) {
+            const int was = atomicCAS(&key[h], -1, b);
+            if (was == -1 || was == b) break;
+        }
+    }
+    for (int i = tid; i < kSlotsOfTable; i += blockDim.x) val[i] = 0x7fffffff;
+    __syncthreads();
+    auto find = [&](int b) -> int {                                       // place of block b, -1 if it is no candidate's
+        for (int h = hash(b);; h = (h + 1) & (kSlotsOfTable - 1)) {
+            const int k = key[h];
+            if (k == b) return h;
+            if (k == -1) return -1;
+        }
+    };
+    if (tid < nc) atomicMin(&val[find(cand_block[tid])], cand_tok[tid] << 8 | tid);      // (the token decides; kAppendChunk <= 256)
+    __syncthreads();
+    if (tid < nc && (val[find(cand_block[tid])] & 255) != tid) cand_dead[tid] = 1;
+    __syncthreads();
+    for (int base = tid; base < n_tok; base += 4 * kLargeThreads) {       // four slots in flight
         int64_t slot[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) slot[k] = base + k * (int)blockDim.x < n_tok ? p.slots[base + k * (int)blockDim.x] : -1;
+        for (int k = 0; k < 4; ++k) slot[k] = base + k * kLargeThreads < n_tok ? p.slots[base + k * kLargeThreads] : -1;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int t = base + k * (int)blockDim.x, b = block_of(p, slot[k]);
-            if (b < 0) continue;
-            for (int c = 0; c < nc; ++c)
-                if (cand_block[c] == b) {
-                    if (t < cand_tok[c]) cand_dead[c] = 1;
-                    else atomicMax(&member[c * bs + ((int)slot[k] & mask)], t);
-                }
+            const int t = base + k * kLargeThreads, b = block_of(p, slot[k]);
+            const int at = b < 0 ? -1 : find(b);
+            if (at < 0) continue;
+            const int c = val[at] & 255;
+            if (t < cand_tok[c]) cand_dead[c] = 1;                        // an earlier token owns the block
+            else atomicMax(&member[c * bs + ((int)slot[k] & mask)], t);
         }
     }
     __syncthreads();
-    for (int c = warp; c < nc; c += kAppendWarps)
-        if (!cand_dead[c]) append_any<T, KV, V>(p, plane, cand_block[c], member + c * bs);
+    if constexpr (V == 8) {
+        if (p.pairs && bs == 16 && p.head_dim == 64) return append_units<T, KV, 64>(p, head, nc, cand_block, cand_dead, member, unit_max, unit_scale);
+        if (p.pairs && bs == 16 && p.head_dim == 128) return append_units<T, KV, 128>(p, head, nc, cand_block, cand_dead, member, unit_max, unit_scale);
+    }
+    for (int i = warp; i < 2 * nc; i += kLargeThreads / 32) {
+        const int c = i >> 1;
+        if (!cand_dead[c]) append_block<T, KV, V>(p, 2 * head + (i & 1), cand_block[c], member + c * bs);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ the kernel
@@ -415,30 +599,18 @@ template <typename T, bool kv8> __device__ __forceinline__ void rotate_pairs(con
     }
 }
 
-// CTAs [0, kv_ctas): the append role (8-bit pools). The others walk (token, V dims, group of heads): the angles of the V dims are
-// loaded once per group.
-template <typename T, typename KV, int V>
-__global__ void __launch_bounds__(kAppendWarps * 32, 2) rope_append_kernel(const RopeAppendParams p) {
-    constexpr bool kv8 = !std::is_same<KV, NoKv8>::value;
-    pdl_launch_dependents();
-    pdl_wait();
-    if constexpr (kv8) {
-        if ((int)blockIdx.x < p.kv_ctas) {
-            if (p.n_tokens <= kSmallStep) append_small<T, KV, V>(p, blockIdx.x);
-            else append_large<T, KV, V>(p, blockIdx.x);
-            return;
-        }
-    }
+// Items are (token, V dims, group of heads): the angles of the V dims are loaded once per group.
+template <typename T, bool kv8, int V> __device__ __forceinline__ void rotate_rows(const RopeAppendParams& p, int cta, int ctas) {
     if constexpr (V == 8) {
         if (p.pairs) {
-            rotate_pairs<T, kv8>(p, blockIdx.x - p.kv_ctas, gridDim.x - p.kv_ctas);
+            rotate_pairs<T, kv8>(p, cta, ctas);
             return;
         }
     }
     const int hd = p.head_dim, cpr = hd / V, half = p.rot / 2, NH = p.n_heads, NKV = p.n_kv_heads;
     const bool pool16 = !kv8 && p.k_pool != nullptr;
     const uint32_t total = (uint32_t)p.n_tokens * p.by_groups.div * cpr;
-    for (uint32_t i = (blockIdx.x - p.kv_ctas) * blockDim.x + threadIdx.x; i < total; i += (gridDim.x - p.kv_ctas) * blockDim.x) {
+    for (uint32_t i = cta * blockDim.x + threadIdx.x; i < total; i += ctas * blockDim.x) {
         const uint32_t tg = p.by_cpr.quot(i);
         const int d0 = (int)(i - tg * cpr) * V;
         const int64_t t = p.by_groups.quot(tg);
@@ -471,9 +643,34 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 2) rope_append_kernel(const
     }
 }
 
+// 16/32-bit pools, and the queries of a large step over an 8-bit pool.
+template <typename T, bool kv8, int V> __global__ void __launch_bounds__(kAppendWarps * 32, 3) rope_rows_kernel(const RopeAppendParams p) {
+    if (!p.overlap) pdl_launch_dependents();
+    pdl_wait();
+    if (p.overlap) pdl_launch_dependents();       // the append kernel of the same call may start: it reads the same inputs
+    rotate_rows<T, kv8, V>(p, blockIdx.x, gridDim.x);
+}
+// A small step over an 8-bit pool, in one launch: CTAs [0, kv_ctas) append, the others take the queries.
+template <typename T, typename KV, int V> __global__ void __launch_bounds__(kAppendWarps * 32, 2) rope_append_small_kernel(const RopeAppendParams p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    if ((int)blockIdx.x < p.kv_ctas) append_small<T, KV, V>(p, blockIdx.x);
+    else rotate_rows<T, true, V>(p, blockIdx.x - p.kv_ctas, gridDim.x - p.kv_ctas);
+}
+// The append of a large step. It runs beside rope_rows_kernel, which was launched just before it and lets it start once the
+// call's inputs exist; it completes after that kernel, so that the next one waits for both.
+template <typename T, typename KV, int V> __global__ void __launch_bounds__(kLargeThreads, 2) append_large_kernel(const RopeAppendParams p) {
+    if (!p.overlap) {
+        pdl_launch_dependents();
+        pdl_wait();
+    }
+    append_large<T, KV, V>(p, blockIdx.x);
+    if (p.overlap) pdl_wait();
+}
+
 template <typename T, typename KV, int V> static int launch_rope_append(RopeAppendParams p, cudaStream_t st) {
     constexpr bool kv8 = !std::is_same<KV, NoKv8>::value;
-    const int threads = kAppendWarps * 32;
+    const dim3 threads(kAppendWarps * 32);
     int sms = device_sm_count();
     if (sms <= 0) sms = 148;
     p.planes = 2 * p.n_kv_heads;
@@ -482,23 +679,28 @@ template <typename T, typename KV, int V> static int launch_rope_append(RopeAppe
     p.pairs = V == 8 && !p.interleaved && p.rot == p.head_dim;
     p.heads_per_item = p.pairs && sizeof(T) == 4 ? 2 : 4;
     const int64_t groups = p.h1 > p.h0 ? (p.h1 - p.h0 + p.heads_per_item - 1) / p.heads_per_item : 0, cpr = p.head_dim / (p.pairs ? 2 * V : V);
-    p.kv_ctas = 0;
-    if (kv8) {
-        const int64_t n = p.n_tokens <= kSmallStep ? (p.n_tokens * p.planes + kAppendWarps - 1) / kAppendWarps
-                                                   : (p.n_tokens + kAppendChunk - 1) / kAppendChunk * p.planes;
-        NS_REQUIRE(n < (1 << 30), NS_ERR_UNSUPPORTED, "rope_append: %lld tokens", (long long)p.n_tokens);
-        p.kv_ctas = (int)n;
-    }
     const int64_t items = p.n_tokens * groups * cpr;
     NS_REQUIRE(items < ((int64_t)1 << 31), NS_ERR_UNSUPPORTED, "rope_append: %lld tokens", (long long)p.n_tokens);
     if (groups > 0) {
         p.by_cpr = FastDiv((uint32_t)cpr);
         p.by_groups = FastDiv((uint32_t)groups);
     }
-    int64_t ctas = (items + threads - 1) / threads;
-    if (ctas > sms * 16) ctas = sms * 16;
-    if (ctas + p.kv_ctas == 0) return NS_OK;
-    cudaError_t e = launch_pdl(rope_append_kernel<T, KV, V>, dim3((unsigned)(ctas + p.kv_ctas)), dim3(threads), 0, st, p);
+    int64_t ctas = (items + threads.x - 1) / threads.x;
+    if (ctas > sms * 12) ctas = sms * 12;
+    cudaError_t e = cudaSuccess;
+    if constexpr (!kv8) {
+        if (ctas > 0) e = launch_pdl(rope_rows_kernel<T, false, V>, dim3((unsigned)ctas), threads, 0, st, p);
+    } else if (p.n_tokens <= kSmallStep) {
+        p.kv_ctas = (int)((p.n_tokens * p.planes + kAppendWarps - 1) / kAppendWarps);
+        e = launch_pdl(rope_append_small_kernel<T, KV, V>, dim3((unsigned)(ctas + p.kv_ctas)), threads, 0, st, p);
+    } else {
+        p.chunk = kAppendChunk;
+        const int64_t n = (p.n_tokens + p.chunk - 1) / p.chunk * p.n_kv_heads;
+        NS_REQUIRE(n < (1 << 30), NS_ERR_UNSUPPORTED, "rope_append: %lld tokens", (long long)p.n_tokens);
+        p.overlap = ctas > 0 ? 1 : 0;
+        if (ctas > 0) e = launch_pdl(rope_rows_kernel<T, true, V>, dim3((unsigned)ctas), threads, 0, st, p);
+        if (e == cudaSuccess) e = launch_pdl(append_large_kernel<T, KV, V>, dim3((unsigned)n), dim3(kLargeThreads), 0, st, p);
+    }
     if (e != cudaSuccess) return fail(NS_ERR_CUDA, "rope_append: launch failed: %s", cudaGetErrorString(e));
     return NS_OK;
 }
@@ -592,7 +794,7 @@ extern "C" int ns_rope_append(const void* q, const void* k, const void* v, int64
         NS_REQUIRE(k_scale && v_scale, NS_ERR_INVALID_ARG, "rope_append: an 8-bit pool needs its scales");
         NS_REQUIRE(block_size <= kAppendMaxBlock && (block_size & (block_size - 1)) == 0, NS_ERR_UNSUPPORTED,
                    "rope_append: 8-bit pools take blocks of 1, 2, 4 ... %d tokens, not %d", kAppendMaxBlock, block_size);
-        NS_REQUIRE(n_tokens <= (1 << 24) && n_slots < ((int64_t)1 << 31), NS_ERR_UNSUPPORTED, "rope_append: %lld tokens / %lld slots",
+        NS_REQUIRE(n_tokens < (1 << 23) && n_slots < ((int64_t)1 << 31), NS_ERR_UNSUPPORTED, "rope_append: %lld tokens / %lld slots",
                    (long long)n_tokens, (long long)n_slots);
     }
     RopeAppendParams p = {};
