@@ -25,6 +25,12 @@ struct KvInt8 {
         return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
     }
     static __device__ __forceinline__ float decode(uint32_t byte) { return (float)(int8_t)byte; }
+    static __device__ __forceinline__ void decode4(uint32_t w, float (&x)[4]) {
+        const uint32_t u = w ^ 0x80808080u;                // 0 .. 255: under the exponent of 2^23, less 2^23 + 128
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 | j)) - 8388736.f;
+    }
+    static __device__ __forceinline__ uint32_t without_nan(uint32_t w) { return w; }
 };
 struct KvE4m3 {
     static constexpr uint32_t kMaxMant = 0x600000u;
@@ -41,6 +47,16 @@ struct KvE4m3 {
     }
     static __device__ __forceinline__ float decode(uint32_t byte) {
         return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)byte, __NV_E4M3)));
+    }
+    static __device__ __forceinline__ void decode4(uint32_t w, float (&x)[4]) {
+        uint32_t lo, hi;
+        asm("{.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;}" : "=r"(lo), "=r"(hi) : "r"(w));
+        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo)), b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+    }
+    // NaN codes (0x7f under either sign) become code 0.
+    static __device__ __forceinline__ uint32_t without_nan(uint32_t w) {
+        return w & ~(((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu);
     }
 };
 

@@ -148,10 +148,10 @@ __device__ __forceinline__ void rotate_vec(const T* head, int rot, int interleav
 //     slots once for all of its leaders' blocks. (256 tokens / one layer of the 14-head shape: 3.4 us against 5.4 for the CTA form;
 //     4096 tokens: a scan per leader and plane would read every slot 2,000 times.)
 constexpr int kSmallStep = 256;
-constexpr int kAppendChunk = 64;              // tokens per CTA of a large step
+constexpr int kAppendChunk = 16;              // tokens per CTA of a large step
 constexpr int kAppendMaxBlock = 64;           // largest block size
-constexpr int kMembers = 4096;
-constexpr int kAppendWarps = 8, kLargeThreads = 512;
+constexpr int kMembers = kAppendChunk * kAppendMaxBlock;
+constexpr int kAppendWarps = 8, kLargeThreads = 256;
 
 // What the owner of a block does with its scale: the magnitude of the written rows, the old scale and whether the call writes the
 // block's first row give the new one.
@@ -189,10 +189,15 @@ template <typename KV> __device__ __forceinline__ void put_codes8(uint8_t* dst, 
             for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(x[j], r.inv);
             w = make_uint2(KV::encode4(y[0], y[1], y[2], y[3]), KV::encode4(y[4], y[5], y[6], y[7]));
         }
-    } else if (!r.fresh) {
+    } else if (!r.fresh && r.ratio < 1.f) {                // (a scale that became NaN, or grew from a NaN: code 0; ratio < 1: no overflow)
+        auto again = [&](uint32_t v) -> uint32_t {
+            float y[4];
+            KV::decode4(KV::without_nan(v), y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            (j < 4 ? w.x : w.y) |= KV::encode(__fmul_rn(KV::decode(((j < 4 ? was.x : was.y) >> (8 * (j & 3))) & 0xffu), r.ratio)) << (8 * (j & 3));
+            for (int j = 0; j < 4; ++j) y[j] = __fmul_rn(y[j], r.ratio);
+            return KV::encode4(y[0], y[1], y[2], y[3]);
+        };
+        w = make_uint2(again(was.x), again(was.y));
     }
     *reinterpret_cast<uint2*>(dst) = w;
 }
@@ -368,7 +373,7 @@ template <typename T, typename KV, int V> __device__ void append_small(const Rop
 template <typename T, typename KV, int HD>
 __device__ __forceinline__ void append_units(const RopeAppendParams& p, int head, int nc, const int* cand_block, const int* cand_dead, const int* member,
                                              uint32_t* unit_max, Rescale* unit_scale) {
-    constexpr int CPR = HD / 16, NI = 16 * CPR / 32, B = 4, NW = kLargeThreads / 32;
+    constexpr int CPR = HD / 16, NI = 16 * CPR / 32, B = 2, NW = kLargeThreads / 32;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int row0 = lane / CPR, d0 = (lane % CPR) * 8;
     const int units = 2 * nc, steps = units * NI;
@@ -425,26 +430,28 @@ __device__ __forceinline__ void append_units(const RopeAppendParams& p, int head
     }
     __syncthreads();
     for (int st0 = warp; st0 < steps; st0 += B * NW) {
-        uint2 was[B][2];
+        uint2 was[B][2];                                  // all loads of B steps before the first store
+        float lo[B][8], hi[B][8];
+        auto dst_of = [&](int c, int u, int off) -> uint8_t* {
+            return reinterpret_cast<uint8_t*>((u & 1) ? p.v_pool : p.k_pool) + head * p.head_stride + cand_block[c] * p.blk_stride + off * p.pos_stride + d0;
+        };
 #pragma unroll
         for (int k = 0; k < B; ++k) {
             const int st = st0 + k * NW, u = st / NI, c = u >> 1, off = (st % NI) * (32 / CPR) + row0;
-            if (st >= steps || cand_dead[c] || !unit_scale[u].grown() || member[c * 16 + off] >= 0) continue;
-            old_codes(reinterpret_cast<const uint8_t*>((u & 1) ? p.v_pool : p.k_pool) + head * p.head_stride + cand_block[c] * p.blk_stride +
-                          off * p.pos_stride + d0, HD / 2, was[k]);
+            if (st >= steps || cand_dead[c]) continue;
+            const int t = member[c * 16 + off];
+            if (t >= 0) pair_values(t, u & 1, lo[k], hi[k]);
+            else if (unit_scale[u].grown()) old_codes(dst_of(c, u, off), HD / 2, was[k]);
         }
 #pragma unroll
         for (int k = 0; k < B; ++k) {
             const int st = st0 + k * NW, u = st / NI, c = u >> 1, off = (st % NI) * (32 / CPR) + row0;
             if (st >= steps || cand_dead[c]) continue;
             const Rescale r = unit_scale[u];
-            const int t = member[c * 16 + off];
-            float lo[8], hi[8];
-            if (t >= 0) pair_values(t, u & 1, lo, hi);
-            uint8_t* dst = reinterpret_cast<uint8_t*>((u & 1) ? p.v_pool : p.k_pool) + head * p.head_stride + cand_block[c] * p.blk_stride +
-                           off * p.pos_stride + d0;
-            put_codes8<KV>(dst, r, t >= 0, lo, was[k][0]);
-            put_codes8<KV>(dst + HD / 2, r, t >= 0, hi, was[k][1]);
+            const bool written = member[c * 16 + off] >= 0;
+            uint8_t* dst = dst_of(c, u, off);
+            put_codes8<KV>(dst, r, written, lo[k], was[k][0]);
+            put_codes8<KV>(dst + HD / 2, r, written, hi[k], was[k][1]);
         }
     }
 }
@@ -455,6 +462,7 @@ template <typename T, typename KV, int V> __device__ void append_large(const Rop
     __shared__ int cand_block[kAppendChunk], cand_tok[kAppendChunk], cand_dead[kAppendChunk];
     __shared__ int key[4 * kAppendChunk], val[4 * kAppendChunk];          // block -> candidate, open addressing, a quarter full at most
     __shared__ int n_cand;
+    __shared__ uint32_t filter;
     __shared__ uint32_t unit_max[2 * kAppendChunk];
     __shared__ Rescale unit_scale[2 * kAppendChunk];
     constexpr int kSlotsOfTable = 4 * kAppendChunk;
@@ -462,7 +470,7 @@ template <typename T, typename KV, int V> __device__ void append_large(const Rop
     const int head = cta % p.n_kv_heads, bs = p.block_size, mask = bs - 1;
     const int t0 = (cta / p.n_kv_heads) * p.chunk, n_tok = (int)p.n_tokens;
     auto hash = [](int b) -> int { return (int)(((uint32_t)b * 2654435761u) >> 16) & (kSlotsOfTable - 1); };
-    if (tid == 0) n_cand = 0;
+    if (tid == 0) n_cand = 0, filter = 0;
     for (int i = tid; i < p.chunk * bs; i += blockDim.x) member[i] = -1;
     for (int i = tid; i < kSlotsOfTable; i += blockDim.x) key[i] = -1;
     __syncthreads();
@@ -473,10 +481,12 @@ template <typename T, typename KV, int V> __device__ void append_large(const Rop
             cand_block[c] = b;
             cand_tok[c] = t;
             cand_dead[c] = 0;
+            atomicOr(&filter, 1u << (b & 31));
         }
     }
     __syncthreads();
     const int nc = n_cand;
+    if (nc == 0) return;                                                  // (the chunk's blocks began in an earlier one)
     // Of two candidates with one block the earlier token's is the owner; the table keeps that one (ends: fewer entries than places).
     if (tid < nc) {
         const int b = cand_block[tid];
@@ -498,12 +508,15 @@ template <typename T, typename KV, int V> __device__ void append_large(const Rop
     __syncthreads();
     if (tid < nc && (val[find(cand_block[tid])] & 255) != tid) cand_dead[tid] = 1;
     __syncthreads();
-    for (int base = tid; base < n_tok; base += 4 * kLargeThreads) {       // four slots in flight
-        int64_t slot[4];
+    // Every CTA looks at every slot, so a slot that is nobody's must cost little: bit (block & 31) of `seen` turns most of them away.
+    const uint32_t seen = filter;
+    for (int base = tid; base < n_tok; base += 8 * kLargeThreads) {       // eight slots in flight
+        int64_t slot[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) slot[k] = base + k * kLargeThreads < n_tok ? p.slots[base + k * kLargeThreads] : -1;
+        for (int k = 0; k < 8; ++k) slot[k] = base + k * kLargeThreads < n_tok ? p.slots[base + k * kLargeThreads] : -1;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 8; ++k) {
+            if (!((seen >> ((uint32_t)(slot[k] >> p.block_shift) & 31u)) & 1u)) continue;
             const int t = base + k * kLargeThreads, b = block_of(p, slot[k]);
             const int at = b < 0 ? -1 : find(b);
             if (at < 0) continue;
@@ -536,7 +549,7 @@ __device__ __forceinline__ int64_t pool_row(const RopeAppendParams& p, int64_t s
 // Half layout, whole head: a thread takes 8 dims of the low half and their partners for several heads, so each row is read once
 // and the angles once per group of heads; all of its loads are in flight before the first is used.
 template <typename T, bool kv8> __device__ __forceinline__ void rotate_pairs(const RopeAppendParams& p, int cta, int ctas) {
-    constexpr int H = sizeof(T) == 2 ? 4 : 2, W = 8 / Vec16<T>::N;        // heads per item; 16-byte words per 8 dims
+    constexpr int H = 2, W = 8 / Vec16<T>::N;        // heads per item; 16-byte words per 8 dims
     const int hd = p.head_dim, half = hd / 2, NH = p.n_heads, NKV = p.n_kv_heads;
     const bool pool16 = !kv8 && p.k_pool != nullptr;
     const uint32_t cpr = p.by_cpr.div, total = (uint32_t)p.n_tokens * p.by_groups.div * cpr;
@@ -644,7 +657,7 @@ template <typename T, bool kv8, int V> __device__ __forceinline__ void rotate_ro
 }
 
 // 16/32-bit pools, and the queries of a large step over an 8-bit pool.
-template <typename T, bool kv8, int V> __global__ void __launch_bounds__(kAppendWarps * 32, 3) rope_rows_kernel(const RopeAppendParams p) {
+template <typename T, bool kv8, int V> __global__ void __launch_bounds__(kAppendWarps * 32, 4) rope_rows_kernel(const RopeAppendParams p) {
     if (!p.overlap) pdl_launch_dependents();
     pdl_wait();
     if (p.overlap) pdl_launch_dependents();       // the append kernel of the same call may start: it reads the same inputs
@@ -659,7 +672,7 @@ template <typename T, typename KV, int V> __global__ void __launch_bounds__(kApp
 }
 // The append of a large step. It runs beside rope_rows_kernel, which was launched just before it and lets it start once the
 // call's inputs exist; it completes after that kernel, so that the next one waits for both.
-template <typename T, typename KV, int V> __global__ void __launch_bounds__(kLargeThreads, 2) append_large_kernel(const RopeAppendParams p) {
+template <typename T, typename KV, int V> __global__ void __launch_bounds__(kLargeThreads, 3) append_large_kernel(const RopeAppendParams p) {
     if (!p.overlap) {
         pdl_launch_dependents();
         pdl_wait();
@@ -677,7 +690,7 @@ template <typename T, typename KV, int V> static int launch_rope_append(RopeAppe
     p.h0 = p.q_out != nullptr ? 0 : p.n_heads;
     p.h1 = (p.v_out || (!kv8 && p.k_pool)) ? p.n_heads + 2 * p.n_kv_heads : p.k_out ? p.n_heads + p.n_kv_heads : p.n_heads;
     p.pairs = V == 8 && !p.interleaved && p.rot == p.head_dim;
-    p.heads_per_item = p.pairs && sizeof(T) == 4 ? 2 : 4;
+    p.heads_per_item = p.pairs ? 2 : 4;
     const int64_t groups = p.h1 > p.h0 ? (p.h1 - p.h0 + p.heads_per_item - 1) / p.heads_per_item : 0, cpr = p.head_dim / (p.pairs ? 2 * V : V);
     const int64_t items = p.n_tokens * groups * cpr;
     NS_REQUIRE(items < ((int64_t)1 << 31), NS_ERR_UNSUPPORTED, "rope_append: %lld tokens", (long long)p.n_tokens);
