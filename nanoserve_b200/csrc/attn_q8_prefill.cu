@@ -32,7 +32,7 @@ constexpr int kConvWarps = kConv / 32;
 constexpr int kRegsSoftmax = 176, kRegsOther = 80;
 constexpr int kScaleRing = 8;       // a converter is at most five tiles ahead of the slowest softmax thread
 template <int HD> struct Depth {
-    static constexpr int K = 3, V = HD == 64 ? 4 : 2, P = 2;
+    static constexpr int K = 4, V = 4;
     // mbarriers: S0 S1, PV0 PV1, P0 P1 ready of each Q tile | K full | V full | K free | V free | scales of a key tile
     static constexpr int BarS = 0, BarPV = 4, BarPReady = 8, BarKFull = 12, BarVFull = BarKFull + K, BarKFree = BarVFull + V,
                          BarVFree = BarKFree + K, BarScale = BarVFree + V, Bars = BarScale + kScaleRing;
@@ -74,9 +74,9 @@ template <int HD, typename KV>
 __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Params p) {
     using namespace q8p;
     using D = Depth<HD>;
-    constexpr int kStagesK = D::K, kStagesV = D::V, kBufsP = D::P;
+    constexpr int kStagesK = D::K, kStagesV = D::V;
     constexpr int ATOMS = HD / 64;
-    constexpr int Q_BYTES = kRows * 128 * ATOMS, KV_BYTES = kKeys * 128 * ATOMS, P_BYTES = kRows * 128;
+    constexpr int Q_BYTES = kRows * 128 * ATOMS, KV_BYTES = kKeys * 128 * ATOMS;
     constexpr uint32_t COL_TILE = 2 * kKeys + HD, COL_O = 2 * kKeys, TMEM_COLS = 512;      // per Q tile: S0, S1, O
     static_assert(D::Bars * 8 + 16 + kScaleRing * (48 + 8 * kConvWarps) <= kTailBytes, "the tail holds the barriers, two words and the rings");
     // V codes that are NaN (e4m3 only): 0 x NaN would reach rows that must not see the key, so the operand gets 0 there and the
@@ -117,8 +117,8 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
 
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
-    const uint32_t sQ0 = base, sK = sQ0 + 2 * Q_BYTES, sV = sK + kStagesK * KV_BYTES, sP0 = sV + kStagesV * KV_BYTES;
-    const uint32_t bar0 = sP0 + 2 * kBufsP * P_BYTES;
+    const uint32_t sQ0 = base, sK = sQ0 + 2 * Q_BYTES, sV = sK + kStagesK * KV_BYTES;
+    const uint32_t bar0 = sV + kStagesV * KV_BYTES;
     auto bar = [&](int i) -> uint32_t { return bar0 + 8u * (uint32_t)i; };
     volatile uint32_t* tail_words = reinterpret_cast<volatile uint32_t*>(smem_raw + (bar0 - raw) + D::Bars * 8);
     volatile uint32_t& tmem_slot = tail_words[0];
@@ -159,9 +159,9 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
             const int w = warp - 8;
             q_ready_barrier(w);
             if (lane == 0 && w < n_q) {
-                const uint32_t sQ = sQ0 + w * Q_BYTES, sP = sP0 + w * (kBufsP * P_BYTES), t_tile = tmem + w * COL_TILE;
+                const uint32_t sQ = sQ0 + w * Q_BYTES, t_tile = tmem + w * COL_TILE;
                 constexpr uint32_t idesc_s = instr_desc(false, kKeys), idesc_pv = instr_desc(true, HD);
-                const uint64_t dQ = smem_desc(sQ, 16, 1024), dK = smem_desc(sK, 16, 1024), dP = smem_desc(sP, 16, 1024);
+                const uint64_t dQ = smem_desc(sQ, 16, 1024), dK = smem_desc(sK, 16, 1024);
                 const uint64_t dV = smem_desc(sV, kKeys * 128, 1024);
                 auto issue_s = [&](int kt) {
                     const int sk = kt % kStagesK;
@@ -182,11 +182,11 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
                     const int sv = kt % kStagesV;
                     if (!mbar_wait_or_abort(bar(D::BarVFull + sv), (uint32_t)((kt / kStagesV) & 1), tail_words + 1)) { ok = false; return; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint64_t p0 = dP + (uint64_t)(((kt % kBufsP) * P_BYTES) >> 4);
+                    const uint32_t t_p = t_tile + (uint32_t)((kt & 1) * kKeys);      // P(kt) lies where S(kt) was
                     const uint64_t v0 = dV + (uint64_t)((sv * KV_BYTES) >> 4);
 #pragma unroll
                     for (int kk = 0; kk < kKeys / 16; ++kk)
-                        tc::mma_f16(t_tile + COL_O, p0 + (uint32_t)((kk * 32) >> 4), v0 + (uint32_t)((kk * 2048) >> 4), idesc_pv,
+                        tc::mma_f16_ts(t_tile + COL_O, t_p + (uint32_t)(kk * 8), v0 + (uint32_t)((kk * 2048) >> 4), idesc_pv,
                                     (kt > 0 || kk > 0) ? 1u : 0u);
                     mma_commit(bar(D::BarPV + 2 * w + (kt & 1)));
                     mma_commit(bar(D::BarVFree + sv));
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         const int w = warp >> 2, row = tid & (kRows - 1);                  // Q tile, its row
-        const uint32_t sQ = sQ0 + w * Q_BYTES, sP = sP0 + w * (kBufsP * P_BYTES);
+        const uint32_t sQ = sQ0 + w * Q_BYTES;
         const uint32_t t_lane = tmem + w * COL_TILE + ((uint32_t)(32 * (warp & 3)) << 16);     // this warp's 32 lanes; lane = row
         const int tok = q_start + w * kPrefillTileTokens + (row >> 3), hh = row & 7;
         const bool row_ok = tok < T && hh < heads && q0 + tok >= 0 && q0 + tok < p.n_tokens;
@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
             }
             const float m_ref = m_run == -INFINITY ? 0.f : m_run;
             const uint64_t neg_m2 = pack_f32x2(-m_ref, -m_ref);
-            const uint32_t p_dst = sP + (kt % kBufsP) * P_BYTES + row * 128;
+            uint32_t pp[32];                                               // the row's P, two f16 each
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
                 float v[32];
@@ -494,13 +494,14 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
                     l_run = sum == 0.f ? l_run : fmaf(sum, isv[2 * hf + q], l_run);      // (a block the row does not see may have any scale)
                 }
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    st_shared16(p_dst + (((4 * hf + c) ^ (row & 7)) << 4), pack_f16x2(v[8 * c + 0], v[8 * c + 1]), pack_f16x2(v[8 * c + 2], v[8 * c + 3]),
-                                pack_f16x2(v[8 * c + 4], v[8 * c + 5]), pack_f16x2(v[8 * c + 6], v[8 * c + 7]));
+                for (int i = 0; i < 16; ++i) pp[16 * hf + i] = pack_f16x2(v[2 * i], v[2 * i + 1]);
             }
+            tmem_st32(s_src, pp);                                          // over S(kt), which this warp has read
+            tmem_st_wait();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             if (!ok) break;
-            warp_arrive(bar(D::BarPReady + 2 * w + (kt & 1)));
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(D::BarPReady + 2 * w + (kt & 1)));
         }
         if (!ok) abort_flag = 1;
         // ---- the row's output: after the last PV, 32 columns at a time
@@ -557,7 +558,7 @@ template <int HD, typename KV> static int launch_prefill_q8_hd(const Q8Params& p
     constexpr int atoms = HD / 64;
     using D = q8p::Depth<HD>;
     // tiles + tail; 1 KB of slack for the 1024-byte alignment
-    constexpr int smem = 2 * q8p::kRows * 128 * atoms + (D::K + D::V) * q8p::kKeys * 128 * atoms + 2 * D::P * q8p::kRows * 128 + q8p::kTailBytes + 1024;
+    constexpr int smem = 2 * q8p::kRows * 128 * atoms + (D::K + D::V) * q8p::kKeys * 128 * atoms + q8p::kTailBytes + 1024;
     static_assert(smem <= 227 * 1024, "one CTA's shared memory");
     static SmemOptIn optin;
     if (optin.needs((size_t)smem)) {
