@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
 #pragma unroll
         for (int i = 0; i < D::Bars; ++i) {
             // K and V free: one commit per Q tile that read them
-            const uint32_t count = i >= D::BarScale ? (kNanCodes ? kConvWarps : 4) : i >= D::BarKFree ? n_q : i >= D::BarVFull ? kConvWarps : i >= D::BarKFull ? 4
+            const uint32_t count = i >= D::BarScale ? (kNanCodes ? kConvWarps : 2) : i >= D::BarKFree ? n_q : i >= D::BarVFull ? kConvWarps : i >= D::BarKFull ? 4
                                    : i >= D::BarPReady ? kRows / 32 : 1;
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar(i)), "r"(count) : "memory");
         }
@@ -163,9 +163,9 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
                 constexpr uint32_t idesc_s = instr_desc(false, kKeys), idesc_pv = instr_desc(true, HD);
                 const uint64_t dQ = smem_desc(sQ, 16, 1024), dK = smem_desc(sK, 16, 1024);
                 const uint64_t dV = smem_desc(sV, kKeys * 128, 1024);
-                auto issue_s = [&](int kt) {
+                auto issue_s = [&](int kt, bool there) {
                     const int sk = kt % kStagesK;
-                    if (!mbar_wait_or_abort(bar(D::BarKFull + sk), (uint32_t)((kt / kStagesK) & 1), tail_words + 1)) { ok = false; return; }
+                    if (!there && !mbar_wait_or_abort(bar(D::BarKFull + sk), (uint32_t)((kt / kStagesK) & 1), tail_words + 1)) { ok = false; return; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint64_t k0 = dK + (uint64_t)((sk * KV_BYTES) >> 4);
                     const uint32_t d = t_tile + (uint32_t)((kt & 1) * kKeys);
@@ -178,9 +178,9 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
                     mma_commit(bar(D::BarS + 2 * w + (kt & 1)));
                     mma_commit(bar(D::BarKFree + sk));
                 };
-                auto issue_pv = [&](int kt) {
+                auto issue_pv = [&](int kt, bool there) {
                     const int sv = kt % kStagesV;
-                    if (!mbar_wait_or_abort(bar(D::BarVFull + sv), (uint32_t)((kt / kStagesV) & 1), tail_words + 1)) { ok = false; return; }
+                    if (!there && !mbar_wait_or_abort(bar(D::BarVFull + sv), (uint32_t)((kt / kStagesV) & 1), tail_words + 1)) { ok = false; return; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t t_p = t_tile + (uint32_t)((kt & 1) * kKeys);      // P(kt) lies where S(kt) was
                     const uint64_t v0 = dV + (uint64_t)((sv * KV_BYTES) >> 4);
@@ -191,13 +191,16 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
                     mma_commit(bar(D::BarPV + 2 * w + (kt & 1)));
                     mma_commit(bar(D::BarVFree + sv));
                 };
-                if (n_tiles > 0) issue_s(0);
-                if (n_tiles > 1) issue_s(1);
+                if (n_tiles > 0) issue_s(0, false);
+                if (n_tiles > 1) issue_s(1, false);
                 for (int kt = 0; kt < n_tiles && ok; ++kt) {
+                    // V and K are usually there long before P: one wait in turn instead of three
+                    const bool v_there = mbar_test(bar(D::BarVFull + kt % kStagesV), (uint32_t)((kt / kStagesV) & 1));
+                    const bool k_there = mbar_test(bar(D::BarKFull + (kt + 2) % kStagesK), (uint32_t)(((kt + 2) / kStagesK) & 1));
                     if (!mbar_wait_or_abort(bar(D::BarPReady + 2 * w + (kt & 1)), (uint32_t)((kt >> 1) & 1), tail_words + 1)) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    issue_pv(kt);
-                    if (kt + 2 < n_tiles) issue_s(kt + 2);
+                    issue_pv(kt, v_there);
+                    if (kt + 2 < n_tiles) issue_s(kt + 2, k_there);
                 }
                 if (!ok) abort_flag = 1;
             }
@@ -207,10 +210,16 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
             // items of two blocks each. A warp's addresses are then a base per block and constant steps: what bounds these warps is
             // the number of their instructions (they share the issue slots with the softmax).
             constexpr int CPR = HD / 16, ROWS = 32 / CPR, PER = 16 / ROWS;       // pieces per row, rows per item, items per block
-            const int cw = warp - 10, row_in = lane / CPR, piece = lane % CPR;
+            const int cw = warp - 10;
+            // Eight lanes of a store (one pass over the 32 banks) hold four pieces of two neighbouring rows: their even 16-byte chunks
+            // are swizzled to all eight places. (Eight pieces of one row would meet in four: 16 codes make two chunks, and the two
+            // halves of a 128-dim head lie at the same banks.)
+            const int row_in = CPR == 4 ? lane >> 2 : ((lane >> 2) & 1) | ((lane >> 4) << 1);
+            const int piece = CPR == 4 ? lane & 3 : (lane & 3) | ((lane >> 1) & 4);
+            auto row_lanes = [](int r) -> uint32_t { return CPR == 4 ? 0xfu << (4 * r) : 0xf0fu << (4 * (r & 1) + 16 * (r >> 1)); };
             const bool k_warp = cw < 4;
             const int b0 = k_warp ? cw : 2 * (cw - 4);                           // this warp's (first) block
-            constexpr int NV = 2 * (PER - 1);                                    // V items of a warp, at most
+            constexpr int VK = HD == 64 ? 1 : 2, VV = PER - VK, NV = 2 * VV;      // V items of a K warp; of a block left to a V warp; of a V warp
             const uint8_t* kb = p.k_pool + g * p.head_stride + piece * 16 + row_in * p.pos_stride;
             const uint8_t* vb = p.v_pool + g * p.head_stride + piece * 16 + row_in * p.pos_stride;
             const int64_t step = ROWS * p.pos_stride;
@@ -252,9 +261,9 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
                 st_shared16(dst + (((chunk0 + 1) ^ r7) << 4), x, y, z, u);
             };
             // V item m of this warp: block and item inside it
-            auto v_block = [&](int m) -> int { return k_warp ? b0 : b0 + m / (PER - 1); };
-            auto v_item = [&](int m) -> int { return k_warp ? PER - 1 : m % (PER - 1); };
-            const int n_v = k_warp ? 1 : NV;
+            auto v_block = [&](int m) -> int { return k_warp ? b0 : b0 + m / VV; };
+            auto v_item = [&](int m) -> int { return k_warp ? VV + m : m % VV; };
+            const int n_v = k_warp ? VK : NV;
             int id0 = fetch_raw(0, b0), id1 = k_warp ? -1 : fetch_raw(0, b0 + 1);
             int raw0 = fetch_raw(1, b0), raw1 = k_warp ? -1 : fetch_raw(1, b0 + 1);
             float sk = 0.f, sv = 1.f;
@@ -262,15 +271,19 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
             auto load_tile_k = [&](int kt, int64_t off0) { load_items(kb, off0, id0, kt, b0, 0, integral_constant<int, PER>(), kr); };
             auto load_tile_v = [&](int kt, int64_t off0, int64_t off1) {
                 if (k_warp) {
-                    load_items(vb, off0, id0, kt, b0, PER - 1, integral_constant<int, 1>(), vr);
+                    load_items(vb, off0, id0, kt, b0, VV, integral_constant<int, VK>(), vr);
                 } else {
-                    load_items(vb, off0, id0, kt, b0, 0, integral_constant<int, PER - 1>(), vr);
-                    load_items(vb, off1, id1, kt, b0 + 1, 0, integral_constant<int, PER - 1>(), vr + PER - 1);
+                    load_items(vb, off0, id0, kt, b0, 0, integral_constant<int, VV>(), vr);
+                    load_items(vb, off1, id1, kt, b0 + 1, 0, integral_constant<int, VV>(), vr + VV);
                 }
             };
+            // scales: lanes 0 and 1 of the two V warps, a block each (the K warps are the slower ones)
+            const bool scale_lane = !k_warp && lane < 2;
+            int its_id = -1;
             auto load_scales = [&]() {
-                if (k_warp && id0 >= 0) {
-                    const int64_t o = (int64_t)id0 * p.sc_blk_stride + (int64_t)g * p.sc_head_stride;
+                its_id = lane == 0 ? id0 : id1;
+                if (scale_lane && its_id >= 0) {
+                    const int64_t o = (int64_t)its_id * p.sc_blk_stride + (int64_t)g * p.sc_head_stride;
                     sk = p.k_scale[o];
                     sv = p.v_scale[o];
                 }
@@ -283,25 +296,18 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
                     load_scales();
                 }
             }
+            bool k_free = true;                                                  // asked for a tile ahead
             for (int kt = 0; kt < n_tiles; ++kt) {
                 const int st_k = kt % kStagesK, st_v = kt % kStagesV;
-                const int here = id0;                                            // this tile's block (scales)
+                const bool v_free = kt < kStagesV || mbar_test(bar(D::BarVFree + st_v), (uint32_t)((kt / kStagesV - 1) & 1));
                 int64_t off0 = 0, off1 = 0;
                 if (k_warp) {
-                    if (kt >= kStagesK)
+                    if (!k_free)
                         ok = mbar_wait_or_abort(bar(D::BarKFree + st_k), (uint32_t)((kt / kStagesK - 1) & 1), tail_words + 1);
                     if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
 #pragma unroll
                     for (int n = 0; n < PER; ++n) store_item(sK + st_k * KV_BYTES, b0, n, kr[n]);
                     warp_arrive(bar(D::BarKFull + st_k));
-                    // scales of the block: log2 and reciprocal by the approximate instructions (2^-22, far below P's 11 bits)
-                    const float svf = sv < kMinScale ? kMinScale : sv;
-                    if (lane == 0) {
-                        float* e = scale_ring + (kt % kScaleRing) * 12 + b0;
-                        e[0] = here >= 0 ? sk : 0.f;
-                        e[4] = here >= 0 ? __log2f(svf) : -INFINITY;
-                        e[8] = here >= 0 ? __fdividef(1.f, svf) : 0.f;
-                    }
                 }
                 id0 = raw0;
                 id1 = raw1;
@@ -309,21 +315,19 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
                 off1 = locate(kt + 1, b0 + 1, id1);
                 raw0 = fetch_raw(kt + 2, b0);
                 raw1 = k_warp ? -1 : fetch_raw(kt + 2, b0 + 1);
-                if (k_warp) {
-                    load_tile_k(kt + 1, off0);
-                    load_scales();
-                }
-                if (kt >= kStagesV)
+                if (k_warp) load_tile_k(kt + 1, off0);
+                if (!v_free)
                     ok = mbar_wait_or_abort(bar(D::BarVFree + st_v), (uint32_t)((kt / kStagesV - 1) & 1), tail_words + 1);
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 if (kNanCodes) {
-                    auto nan_of = [](uint32_t w) -> uint32_t { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; };   // bit 7 of a NaN byte
+                    auto carry = [](uint32_t w) -> uint32_t { return (w & 0x7f7f7f7fu) + 0x01010101u; };     // bit 7 of a NaN byte is set
+                    auto nan_of = [&](uint32_t w) -> uint32_t { return carry(w) & 0x80808080u; };
                     uint32_t any = 0;
 #pragma unroll
                     for (int m = 0; m < NV; ++m)
-                        if (m < n_v) any |= nan_of(vr[m].x) | nan_of(vr[m].y) | nan_of(vr[m].z) | nan_of(vr[m].w);
+                        if (m < n_v) any |= (carry(vr[m].x) | carry(vr[m].y)) | (carry(vr[m].z) | carry(vr[m].w));
                     uint64_t keys = 0;
-                    if (__any_sync(0xffffffffu, any != 0)) {
+                    if (__any_sync(0xffffffffu, (any & 0x80808080u) != 0)) {
 #pragma unroll
                         for (int m = 0; m < NV; ++m) {
                             if (m >= n_v) continue;
@@ -334,16 +338,29 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
                             vr[m].z &= ~((fz >> 7) * 0xffu);
                             vr[m].w &= ~((fw >> 7) * 0xffu);
                             for (int r = 0; r < ROWS; ++r)
-                                if ((lanes >> (r * CPR)) & ((1u << CPR) - 1u)) keys |= 1ull << (16 * v_block(m) + v_item(m) * ROWS + r);
+                                if (lanes & row_lanes(r)) keys |= 1ull << (16 * v_block(m) + v_item(m) * ROWS + r);
                         }
                     }
                     if (lane == 0) nan_ring[(kt % kScaleRing) * kConvWarps + cw] = keys;
                 }
-                if (lane == 0 && (k_warp || kNanCodes)) mbar_arrive(bar(D::BarScale + kt % kScaleRing));
+                if (!k_warp) {
+                    // log2 and reciprocal by the approximate instructions (2^-22, far below P's 11 bits)
+                    const float svf = sv < kMinScale ? kMinScale : sv;
+                    if (scale_lane) {
+                        float* e = scale_ring + (kt % kScaleRing) * 12 + b0 + lane;
+                        e[0] = its_id >= 0 ? sk : 0.f;
+                        e[4] = its_id >= 0 ? __log2f(svf) : -INFINITY;
+                        e[8] = its_id >= 0 ? __fdividef(1.f, svf) : 0.f;
+                    }
+                    load_scales();
+                    __syncwarp();
+                }
+                if (lane == 0 && (!k_warp || kNanCodes)) mbar_arrive(bar(D::BarScale + kt % kScaleRing));
 #pragma unroll
                 for (int m = 0; m < NV; ++m)
                     if (m < n_v) store_item(sV + st_v * KV_BYTES, v_block(m), v_item(m), vr[m]);
                 warp_arrive(bar(D::BarVFull + st_v));
+                if (k_warp) k_free = kt + 1 < kStagesK || mbar_test(bar(D::BarKFree + (kt + 1) % kStagesK), (uint32_t)(((kt + 1) / kStagesK - 1) & 1));
                 load_tile_v(kt + 1, off0, off1);
             }
             if (!ok) abort_flag = 1;
@@ -388,13 +405,16 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
         const volatile uint32_t* abort_now = tail_words + 1;
         float m_run = -INFINITY, l_run = 0.f;
         const int my_tiles = w < n_q ? n_tiles : 0;
+        bool ready = false;                // S and the scales of the next tile: asked for while this tile's exponentials are computed
         for (int kt = 0; kt < my_tiles; ++kt) {
             // The scales of tile kt were written before its S was issued: their barrier is only looked at. (A warp gives up as a whole:
             // its tensor-memory accesses and votes are warp-wide.)
-            ok = mbar_wait_or_abort(bar(D::BarS + 2 * w + (kt & 1)), (uint32_t)((kt >> 1) & 1), abort_now) &&
-                 mbar_wait_or_abort(bar(D::BarScale + kt % kScaleRing), (uint32_t)((kt / kScaleRing) & 1), abort_now);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
+            if (!__all_sync(0xffffffffu, ready)) {
+                ok = mbar_wait_or_abort(bar(D::BarS + 2 * w + (kt & 1)), (uint32_t)((kt >> 1) & 1), abort_now) &&
+                     mbar_wait_or_abort(bar(D::BarScale + kt % kScaleRing), (uint32_t)((kt / kScaleRing) & 1), abort_now);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+            }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t s_src = t_lane + (uint32_t)((kt & 1) * kKeys);
             const int key_base = kt * kKeys;
@@ -405,6 +425,12 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
             const float* ring = scale_ring + (kt % kScaleRing) * 12;
             const float4 sk4 = *reinterpret_cast<const float4*>(ring), lv4 = *reinterpret_cast<const float4*>(ring + 4),
                          iv4 = *reinterpret_cast<const float4*>(ring + 8);
+            uint64_t keys = 0;                                             // NaN keys of the tile
+            if (kNanCodes) {
+                const ulonglong2* nr = reinterpret_cast<const ulonglong2*>(nan_ring + (kt % kScaleRing) * kConvWarps);
+                const ulonglong2 n0 = nr[0], n1 = nr[1], n2 = nr[2];
+                keys = n0.x | n0.y | n1.x | n1.y | n2.x | n2.y;
+            }
             const float fac[4] = {f_row * sk4.x, f_row * sk4.y, f_row * sk4.z, f_row * sk4.w};
             const float lv[4] = {lv4.x, lv4.y, lv4.z, lv4.w}, isv[4] = {iv4.x, iv4.y, iv4.z, iv4.w};
             tmem_ld_wait();
@@ -421,10 +447,6 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
                     sr[hf][i + 1] = __float_as_uint(x1);
                 }
             if (kNanCodes) {
-                const uint64_t* nr = nan_ring + (kt % kScaleRing) * kConvWarps;
-                uint64_t keys = 0;
-#pragma unroll
-                for (int i = 0; i < kConvWarps; ++i) keys |= nr[i];
                 if (keys != 0) {
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf)
@@ -496,6 +518,8 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
 #pragma unroll
                 for (int i = 0; i < 16; ++i) pp[16 * hf + i] = pack_f16x2(v[2 * i], v[2 * i + 1]);
             }
+            ready = mbar_test(bar(D::BarS + 2 * w + ((kt + 1) & 1)), (uint32_t)(((kt + 1) >> 1) & 1)) &
+                    mbar_test(bar(D::BarScale + (kt + 1) % kScaleRing), (uint32_t)(((kt + 1) / kScaleRing) & 1));
             tmem_st32(s_src, pp);                                          // over S(kt), which this warp has read
             tmem_st_wait();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

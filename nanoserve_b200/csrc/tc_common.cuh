@@ -87,6 +87,21 @@ __device__ __forceinline__ bool mbar_wait(uint32_t mbar_saddr, uint32_t parity) 
     return false;
 }
 
+// Has this phase completed? Asked ahead of time, so that the answer is there when it is needed.
+__device__ __forceinline__ bool mbar_test(uint32_t mbar_saddr, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "}\n"
+        : "=r"(done)
+        : "r"(mbar_saddr), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
 // The copying thread's wait: also gives up when the softmax threads raised the CTA's abort flag.
 __device__ __forceinline__ bool mbar_wait_or_abort(uint32_t mbar_saddr, uint32_t parity, const volatile uint32_t* abort_flag) {
     for (uint32_t i = 0; i < kWaitLimit; ++i) {
