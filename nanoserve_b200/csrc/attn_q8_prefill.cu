@@ -59,6 +59,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+// One lane of a converged warp, the same one at every call.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
 // Every lane's generic-proxy stores become visible to the tensor cores, then one arrival for the warp.
 __device__ __forceinline__ void warp_arrive(uint32_t mbar_saddr) {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -156,51 +162,64 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
         if (warp < 10) {
-            const int w = warp - 8;
+            // The whole warp runs the loop with warp-uniform values and one elected lane issues: descriptors and addresses then stay
+            // in uniform registers, where the instruction wants them.
+            const int w = __shfl_sync(0xffffffffu, warp, 0) - 8;
             q_ready_barrier(w);
-            if (lane == 0 && w < n_q) {
-                const uint32_t sQ = sQ0 + w * Q_BYTES, t_tile = tmem + w * COL_TILE;
+            if (w < n_q) {
+                const uint32_t sQ = sQ0 + w * Q_BYTES, t_tile = __shfl_sync(0xffffffffu, tmem, 0) + w * COL_TILE;
+                const int tiles = __shfl_sync(0xffffffffu, n_tiles, 0);
+                const bool leader = elect_one();
                 constexpr uint32_t idesc_s = instr_desc(false, kKeys), idesc_pv = instr_desc(true, HD);
                 const uint64_t dQ = smem_desc(sQ, 16, 1024), dK = smem_desc(sK, 16, 1024);
                 const uint64_t dV = smem_desc(sV, kKeys * 128, 1024);
+                auto wait = [&](int i, uint32_t parity) -> bool {
+                    return __all_sync(0xffffffffu, mbar_wait_or_abort(bar(i), parity, tail_words + 1));
+                };
                 auto issue_s = [&](int kt, bool there) {
                     const int sk = kt % kStagesK;
-                    if (!there && !mbar_wait_or_abort(bar(D::BarKFull + sk), (uint32_t)((kt / kStagesK) & 1), tail_words + 1)) { ok = false; return; }
+                    if (!there && !wait(D::BarKFull + sk, (uint32_t)((kt / kStagesK) & 1))) { ok = false; return; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint64_t k0 = dK + (uint64_t)((sk * KV_BYTES) >> 4);
                     const uint32_t d = t_tile + (uint32_t)((kt & 1) * kKeys);
+                    if (leader) {
 #pragma unroll
-                    for (int kk = 0; kk < HD / 16; ++kk) {
-                        const uint32_t a_off = (uint32_t)(((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4);
-                        const uint32_t b_off = (uint32_t)(((kk >> 2) * (kKeys * 128) + (kk & 3) * 32) >> 4);
-                        tc::mma_f16(d, dQ + a_off, k0 + b_off, idesc_s, kk > 0);
+                        for (int kk = 0; kk < HD / 16; ++kk) {
+                            const uint32_t a_off = (uint32_t)(((kk >> 2) * (kRows * 128) + (kk & 3) * 32) >> 4);
+                            const uint32_t b_off = (uint32_t)(((kk >> 2) * (kKeys * 128) + (kk & 3) * 32) >> 4);
+                            tc::mma_f16(d, dQ + a_off, k0 + b_off, idesc_s, kk > 0);
+                        }
+                        mma_commit(bar(D::BarS + 2 * w + (kt & 1)));
+                        mma_commit(bar(D::BarKFree + sk));
                     }
-                    mma_commit(bar(D::BarS + 2 * w + (kt & 1)));
-                    mma_commit(bar(D::BarKFree + sk));
+                    __syncwarp();
                 };
                 auto issue_pv = [&](int kt, bool there) {
                     const int sv = kt % kStagesV;
-                    if (!there && !mbar_wait_or_abort(bar(D::BarVFull + sv), (uint32_t)((kt / kStagesV) & 1), tail_words + 1)) { ok = false; return; }
+                    if (!there && !wait(D::BarVFull + sv, (uint32_t)((kt / kStagesV) & 1))) { ok = false; return; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     const uint32_t t_p = t_tile + (uint32_t)((kt & 1) * kKeys);      // P(kt) lies where S(kt) was
                     const uint64_t v0 = dV + (uint64_t)((sv * KV_BYTES) >> 4);
+                    if (leader) {
 #pragma unroll
-                    for (int kk = 0; kk < kKeys / 16; ++kk)
-                        tc::mma_f16_ts(t_tile + COL_O, t_p + (uint32_t)(kk * 8), v0 + (uint32_t)((kk * 2048) >> 4), idesc_pv,
-                                    (kt > 0 || kk > 0) ? 1u : 0u);
-                    mma_commit(bar(D::BarPV + 2 * w + (kt & 1)));
-                    mma_commit(bar(D::BarVFree + sv));
+                        for (int kk = 0; kk < kKeys / 16; ++kk)
+                            tc::mma_f16_ts(t_tile + COL_O, t_p + (uint32_t)(kk * 8), v0 + (uint32_t)((kk * 2048) >> 4), idesc_pv,
+                                           (kt > 0 || kk > 0) ? 1u : 0u);
+                        mma_commit(bar(D::BarPV + 2 * w + (kt & 1)));
+                        mma_commit(bar(D::BarVFree + sv));
+                    }
+                    __syncwarp();
                 };
-                if (n_tiles > 0) issue_s(0, false);
-                if (n_tiles > 1) issue_s(1, false);
-                for (int kt = 0; kt < n_tiles && ok; ++kt) {
+                if (tiles > 0) issue_s(0, false);
+                if (tiles > 1) issue_s(1, false);
+                for (int kt = 0; kt < tiles && ok; ++kt) {
                     // V and K are usually there long before P: one wait in turn instead of three
-                    const bool v_there = mbar_test(bar(D::BarVFull + kt % kStagesV), (uint32_t)((kt / kStagesV) & 1));
-                    const bool k_there = mbar_test(bar(D::BarKFull + (kt + 2) % kStagesK), (uint32_t)(((kt + 2) / kStagesK) & 1));
-                    if (!mbar_wait_or_abort(bar(D::BarPReady + 2 * w + (kt & 1)), (uint32_t)((kt >> 1) & 1), tail_words + 1)) { ok = false; break; }
+                    const bool v_there = __all_sync(0xffffffffu, mbar_test(bar(D::BarVFull + kt % kStagesV), (uint32_t)((kt / kStagesV) & 1)));
+                    const bool k_there = __all_sync(0xffffffffu, mbar_test(bar(D::BarKFull + (kt + 2) % kStagesK), (uint32_t)(((kt + 2) / kStagesK) & 1)));
+                    if (!wait(D::BarPReady + 2 * w + (kt & 1), (uint32_t)((kt >> 1) & 1))) { ok = false; break; }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     issue_pv(kt, v_there);
-                    if (kt + 2 < n_tiles) issue_s(kt + 2, k_there);
+                    if (kt + 2 < tiles) issue_s(kt + 2, k_there);
                 }
                 if (!ok) abort_flag = 1;
             }
