@@ -11,12 +11,22 @@
 //   x = s * (scale log2 e * 2^e_q * sk) + log2 sv,   P = 2^(x - m),   l += sum(P) / sv   per block of 16 keys
 // (Q is scaled by a power of two per row, P is relative to the row's largest contribution; see attn_q8_decode.cu.)
 // Four warpgroups, 512 threads, one CTA per SM (all 512 columns of its tensor memory):
-//   warps 0-3, 4-7   one softmax thread per row of tile A, of tile B. 176 registers a thread
-//   warps 8, 9       lane 0 issues the tcgen05.mma of tile A, of tile B
+//   warps 0-3, 4-7   softmax and output of tiles A and B, one thread per row; 176 registers
+//   warps 8, 9       issue the tcgen05.mma of tile A, of tile B: the warp runs converged on uniform values, one elected lane issues
+//                    (a lone lane, with its operands moved to uniform registers one by one: 310 us against 307, mixed 68 against 64)
 //   warps 10-15      convert K and V tiles. 80 registers a thread: 2 (176 + 80) 128 = 128 * 512, what the block was launched with
-// Pipeline per tile as in the 16-bit kernel: S runs two key tiles ahead, P double buffered, O stays in tensor memory and is
-// rescaled only when a row's reference has to move; A and B fill each other's gaps. Every mbarrier wait is bounded: on expiry the
-// CTA counts an error in the plan header (ns_collect_status), skips its stores, frees its tensor memory and returns.
+// Pipeline per tile: S runs two key tiles ahead in two buffers; P(kt) goes back into the columns that S(kt) was read from and is the
+// A operand from there, so it never passes through shared memory (in shared memory, double buffered: 356 us against 322). S(kt + 2)
+// overwrites it after PV(kt): one warp issues both, and the tensor cores keep its order. O stays in tensor memory and is rescaled only
+// when a row's reference has to move; A and B fill each other's gaps. Barriers are asked for ahead of the wait. Every mbarrier wait is
+// bounded: on expiry the CTA counts an error in the plan header (ns_collect_status), skips its stores, frees its tensor memory and
+// returns.
+// What bounds it (2,048 tokens on 6,001 keys, 28 / 4 heads of 128: 306 us, 674 TFLOP/s of the rows that exist; 256 items on 148 SMs
+// are two rounds, the second three quarters full, and seven of eight head slots are used: 890 TFLOP/s inside a full round): with
+// the softmax and the conversion cut out the same chain of waits and products takes 208 us, with the softmax alone cut out 239, with
+// the conversion alone cut out 298. Reading Q once per 64 keys costs the products 48 of every 32 cycles of arithmetic (S of 128 keys
+// would need 384 of a tile's 256 columns). Two softmax warpgroups per tile taking turns, with the scores read twice so that 768
+// threads fit the registers: 372 us.
 #include "attn_q8.cuh"
 #include "tc_common.cuh"
 
@@ -30,6 +40,7 @@ constexpr int kRows = 128, kKeys = 64, kThreads = 512, kConv = 192;    // rows o
 constexpr int kTokens = 2 * kPrefillTileTokens;                        // query tokens per item
 constexpr int kConvWarps = kConv / 32;
 constexpr int kRegsSoftmax = 176, kRegsOther = 80;
+constexpr int kSplitTiles = 8;      // key tiles from which an item is split
 constexpr int kScaleRing = 8;       // a converter is at most five tiles ahead of the slowest softmax thread
 template <int HD> struct Depth {
     static constexpr int K = 4, V = 4;
@@ -59,6 +70,29 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
 }
+__device__ __forceinline__ uint32_t cluster_ctas() {
+    uint32_t n;
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+    return n;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctaid.x;" : "=r"(r));
+    return r;
+}
+// All threads of the cluster's CTAs that have not exited (no role waits here for another without a limit of its own before).
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_address(uint32_t saddr, int rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(saddr), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void st_cluster16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 // One lane of a converged warp, the same one at every call.
 __device__ __forceinline__ bool elect_one() {
     uint32_t one;
@@ -76,7 +110,8 @@ __device__ __forceinline__ void q_ready_barrier(int tile) { asm volatile("bar.sy
 
 }  // namespace q8p
 
-template <int HD, typename KV>
+// SPLIT: the CTAs of a cluster share an item, each with its part of the keys.
+template <int HD, typename KV, bool SPLIT>
 __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Params p) {
     using namespace q8p;
     using D = Depth<HD>;
@@ -95,10 +130,10 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
     int item_idx, vh;
     {
         // the plan lists tiles of 16 tokens, heaviest first: the even ones of a sequence stand for a pair, the odd ones for nothing
-        const int n_items = hdr->n_prefill_items, n_kv = (int)gridDim.y;
-        const int lin = (int)(blockIdx.x + gridDim.x * blockIdx.y);
-        item_idx = lin < n_items * n_kv ? lin / n_kv : n_items;
-        vh = lin % n_kv;
+        const int n_items = hdr->n_prefill_items, n_vh = p.n_kv_heads * sub;
+        const int lin = SPLIT ? (int)(blockIdx.x / cluster_ctas()) : (int)blockIdx.x;
+        item_idx = lin / n_vh;
+        vh = lin - item_idx * n_vh;
         if (item_idx >= n_items) {
             pdl_wait();                           // the grid must not complete before the decode kernel it overlaps
             return;
@@ -119,7 +154,19 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
     const int32_t* table = p.block_tables + (int64_t)(p.table_rows ? p.table_rows[s] : s) * p.table_stride;
     const int kv_end = min(len, ctx + min(q_start + kTokens, T));
     const int n_q = T - q_start > kPrefillTileTokens ? 2 : 1;                // Q tiles
-    const int n_tiles = kv_end > 0 ? (kv_end + kKeys - 1) / kKeys : 0;
+    int n_tiles = kv_end > 0 ? (kv_end + kKeys - 1) / kKeys : 0, tile0 = 0;   // this CTA's key tiles: tile0 .. tile0 + n_tiles - 1
+    int parts = 1, part = 0;
+    if (SPLIT) {
+        part = (int)cluster_rank();
+        if (n_tiles >= kSplitTiles) {
+            parts = (int)cluster_ctas();
+            tile0 = (int)((unsigned)(n_tiles * part) / (unsigned)parts);
+            n_tiles = (int)((unsigned)(n_tiles * (part + 1)) / (unsigned)parts) - tile0;
+        } else if (part > 0) {                    // a short item is the first CTA's alone
+            pdl_wait();
+            return;
+        }
+    }
 
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
@@ -246,19 +293,19 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
             uint4 kr[PER], vr[NV];
             // the table entry of keys 16 b .. of a tile, -1 past the last visible key; it is requested a whole tile before it is looked at
             auto fetch_raw = [&](int kt, int b) -> int {
-                const int key = kt * kKeys + 16 * b;
+                const int key = (tile0 + kt) * kKeys + 16 * b;
                 return kt < n_tiles && key < kv_end ? table[key >> p.block_shift] : -1;
             };
             auto locate = [&](int kt, int b, int& raw) -> int64_t {              // offset of the block's first key in a pool; raw -1: absent
                 int64_t off = (int64_t)raw * p.blk_stride;
-                if (p.block_size != 16) off += (int64_t)((kt * kKeys + 16 * b) & (p.block_size - 1)) * p.pos_stride;
+                if (p.block_size != 16) off += (int64_t)(((tile0 + kt) * kKeys + 16 * b) & (p.block_size - 1)) * p.pos_stride;
                 if ((unsigned)raw >= (unsigned)p.num_blocks) raw = -1;
                 return off;
             };
             // items n0 .. of a block into r: a block that is there and full takes plain loads (the usual case, and warp-uniform)
             auto load_items = [&](const uint8_t* pool, int64_t off, int id, int kt, int b, int n0, auto count, uint4* r) {
                 const uint8_t* src = pool + off;
-                const int left = len - (kt * kKeys + 16 * b);                    // keys of the block
+                const int left = len - ((tile0 + kt) * kKeys + 16 * b);                    // keys of the block
                 if (id >= 0 && left >= 16) {
 #pragma unroll
                     for (int n = 0; n < decltype(count)::value; ++n) r[n] = __ldcg(reinterpret_cast<const uint4*>(src + (n0 + n) * step));
@@ -384,6 +431,10 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
             }
             if (!ok) abort_flag = 1;
         }
+        if (SPLIT && parts > 1) {                  // the two meetings of the softmax threads below
+            cluster_sync();
+            cluster_sync();
+        }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
         const int w = warp >> 2, row = tid & (kRows - 1);                  // Q tile, its row
@@ -436,7 +487,7 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t s_src = t_lane + (uint32_t)((kt & 1) * kKeys);
-            const int key_base = kt * kKeys;
+            const int key_base = (tile0 + kt) * kKeys;
             const bool masked = key_base + kKeys - 1 > ctx + q_start + w * kPrefillTileTokens;      // else every row sees every key of the tile
             uint32_t sr[2][32];
             tmem_ld32_issue(s_src, sr[0]);
@@ -553,9 +604,55 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
             ok = __all_sync(0xffffffffu, mbar_wait_or_abort(bar(D::BarPV + 2 * w + ((n_tiles - 1) & 1)), (uint32_t)(((n_tiles - 1) >> 1) & 1), abort_now));
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         }
-        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
         __nv_bfloat16* out_row = reinterpret_cast<__nv_bfloat16*>(p.out) + (int64_t)(row_ok ? q0 + tok : 0) * p.out_stride +
                                  (int64_t)(row_ok ? g * p.group + h0 + hh : 0) * HD;
+        bool store = row_ok;
+        float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+        // A split item: every CTA finishes 256 / parts of the rows. The others send it {O, m, l} of these into its K and V
+        // buffers, which nothing reads any more once both sides' last PV is over; then it joins them, its own first, the others in
+        // the order of their ranks.
+        constexpr int RS = HD + 4;
+        const int rows_of = 2 * kRows / (SPLIT ? parts : 1), R = w * kRows + row, owner = R / rows_of;
+        float own_w = 1.f, w_of[3] = {0.f, 0.f, 0.f};                       // weights of the parts
+        const float* const got = reinterpret_cast<const float*>(smem_raw + (sK - raw)) + (R - owner * rows_of) * RS;   // of source i: + i rows_of RS
+        if (SPLIT && parts > 1) {
+            static_assert(2 * kRows * 3 / 4 * RS * 4 <= (kStagesK + kStagesV) * KV_BYTES, "what the others send fits the K and V buffers");
+            cluster_sync();
+            if (__any_sync(0xffffffffu, owner != part)) {                   // (rows_of is a multiple of 32: the same for a whole warp)
+                const uint32_t dst = cluster_address(sK + (uint32_t)((((part < owner ? part : part - 1) * rows_of + R - owner * rows_of) * RS) * 4), owner);
+#pragma unroll
+                for (int c = 0; c < HD / 32; ++c) {
+                    if (!have_o || !ok) break;
+                    uint32_t r[32];
+                    tmem_ld32_issue(t_o + 32 * c, r);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) st_cluster16(dst + (32 * c + 4 * e) * 4, r[4 * e], r[4 * e + 1], r[4 * e + 2], r[4 * e + 3]);
+                }
+                // (a CTA that gave up makes these rows NaN; a part without a visible key has O = 0 that was perhaps never written: its weight is 0)
+                st_cluster16(dst + HD * 4, __float_as_uint(m_run), ok ? __float_as_uint(l_run) : 0x7fffffffu, 0u, 0u);
+            }
+            cluster_sync();
+            store = row_ok && owner == part;
+            if (store) {
+                float top = m_run;
+                for (int i = 0; i < parts - 1; ++i) top = fmaxf(top, got[i * rows_of * RS + HD]);
+                const float ref = top == -INFINITY ? 0.f : top;
+                // weight of a part; 0 only for one without a visible key, so that NaN comes through
+                auto weight = [&](float m, float l) { return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2(m - ref); };
+                own_w = weight(m_run, l_run);
+                float l = l_run * own_w;
+#pragma unroll
+                for (int i = 0; i < 3; ++i) {
+                    if (i >= parts - 1) continue;
+                    const float m_i = got[i * rows_of * RS + HD], l_i = got[i * rows_of * RS + HD + 1];
+                    w_of[i] = weight(m_i, l_i);
+                    if (m_i == -INFINITY && l_i == 0.f) w_of[i] = -1.f;     // nothing to read
+                    else l = fmaf(l_i, w_of[i], l);
+                }
+                inv = l == 0.f ? 0.f : 1.f / l;
+            }
+        }
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) {
             float v[32];
@@ -564,12 +661,31 @@ __global__ void __launch_bounds__(q8p::kThreads, 1) prefill_q8_kernel(const Q8Pa
                 tmem_ld32_issue(t_o + 32 * c, r);
                 tmem_ld_wait();
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]) * inv;
+                for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
             } else {
 #pragma unroll
                 for (int i = 0; i < 32; ++i) v[i] = 0.f;
             }
-            if (ok && row_ok) {
+            if (SPLIT && parts > 1 && store) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] *= own_w;
+#pragma unroll
+                for (int j = 0; j < 3; ++j) {
+                    if (j >= parts - 1 || w_of[j] < 0.f) continue;
+                    const float4* o = reinterpret_cast<const float4*>(got + j * rows_of * RS + 32 * c);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float4 x = o[e];
+                        v[4 * e] = fmaf(x.x, w_of[j], v[4 * e]);
+                        v[4 * e + 1] = fmaf(x.y, w_of[j], v[4 * e + 1]);
+                        v[4 * e + 2] = fmaf(x.z, w_of[j], v[4 * e + 2]);
+                        v[4 * e + 3] = fmaf(x.w, w_of[j], v[4 * e + 3]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= inv;
+            if (ok && store) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     uint4 o;
@@ -597,27 +713,49 @@ bool q8_prefill_supported(const Q8Params& p, int dtype) {
 }
 
 // NS_ERR_UNSUPPORTED: the kernel was not built with the register count its split needs; the scalar kernel serves then.
-template <int HD, typename KV> static int launch_prefill_q8_hd(const Q8Params& p, int max_items, cudaStream_t st) {
+template <int HD, typename KV, bool SPLIT> static int launch_prefill_q8_as(const Q8Params& p, int max_items, int parts, cudaStream_t st) {
     constexpr int atoms = HD / 64;
     using D = q8p::Depth<HD>;
     // tiles + tail; 1 KB of slack for the 1024-byte alignment
     constexpr int smem = 2 * q8p::kRows * 128 * atoms + (D::K + D::V) * q8p::kKeys * 128 * atoms + q8p::kTailBytes + 1024;
     static_assert(smem <= 227 * 1024, "one CTA's shared memory");
+    const auto kernel = prefill_q8_kernel<HD, KV, SPLIT>;
     static SmemOptIn optin;
     if (optin.needs((size_t)smem)) {
         // setmaxnreg moves registers between the warpgroups within what the block was launched with: it must be all of 128 a thread
         cudaFuncAttributes attr;
-        cudaError_t e = cudaFuncGetAttributes(&attr, prefill_q8_kernel<HD, KV>);
+        cudaError_t e = cudaFuncGetAttributes(&attr, kernel);
         if (e != cudaSuccess) return fail(NS_ERR_CUDA, "prefill_q8: cannot query the kernel: %s", cudaGetErrorString(e));
         if (attr.numRegs * q8p::kThreads < 2 * (q8p::kRegsSoftmax + q8p::kRegsOther) * 128) return NS_ERR_UNSUPPORTED;
-        e = cudaFuncSetAttribute(prefill_q8_kernel<HD, KV>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
         if (e != cudaSuccess) return fail(NS_ERR_CUDA, "prefill_q8: cannot reserve %d bytes of shared memory: %s", smem, cudaGetErrorString(e));
         optin.done((size_t)smem);
     }
-    cudaError_t e = launch_pdl(prefill_q8_kernel<HD, KV>, dim3((unsigned)max_items, (unsigned)(p.n_kv_heads * ((p.group + 7) / 8))),
-                               dim3(q8p::kThreads), (size_t)smem, st, p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(max_items * p.n_kv_heads * ((p.group + 7) / 8) * parts));
+    cfg.blockDim = dim3(q8p::kThreads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)parts;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = SPLIT ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
     if (e != cudaSuccess) return fail(NS_ERR_CUDA, "prefill_q8: launch failed: %s", cudaGetErrorString(e));
     return NS_OK;
+}
+// An item is split over its keys where the items leave most SMs without one: by four while four parts of each fit one wave, else by
+// two. (512 tokens on 4,096 keys, 14 heads of 64, 32 items: 83 us whole, 50 in two parts, 33 in four; 28 heads of 128, 64
+// items: 105 / 64 / 86. 1,024 tokens on 1,024 keys, 128 items of the latter: 55 / 66 / 111 - a second wave costs more than it
+// saves, a CTA takes 6 us to start and to finish. Items below kSplitTiles stay whole; the clusters cost those 0.8 us.)
+template <int HD, typename KV> static int launch_prefill_q8_hd(const Q8Params& p, int max_items, cudaStream_t st) {
+    const int64_t items = p.n_tokens / q8p::kTokens * p.n_kv_heads * ((p.group + 7) / 8);
+    const int parts = 4 * items <= p.sm_count ? 4 : 2 * items <= p.sm_count ? 2 : 1;
+    return parts > 1 ? launch_prefill_q8_as<HD, KV, true>(p, max_items, parts, st) : launch_prefill_q8_as<HD, KV, false>(p, max_items, 1, st);
 }
 
 int launch_q8_prefill(const Q8Params& p, int pool_dtype, int max_items, cudaStream_t st) {
