@@ -332,6 +332,7 @@ int ns_rope_tables(const int64_t* positions, const float* inv_freq, double facto
  *   Otherwise scale' = max(scale, S), and if it grew the other rows are re-coded round(code * scale / scale').
  *   code = x / scale' to the nearest code, ties to even. Tokens may come in any order; of two that name one slot the later
  *   stays. block_size: a power of two up to 64.
+ * Outputs and pools must not overlap the inputs or each other.
  * Replaces, widened: nanoserve/kernels/fused.py:156 rope_qkv and nanoserve/kv_cache.py:274-279 PagedKVCache.write. */
 int ns_rope_append(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride,
                    const float* cos, const float* sin, int32_t rot_dim, int32_t interleaved, void* q_out, void* k_out,

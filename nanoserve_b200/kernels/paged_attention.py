@@ -97,7 +97,9 @@ def _attend_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, se
     assert q2 == 1 and (q1 == head_dim or n_heads == 1), "query heads must be adjacent (head stride == head_dim)"
     assert block_tables.dtype is i32 and (t1 == 1 or width <= 1)
     assert seq_lens.dtype is i32 and seq_lens.is_contiguous() and seq_lens.shape[0] >= n_seqs
-    dev = _lib.same_device(q, k_pool, v_pool, k_scale, v_scale, block_tables, seq_lens)
+    if ws is not None and (ws.n_heads != n_heads or ws.head_dim != head_dim):
+        raise ValueError(f"a workspace for {ws.n_heads} heads of {ws.head_dim} does not serve {n_heads} heads of {head_dim}")
+    dev = _lib.same_device(q, k_pool, v_pool, k_scale, v_scale, block_tables, seq_lens, None if ws is None else ws.buf)
     cu = rows_ptr = None
     if cu_seqlens is None:
         assert N == n_seqs, "without cu_seqlens every sequence has one token"

@@ -68,6 +68,28 @@ def test_attention_refusals():
     assert simple(hd=300) == UNSUPPORTED and "head_dim" in msg()
 
 
+def test_attention_workspace_refusals():
+    lib = _lib.load()
+    f = lambda **kw: lib.ns_ragged_paged_attn_q8(*attn_args(**kw))
+    need = lib.ns_attn_workspace_bytes(2, 2, 14, 64)
+    assert f(ws=NUL) == INVALID and "null" in msg()
+    assert f(ws=P(4096 + 16), wsb=need, wss=2, wst=2) == INVALID and "aligned" in msg()
+    assert f(ws=P(4096), wsb=need, wss=1, wst=2) == WORKSPACE and "exceeds" in msg()
+    assert f(ws=P(4096), wsb=need, wss=2, wst=1) == WORKSPACE
+    assert f(ws=P(4096), wsb=need - 1, wss=2, wst=2) == WORKSPACE and "needed" in msg()
+
+
+def test_a_workspace_of_another_shape_is_refused():
+    """Its counters lie elsewhere: they would be found non-zero."""
+    from nanoserve_b200.kernels.paged_attention import AttnWorkspace, paged_attention_decode
+    q, t, L = torch.zeros(2, 14, 64, dtype=torch.bfloat16), torch.zeros(2, 1, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    i8, s = torch.zeros(2, 16, 2, 64, dtype=torch.int8), torch.zeros(2, 2)
+    for heads, hd in ((12, 64), (14, 128)):
+        ws = AttnWorkspace(4, 4, heads, hd, device="cpu")
+        with pytest.raises(ValueError, match="workspace"):
+            paged_attention_decode(q, i8, i8, t, L, 0.125, workspace=ws, k_scale=s, v_scale=s)
+
+
 def test_values_and_tables_refusals():
     lib = _lib.load()
     v = lambda dt, pdt, **kw: lib.ns_kv_values(P(256), kw.get("scale", P(512)), P(1024), kw.get("nb", 2), 16, 2, 64, 2048, 128, 64, 2, 1, dt, pdt, NUL)
