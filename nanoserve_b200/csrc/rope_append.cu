@@ -145,13 +145,18 @@ __device__ __forceinline__ void rotate_vec(const T* head, int rot, int interleav
 // slot is named. The owner needs the block's members: for each row, the last token of the call that names it.
 //   steps of up to kSmallStep tokens: a warp per (token, plane) looks through all slots itself; nothing is shared, no barrier.
 //   larger steps: a CTA takes kAppendChunk tokens of a KV head, finds the leaders among them, and its threads look through all
-//     slots once for all of its leaders' blocks. (256 tokens / one layer of the 14-head shape: 3.4 us against 5.4 for the CTA form;
-//     4096 tokens: a scan per leader and plane would read every slot 2,000 times.)
+//     slots once for all of its leaders' blocks.
+// (A layer of 14 / 2 heads of 64, 256 tokens: 3.3 us in blocks of their own and 3.6 as one chunk, against 11 and 5.6 for the CTA form.
+// The first form at 512 tokens: 4.4 and 4.6 against 11 and 5.8, but 9.0 and 8.0 against 12.0 and 7.4 for 28 / 4 heads of 128, and the
+// registers that twice as many slots take cost every decode step 0.5 us.) What bounds the large form is latency: a CTA's chain of slot,
+// row and code loads, in some rounds of six CTAs per SM; DRAM is 4 % busy. With 28 / 4 heads of 128, 2,048 tokens of one prompt take
+// 12.6 us, 37 decode rows and four chunks of 1,021 24.8. Chunks of 16 tokens and 256 threads: 13.8 and 25.8; one CTA for four heads of
+// a chunk, which looks through the slots once: 20.1 and 33.8.
 constexpr int kSmallStep = 256;
-constexpr int kAppendChunk = 16;              // tokens per CTA of a large step
+constexpr int kAppendChunk = 8;               // tokens per CTA of a large step
 constexpr int kAppendMaxBlock = 64;           // largest block size
 constexpr int kMembers = kAppendChunk * kAppendMaxBlock;
-constexpr int kAppendWarps = 8, kLargeThreads = 256;
+constexpr int kAppendWarps = 8, kLargeThreads = 128;
 
 // What the owner of a block does with its scale: the magnitude of the written rows, the old scale and whether the call writes the
 // block's first row give the new one.
@@ -527,6 +532,14 @@ template <typename T, typename KV, int V> __device__ void append_large(const Rop
     }
     __syncthreads();
     if constexpr (V == 8) {
+        // Many candidates are blocks with a row or two each (decode rows): a warp takes a block's K or V as a whole, its loads all in
+        // flight at once. (512 tokens in blocks of their own, 28 / 4 heads of 128: 12.4 us against 24.8 by all warps; 37 of those
+        // before a 2,048-token chunk: 14.9 against 26.6.)
+        if (p.pairs && bs == 16 && nc > 2 && (p.head_dim == 64 || p.head_dim == 128)) {
+            for (int i = warp; i < 2 * nc; i += kLargeThreads / 32)
+                if (!cand_dead[i >> 1]) append_any<T, KV, V>(p, 2 * head + (i & 1), cand_block[i >> 1], member + (i >> 1) * bs);
+            return;
+        }
         if (p.pairs && bs == 16 && p.head_dim == 64) return append_units<T, KV, 64>(p, head, nc, cand_block, cand_dead, member, unit_max, unit_scale);
         if (p.pairs && bs == 16 && p.head_dim == 128) return append_units<T, KV, 128>(p, head, nc, cand_block, cand_dead, member, unit_max, unit_scale);
     }
@@ -672,7 +685,7 @@ template <typename T, typename KV, int V> __global__ void __launch_bounds__(kApp
 }
 // The append of a large step. It runs beside rope_rows_kernel, which was launched just before it and lets it start once the
 // call's inputs exist; it completes after that kernel, so that the next one waits for both.
-template <typename T, typename KV, int V> __global__ void __launch_bounds__(kLargeThreads, 3) append_large_kernel(const RopeAppendParams p) {
+template <typename T, typename KV, int V> __global__ void __launch_bounds__(kLargeThreads, 6) append_large_kernel(const RopeAppendParams p) {
     if (!p.overlap) {
         pdl_launch_dependents();
         pdl_wait();
