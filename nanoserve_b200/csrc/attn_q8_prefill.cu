@@ -22,10 +22,10 @@
 // bounded: on expiry the CTA counts an error in the plan header (ns_collect_status), skips its stores, frees its tensor memory and
 // returns.
 // What bounds it (2,048 tokens on 6,001 keys, 28 / 4 heads of 128: 306 us, 674 TFLOP/s of the rows that exist; 256 items on 148 SMs
-// are two rounds, the second three quarters full, and seven of eight head slots are used: 890 TFLOP/s inside a full round): with
+// are two rounds, the second three quarters full, and seven of eight head slots are used): with
 // the softmax and the conversion cut out the same chain of waits and products takes 208 us, with the softmax alone cut out 239, with
-// the conversion alone cut out 298. Reading Q once per 64 keys costs the products 48 of every 32 cycles of arithmetic (S of 128 keys
-// would need 384 of a tile's 256 columns). Two softmax warpgroups per tile taking turns, with the scores read twice so that 768
+// the conversion alone cut out 298. Q is read again for every 64 keys, which makes 48 cycles of shared memory for 32 of arithmetic in Q.K
+// (scores of 128 keys, double buffered, and O would need 384 of the 256 columns a tile has). Two softmax warpgroups per tile taking turns, with the scores read twice so that 768
 // threads fit the registers: 372 us.
 #include "attn_q8.cuh"
 #include "tc_common.cuh"

@@ -1,5 +1,6 @@
 // Scalar ragged paged attention over 8-bit pools: one warp per (query token, query head), fp32 everywhere. Serves the head
-// layouts and block sizes the tensor-core kernels do not cover, fp32 prefill chunks, and on-device cross-checks.
+// layouts and block sizes the tensor-core kernels do not cover, fp32 prefill chunks, and on-device cross-checks. A lane scores a key, the
+// warp then adds up the values a dim per lane; bound by its scalar loads and multiply-adds.
 #include "attn_q8.cuh"
 
 namespace ns {
