@@ -18,7 +18,7 @@ There is no CPU path: weights must be CUDA tensors.
 from __future__ import annotations
 
 import copy
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 import torch.nn.functional as F
@@ -37,7 +37,7 @@ class ModelConfig:
     rms_norm_eps: float
     tie_word_embeddings: bool
     # rotary positions beyond the reference's (half layout, whole head, unscaled): see kernels.rotary
-    rope_scaling: dict | None = None         # a checkpoint's rope_scaling entry (linear, ntk, yarn)
+    rope_scaling: dict | None = field(default=None, hash=False)      # a checkpoint's rope_scaling entry (linear, ntk, yarn)
     partial_rotary_factor: float = 1.0       # share of each head that is rotated
     rope_interleaved: bool = False           # pairs (2i, 2i + 1) instead of (i, i + r/2)
 
@@ -51,16 +51,20 @@ class ModelConfig:
         return not scaled and self.rotary_dim == self.head_dim and not self.rope_interleaved
 
     @classmethod
-    def from_hf_config(cls, d: dict) -> "ModelConfig":
+    def from_hf_config(cls, d: dict, rope_extensions: bool = False) -> "ModelConfig":
+        """rope_extensions: also take the checkpoint's rope scaling and partial_rotary_factor, which the reference (and the default)
+        passes over."""
         params = d.get("rope_parameters") or {}
         theta = d.get("rope_theta") or params.get("rope_theta")
-        scaling = d.get("rope_scaling") or (params if params.get("rope_type", "default") != "default" else None)
+        extra = {}
+        if rope_extensions:
+            extra = dict(rope_scaling=d.get("rope_scaling") or (params if params.get("rope_type", "default") != "default" else None),
+                         partial_rotary_factor=float(d.get("partial_rotary_factor") or params.get("partial_rotary_factor") or 1.0))
         return cls(vocab_size=d["vocab_size"], hidden_size=d["hidden_size"], n_layers=d["num_hidden_layers"],
                    n_heads=d["num_attention_heads"], n_kv_heads=d["num_key_value_heads"],
                    head_dim=d.get("head_dim") or d["hidden_size"] // d["num_attention_heads"],
                    intermediate_size=d["intermediate_size"], rope_theta=float(theta),
-                   rms_norm_eps=d["rms_norm_eps"], tie_word_embeddings=d.get("tie_word_embeddings", False),
-                   rope_scaling=scaling, partial_rotary_factor=float(d.get("partial_rotary_factor") or params.get("partial_rotary_factor") or 1.0))
+                   rms_norm_eps=d["rms_norm_eps"], tie_word_embeddings=d.get("tie_word_embeddings", False), **extra)
 
     def kv_bytes_per_token(self, dtype: torch.dtype) -> int:
         return self.n_layers * 2 * self.n_kv_heads * self.head_dim * torch.finfo(dtype).bits // 8

@@ -205,8 +205,11 @@ def test_configuration_of_rotary_positions():
               rms_norm_eps=1e-6, rope_theta=1e6)
     yarn = {"type": "yarn", "factor": 4.0, "original_max_position_embeddings": 32768}
     assert ModelConfig.from_hf_config(hf).plain_rope
-    assert ModelConfig.from_hf_config(dict(hf, rope_scaling=yarn)).rope_scaling == yarn
+    scaled = dict(hf, rope_scaling=yarn, partial_rotary_factor=0.5)
+    assert ModelConfig.from_hf_config(scaled) == ModelConfig.from_hf_config(hf)          # as before there were such positions
+    cfg = ModelConfig.from_hf_config(scaled, rope_extensions=True)
+    assert cfg.rope_scaling == yarn and cfg.rotary_dim == 32 and hash(cfg) == hash(cfg)
     new = ModelConfig.from_hf_config(dict({k: v for k, v in hf.items() if k != "rope_theta"},
-                                          rope_parameters=dict(rope_type="linear", factor=2.0, rope_theta=5e5, partial_rotary_factor=0.5)))
+                                          rope_parameters=dict(rope_type="linear", factor=2.0, rope_theta=5e5, partial_rotary_factor=0.5)), True)
     assert new.rope_theta == 5e5 and new.rotary_dim == 32 and new.rope_scaling["factor"] == 2.0
-    assert ModelConfig.from_hf_config(dict(hf, rope_parameters=dict(rope_type="default", rope_theta=1e6))).plain_rope
+    assert ModelConfig.from_hf_config(dict(hf, rope_parameters=dict(rope_type="default", rope_theta=1e6)), True).plain_rope
