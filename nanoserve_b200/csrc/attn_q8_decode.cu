@@ -22,12 +22,14 @@
 //          where the last CTA to arrive (one counter, nobody waits) joins them in CTA order: the result does not depend on
 //          the order of arrival.
 // Bound  : the stream itself runs at the copy rate (12 K cycles for 304 KB per SM); 8 K cycles before the first key is multiplied and
-//          10 K of joins after the last are cold instructions and dependent loads. 48 rows U[128, 8192] of 14 / 2 heads of 64: 22.9 us,
-//          45 MB (6.9 us at the copy rate); 64 rows U[256, 4608] of 28 / 4 heads of 128: 40.2 us, 144 MB (22.0); 2 rows of 131 K keys
-//          of 12 / 2 heads of 128: 40.6 us, 134 MB (20.5).
+//          10 K of joins after the last are dependent loads. 48 rows U[128, 8192] of 14 / 2 heads of 64: 22.4 us, 45 MB (6.9 us at
+//          the copy rate); 64 rows U[256, 4608] of 28 / 4 heads of 128: 38.2 us, 144 MB (22.0); 2 rows of 131 K keys of 12 / 2 heads
+//          of 128: 41.3 us, 134 MB (20.5).
 // Cuts   : a CTA takes at least two tiles per warp (one row of 300 keys: 7.3 us; at least one: 8.3; at least four: 7.1, and no
-//          difference elsewhere); a cut moves by at most a quarter of a CTA's share (not at all: 10.4 us for that row, 23.9 against
-//          22.9, 40.9 against 40.2, 41.7 against 40.6; by half: 7.3, 23.0, 43.4, 44.7).
+//          difference elsewhere). A cut moves onto a unit's end that is nearer than a join costs, or than half a share: 64 rows of
+//          28 heads 38.0 us, 128 rows U[512, 4096] of 14 heads 27.8, 32 rows of 1,000 keys 10.9. By up to a quarter of a share: 39.8, 28.7,
+//          12.4 (2 rows of 131 K: 40.5 against 41.5); by up to half: 43.4 for the first; not at all: 40.9, and 10.4 against 7.3 for
+//          the row of 300 keys.
 #include "attn_q8.cuh"
 
 namespace ns {
@@ -37,6 +39,9 @@ namespace q8 {
 constexpr float kLazy = 8.f;               // the exponent's reference may lag the maximum by this many powers of two
 constexpr float kMinScale = 7.8886090522101181e-31f;    // 2^-100: a smaller V scale (zero included) counts as this
 constexpr int kMaxSeqs = 8192;             // sequences per launch (prefix, length and table row of each in shared memory)
+
+// Tiles a CTA streams in the time that a join across CTAs costs it (about 4 K cycles at 25 bytes per cycle and SM).
+template <int HD> constexpr int kJoinTiles = HD == 64 ? 48 : 24;
 
 template <int HD> struct Cfg;
 template <> struct Cfg<64> { static constexpr int kWarps = 16, kDepth = 3; };
@@ -156,7 +161,8 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
                 }
             }
     if (W == 0) return;
-    // row that holds tile x of the list: the last r with prefix[r] * VH <= x (empty rows share their successor's prefix)
+    // row that holds tile x of the list: the last r with prefix[r] * VH <= x (empty rows share their successor's prefix). By one lane
+    // for itself, or by a warp for one x: 32 rows are compared at once.
     auto row_of = [&](int x) -> int {
         int lo = 0, hi = n_rows;
         while (hi - lo > 1) {
@@ -165,13 +171,24 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
         }
         return lo;
     };
+    auto warp_row_of = [&](int x) -> int {
+        int lo = 0, hi = n_rows, step = 1;                // prefix[lo] VH <= x; rows lo + step, lo + 2 step ... below hi are compared
+        while (step * 32 < n_rows) step *= 32;
+        for (;; step >>= 5) {
+            const int r = lo + (lane + 1) * step;
+            lo += step * __popc(__ballot_sync(0xffffffffu, r < hi && prefix[r] * VH <= x));
+            if (step == 1) return lo;
+        }
+    };
     // First tile of CTA c: an even cut, moved onto the end or the start of a unit that is near (no cross-CTA join then).
-    const int per = max((W + G - 1) / G, min_tiles), slack = per >> 2;
-    auto cta_cut = [&](int c) -> int {
+    const int per = max((W + G - 1) / G, min_tiles), slack = min(per >> 1, kJoinTiles<HD>);
+    auto even_cut = [&](int c) -> int {
         const long long want = (long long)c * per;
-        int x = want >= W ? W : (int)want;
+        return want >= W ? W : (int)want;
+    };
+    auto moved_cut = [&](int x, int r) -> int {           // r: row of x
         if (x > 0 && x < W) {
-            const int r = row_of(x), nt = prefix[r + 1] - prefix[r], start = prefix[r] * VH;
+            const int nt = prefix[r + 1] - prefix[r], start = prefix[r] * VH;
             const int lo = start + (int)((unsigned)(x - start) / (unsigned)nt) * nt, hi = lo + nt;
             if (x - lo <= hi - x) {
                 if (x - lo <= slack) x = lo;
@@ -181,7 +198,13 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
         }
         return x;
     };
-    int c0 = cta_cut(cta + (lane & 1));                   // every warp for itself: lane 0 the CTA's first tile, lane 1 the next CTA's
+    auto cta_cut = [&](int c) -> int {
+        const int x = even_cut(c);
+        return moved_cut(x, row_of(x));
+    };
+    // every warp for itself: lane 0 the CTA's first tile, lane 1 the next CTA's
+    const int e0 = even_cut(cta), e1 = even_cut(cta + 1), r0 = warp_row_of(e0), r1 = warp_row_of(e1);
+    int c0 = moved_cut(lane & 1 ? e1 : e0, lane & 1 ? r1 : r0);
     const int c1 = __shfl_sync(0xffffffffu, c0, 1);
     c0 = __shfl_sync(0xffffffffu, c0, 0);
     const int n_mine = c1 - c0;
@@ -191,7 +214,7 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
 
     // ---- this warp's tiles
     if (a < b) {
-        int r = row_of(a), nt = prefix[r + 1] - prefix[r], us = prefix[r] * VH;
+        int r = warp_row_of(a), nt = prefix[r + 1] - prefix[r], us = prefix[r] * VH;
         int vh = (int)((unsigned)(a - us) / (unsigned)nt);
         us += vh * nt;
         int x = a;
@@ -483,25 +506,26 @@ __global__ void __launch_bounds__(q8::Cfg<HD>::kWarps * 32, 1) decode_q8_kernel(
         float acc[C];
 #pragma unroll
         for (int i = 0; i < C; ++i) acc[i] = 0.f;
-        // all pieces' columns are requested before the first is used (a piece without tiles, or one that weighs nothing, is skipped:
+        // four pieces' columns are requested before the first is used (a piece without tiles, or one that weighs nothing, is skipped:
         // its slot may hold anything)
-        float v[NW][C];
+#pragma unroll 1
+        for (int k0 = 0; k0 <= w1 - w0; k0 += 4) {
+            float v[4][C], f[4];
 #pragma unroll
-        for (int k = 0; k < NW; ++k) {
-            const bool on = w0 + k <= w1 && __shfl_sync(0xffffffffu, wt, k) != 0.f;
-            const float* src = (k == 0 ? piece0 : slots + ((w0 + k) * 16 + h) * RS) + C * lane;
+            for (int k = 0; k < 4; ++k) {
+                f[k] = __shfl_sync(0xffffffffu, wt, k0 + k);              // (lanes past the last piece: 0)
+                const float* src = (k0 + k == 0 ? piece0 : slots + ((w0 + k0 + k) * 16 + h) * RS) + C * lane;
 #pragma unroll
-            for (int i = 0; i < C; i += 2) {
-                const float2 u = on ? *reinterpret_cast<const float2*>(src + i) : make_float2(0.f, 0.f);
-                v[k][i] = u.x;
-                v[k][i + 1] = u.y;
+                for (int i = 0; i < C; i += 2) {
+                    const float2 u = f[k] != 0.f ? *reinterpret_cast<const float2*>(src + i) : make_float2(0.f, 0.f);
+                    v[k][i] = u.x;
+                    v[k][i + 1] = u.y;
+                }
             }
-        }
 #pragma unroll
-        for (int k = 0; k < NW; ++k) {
-            const float f = __shfl_sync(0xffffffffu, wt, k);
+            for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int i = 0; i < C; ++i) acc[i] = fmaf(f, v[k][i], acc[i]);
+                for (int i = 0; i < C; ++i) acc[i] = fmaf(f[k], v[k][i], acc[i]);
         }
         if (ch.w == 1) {
             const float inv = l == 0.f ? 0.f : 1.f / l;
