@@ -25,7 +25,7 @@
 // are two rounds, the second three quarters full, and seven of eight head slots are used): with
 // the softmax and the conversion cut out the same chain of waits and products takes 208 us, with the softmax alone cut out 239, with
 // the conversion alone cut out 298. Q is read again for every 64 keys, which makes 48 cycles of shared memory for 32 of arithmetic in Q.K
-// (scores of 128 keys, double buffered, and O would need 384 of the 256 columns a tile has). Two softmax warpgroups per tile taking turns, with the scores read twice so that 768
+// (scores of 128 keys, double buffered, and O would need 384 of the 256 columns a tile has; single-buffered: 445 us). Two softmax warpgroups per tile taking turns, with the scores read twice so that 768
 // threads fit the registers: 372 us.
 #include "attn_q8.cuh"
 #include "tc_common.cuh"
