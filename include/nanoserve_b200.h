@@ -371,6 +371,11 @@ int ns_ragged_paged_attn_q8_simple(const void* q, const void* k_pool, const void
                                    int64_t pool_head_stride, int64_t scale_block_stride, int64_t scale_head_stride,
                                    float scale, int dtype, int pool_dtype, void* stream);
 
+/* The entry points above with their arguments, in order, as 64-bit words: pointers and integers as they are, float and double
+ * arguments as the bits of a double. For bindings that pay for every argument. n_words must be the operation's count. */
+enum ns_op { NS_OP_ROPE_TABLES = 0, NS_OP_ROPE_APPEND = 1, NS_OP_KV_VALUES = 2, NS_OP_RAGGED_PAGED_ATTN_Q8 = 3 };
+int ns_call(int32_t op, const int64_t* words, int32_t n_words);
+
 /* ------------------------------------------------------------------------------------------------
  * Step metadata and greedy sampling on the device.
  *

@@ -10,6 +10,7 @@ from ctypes import c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_void_
 from pathlib import Path
 
 import os
+import struct
 
 # NS_DEBUG_LIB=1 loads the -DNS_DEBUG_HOOKS build (python -m nanoserve_b200.build --debug-hooks) instead: the same
 # entry points plus the profiling hooks
@@ -72,6 +73,7 @@ SIGNATURES: dict[str, tuple] = {
                                         _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, c_int, c_int, _P, _I64, _I32, _I32, _P]),
     "ns_ragged_paged_attn_q8_simple": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _I32, _I32, _I32,
                                                _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _F, c_int, c_int, _P]),
+    "ns_call": (c_int, [_I32, c_char_p, _I32]),
     "ns_build_step_metadata": (c_int, [_P, _I32, _P, _P, _I32, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _P]),
     "ns_argmax_rows": (c_int, [_P, _I64, _I32, _I32, _P, _P, _P, c_int, _P]),
     "ns_sample_rows": (c_int, [_P, _I64, _I32, _I32, _P, _P, _P, _P, _P, _P, c_int, _P]),
@@ -185,18 +187,32 @@ def same_device(*tensors) -> int:
     return dev
 
 
-_cuda_state = None
+class PackedOp:
+    """An entry point behind ns_call: its arguments (the stream aside, which is the last) become an array of 64-bit words. `fmt` is
+    struct's format of the words: q an integer or pointer (0, not None, for a null pointer), d a float or double."""
+    __slots__ = ("name", "op", "pack", "words", "_fn", "_current", "_raw_stream", "_guard")
+
+    def __init__(self, name: str, op: int, fmt: str):
+        packer = struct.Struct("=" + fmt)
+        self.name, self.op, self.pack, self.words, self._fn = name, op, packer.pack, packer.size // 8, None
+
+    def __call__(self, device: int, *args) -> None:
+        """Launch with CUDA device `device` current (a launch needs that), on its current stream."""
+        global launch_count
+        if self._fn is None:
+            import torch
+            self._current, self._raw_stream, self._guard = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.cuda.device
+            self._fn = load().ns_call
+        if device != self._current():
+            with self._guard(device):
+                return self(device, *args)
+        status = self._fn(self.op, self.pack(*args, self._raw_stream(device)), self.words)
+        launch_count += 1
+        if status != 0:
+            raise NanoserveB200Error(f"{self.name} failed (status {status}): {load().ns_last_error().decode()}")
 
 
-def call_on(device: int, name: str, *args) -> None:
-    """call() with CUDA device `device` current (a launch needs that) and its current stream as the last argument."""
-    global _cuda_state
-    if _cuda_state is None:
-        import torch
-        _cuda_state = (torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream, torch.cuda.device)
-    current, raw_stream, guard = _cuda_state
-    if device == current():
-        call(name, *args, raw_stream(device))
-        return
-    with guard(device):
-        call(name, *args, raw_stream(device))
+rope_tables = PackedOp("ns_rope_tables", 0, "2qd5q")
+rope_append = PackedOp("ns_rope_append", 1, "32q")
+kv_values = PackedOp("ns_kv_values", 2, "15q")
+ragged_paged_attn_q8 = PackedOp("ns_ragged_paged_attn_q8", 3, "26qd7q")

@@ -20,7 +20,7 @@ LIB_DIR = PKG / "lib"
 LIB_PATH = LIB_DIR / "libnanoserve_b200.so"
 SOURCES = ["c_api.cu", "fused_ops.cu", "attn_plan.cu", "attn_decode.cu", "attn_decode_static.cu", "attn_prefill_mma.cu", "attn_prefill_tc.cu", "attn_simple.cu",
            "metadata.cu", "sampling.cu", "skinny_gemm.cu", "thin_gemm.cu", "stream_gemm.cu", "umma_gemm.cu", "tp_allreduce.cu", "rope_append.cu",
-           "attn_q8.cu", "attn_q8_simple.cu", "attn_q8_decode.cu", "attn_q8_prefill.cu"]
+           "attn_q8.cu", "attn_q8_simple.cu", "attn_q8_decode.cu", "attn_q8_prefill.cu", "packed_call.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--use_fast_math=false"]
 
 

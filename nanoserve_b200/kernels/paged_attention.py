@@ -100,7 +100,7 @@ def _attend_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, se
     if ws is not None and (ws.n_heads != n_heads or ws.head_dim != head_dim):
         raise ValueError(f"a workspace for {ws.n_heads} heads of {ws.head_dim} does not serve {n_heads} heads of {head_dim}")
     dev = _lib.same_device(q, k_pool, v_pool, k_scale, v_scale, block_tables, seq_lens, None if ws is None else ws.buf)
-    cu = rows_ptr = None
+    cu = rows_ptr = 0
     if cu_seqlens is None:
         assert N == n_seqs, "without cu_seqlens every sequence has one token"
     else:
@@ -114,7 +114,7 @@ def _attend_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, se
         rows_ptr = table_rows.data_ptr()
         _lib.same_device(q, table_rows)
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty_like(q, memory_format=torch.contiguous_format)
         o0 = n_heads * head_dim
     else:
         o0, o1, o2 = out.stride()
@@ -124,20 +124,19 @@ def _attend_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, se
         with torch.cuda.device(dev):                       # a launch needs its device current
             return _attend_q8(q, k_pool, v_pool, k_scale, v_scale, block_tables, table_rows, seq_lens, cu_seqlens, scale, n_seqs, ws, planned,
                               out, simple)
-    stream = torch._C._cuda_getCurrentRawStream(dev)
     args = (q.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), block_tables.data_ptr(), rows_ptr,
             seq_lens.data_ptr(), cu, out.data_ptr(), n_seqs, N, n_heads, n_kv_heads, head_dim, block_size, num_blocks, width, t0, q0, o0, p0, p1,
             p2, s0, s1, scale, _lib.dtype_code(q_dtype), _lib.kv8_code(kv_dtype))
     if simple:
-        _lib.call("ns_ragged_paged_attn_q8_simple", *args, stream)
+        _lib.call("ns_ragged_paged_attn_q8_simple", *args, torch._C._cuda_getCurrentRawStream(dev))
         return out
     if ws is None:
         ws = _workspace_q8(q.device, n_seqs, N, n_heads, head_dim)
-    if cu is not None and N > 1:
+    if cu and N > 1:
         if not planned:
             ws.plan(seq_lens, cu_seqlens, n_seqs, block_size, table_rows)
         _lib.note_launches(1)          # the prefill-tile kernel is launched next to the decode kernel
-    _lib.call("ns_ragged_paged_attn_q8", *args, ws.ptr, ws.nbytes, ws.max_seqs, ws.max_tokens, stream)
+    _lib.ragged_paged_attn_q8(dev, *args, ws.ptr, ws.nbytes, ws.max_seqs, ws.max_tokens)
     return out
 
 

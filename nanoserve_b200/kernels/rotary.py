@@ -69,7 +69,7 @@ def rope_tables(positions: torch.Tensor, inv_freq: torch.Tensor, factor: float =
     t, half = positions.shape[0], inv_freq.shape[0]
     cos = inv_freq.new_empty((t, half))
     sin = torch.empty_like(cos)
-    _lib.call_on(dev, "ns_rope_tables", positions.data_ptr(), inv_freq.data_ptr(), float(factor), cos.data_ptr(), sin.data_ptr(), t, half)
+    _lib.rope_tables(dev, positions.data_ptr(), inv_freq.data_ptr(), factor, cos.data_ptr(), sin.data_ptr(), t, half)
     return cos, sin
 
 
@@ -77,7 +77,8 @@ def check_kv8_scales(pool: torch.Tensor, scale: torch.Tensor | None, other: torc
     """An 8-bit pool's scales: fp32 [num_blocks, n_kv_heads], one for K and one for V, of equal strides; returns the strides."""
     if scale is None:
         raise ValueError(f"a {pool.dtype} pool needs k_scale and v_scale (fp32 [num_blocks, n_kv_heads])")
-    shape, strides = (pool.shape[0], pool.shape[2]), scale.stride()
+    (blocks, _, heads, _), strides = pool.shape, scale.stride()
+    shape = (blocks, heads)
     assert scale.dtype is torch.float32 and scale.shape == shape, "scales are fp32 [num_blocks, n_kv_heads]"
     if other is not None:
         assert other.dtype is torch.float32 and other.shape == shape, "scales are fp32 [num_blocks, n_kv_heads]"
@@ -85,7 +86,7 @@ def check_kv8_scales(pool: torch.Tensor, scale: torch.Tensor | None, other: torc
     return strides
 
 
-_NO_POOL = (None, None, None, None, None)
+_NO_POOL = (0, 0, 0, 0, 0)
 
 
 def _pool_args(dtype, n, n_kv_heads, head_dim, k_cache, v_cache, slots, k_scale, v_scale):
@@ -94,22 +95,25 @@ def _pool_args(dtype, n, n_kv_heads, head_dim, k_cache, v_cache, slots, k_scale,
         return _NO_POOL, 0, 1, (0, 0, 0, 0, 0), _lib.dtype_code(dtype)
     if v_cache is None or slots is None:
         raise ValueError("a cache layer needs k_cache, v_cache and slots")
-    shape, strides = k_cache.shape, k_cache.stride()
-    assert len(shape) == 4 and v_cache.shape == shape and shape[2] == n_kv_heads and shape[3] == head_dim, "cache layer shape"
-    assert v_cache.stride() == strides and strides[3] == 1 and v_cache.dtype is k_cache.dtype
+    shape, strides, kv_dtype = k_cache.shape, k_cache.stride(), k_cache.dtype
+    assert len(shape) == 4, "cache layer shape"
+    blocks, block_size, heads, hd = shape
+    assert heads == n_kv_heads and hd == head_dim and v_cache.shape == shape, "cache layer shape"
+    s0, s1, s2, s3 = strides
+    assert v_cache.stride() == strides and s3 == 1 and v_cache.dtype is kv_dtype
     assert slots.dtype is torch.int64 and slots.is_contiguous() and slots.shape[0] >= n
-    code, sc = _lib.kv8_code(k_cache.dtype), (0, 0)
+    code, sc0, sc1 = _lib.kv8_code(kv_dtype), 0, 0
     if code is None:
-        assert k_cache.dtype is dtype, "the pool holds the activations' dtype, int8 or float8_e4m3fn"
+        assert kv_dtype is dtype, "the pool holds the activations' dtype, int8 or float8_e4m3fn"
         assert k_scale is None and v_scale is None, "scales belong to 8-bit pools"
         code = _lib.dtype_code(dtype)
-        scales = (None, None)
+        ks = vs = 0
     else:
         if v_scale is None:
-            raise ValueError(f"a {k_cache.dtype} pool needs k_scale and v_scale (fp32 [num_blocks, n_kv_heads])")
-        sc = check_kv8_scales(k_cache, k_scale, v_scale)
-        scales = (k_scale.data_ptr(), v_scale.data_ptr())
-    return ((k_cache.data_ptr(), v_cache.data_ptr(), *scales, slots.data_ptr()), shape[0] * shape[1], shape[1], strides[:3] + sc, code)
+            raise ValueError(f"a {kv_dtype} pool needs k_scale and v_scale (fp32 [num_blocks, n_kv_heads])")
+        sc0, sc1 = check_kv8_scales(k_cache, k_scale, v_scale)
+        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
+    return (k_cache.data_ptr(), v_cache.data_ptr(), ks, vs, slots.data_ptr()), blocks * block_size, block_size, (s0, s1, s2, sc0, sc1), code
 
 
 def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int,
@@ -138,9 +142,9 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_heads
     v = torch.empty_like(k) if dense_kv else None
     base, size = qkv.data_ptr(), 2 if dtype is torch.bfloat16 else 4
     base_k = base + n_heads * head_dim * size
-    _lib.call_on(dev, "ns_rope_append", base, base_k, base_k + n_kv_heads * head_dim * size, row, row, row, cos.data_ptr(), sin.data_ptr(),
-                 2 * half, 1 if interleaved else 0, q.data_ptr(), None if k is None else k.data_ptr(), None if v is None else v.data_ptr(),
-                 *pool, n, n_slots, n_heads, n_kv_heads, head_dim, block_size, *strides, _lib.dtype_code(dtype), code)
+    _lib.rope_append(dev, base, base_k, base_k + n_kv_heads * head_dim * size, row, row, row, cos.data_ptr(), sin.data_ptr(), 2 * half,
+                     1 if interleaved else 0, q.data_ptr(), 0 if k is None else k.data_ptr(), 0 if v is None else v.data_ptr(), *pool, n, n_slots,
+                     n_heads, n_kv_heads, head_dim, block_size, *strides, _lib.dtype_code(dtype), code)
     return q, k, v
 
 
@@ -154,8 +158,8 @@ def kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v
     dtype = k_new.dtype
     pool, n_slots, block_size, strides, code = _pool_args(dtype, n, n_kv_heads, head_dim, k_cache, v_cache, slots, k_scale, v_scale)
     dev = _lib.same_device(k_new, v_new, k_cache, v_cache, slots, k_scale, v_scale)
-    _lib.call_on(dev, "ns_rope_append", None, k_new.data_ptr(), v_new.data_ptr(), 0, k_new.stride(0), v_new.stride(0), None, None, 0, 0, None,
-                 None, None, *pool, n, n_slots, 0, n_kv_heads, head_dim, block_size, *strides, _lib.dtype_code(dtype), code)
+    _lib.rope_append(dev, 0, k_new.data_ptr(), v_new.data_ptr(), 0, k_new.stride(0), v_new.stride(0), 0, 0, 0, 0, 0, 0, 0, *pool, n, n_slots, 0,
+                     n_kv_heads, head_dim, block_size, *strides, _lib.dtype_code(dtype), code)
 
 
 def kv_values(pool: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -166,7 +170,7 @@ def kv_values(pool: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torc
         raise NotImplementedError(f"kv_values reads int8 and float8_e4m3fn pools, not {pool.dtype}")
     assert pool.dim() == 4 and pool.stride(3) == 1
     strides = check_kv8_scales(pool, scale)
-    out = torch.empty(pool.shape, device=pool.device, dtype=dtype)
-    _lib.call_on(dev, "ns_kv_values", pool.data_ptr(), scale.data_ptr(), out.data_ptr(), *pool.shape, *pool.stride()[:3], *strides,
-                 _lib.dtype_code(dtype), code)
+    out = scale.new_empty(pool.shape) if dtype is torch.float32 else scale.new_empty(pool.shape, dtype=dtype)
+    _lib.kv_values(dev, pool.data_ptr(), scale.data_ptr(), out.data_ptr(), *pool.shape, *pool.stride()[:3], *strides, _lib.dtype_code(dtype),
+                   code)
     return out

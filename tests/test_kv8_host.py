@@ -79,6 +79,24 @@ def test_attention_workspace_refusals():
     assert f(ws=P(4096), wsb=need - 1, wss=2, wst=2) == WORKSPACE and "needed" in msg()
 
 
+def test_packed_calls():
+    """The same checks behind ns_call, and its own: an operation it does not know, a wrong number of words, none at all."""
+    import struct
+    f = _lib.load().ns_call
+    words = struct.pack("=2qd5q", 0, 0, 1.0, 0, 0, 1, 4, 0)
+    assert f(0, words, 8) == INVALID and "null" in msg()
+    assert f(0, words, 7) == INVALID and "takes 8 words, not 7" in msg()
+    assert f(0, None, 8) == INVALID
+    assert f(4, words, 8) == INVALID and "unknown operation 4" in msg() and f(-1, words, 8) == INVALID
+    plain = [a.value if isinstance(a, (ctypes.c_void_p, ctypes.c_float)) else a or 0 for a in rope_args(bs=24)]
+    assert f(1, struct.pack("=32q", *plain), 32) == UNSUPPORTED and "blocks of" in msg()
+    plain = [a.value if isinstance(a, (ctypes.c_void_p, ctypes.c_float)) else a or 0 for a in attn_args(nh=15)]
+    assert f(3, struct.pack("=26qd7q", *plain), 34) == INVALID and "15 heads not divisible" in msg()
+    assert f(2, struct.pack("=15q", 256, 512, 1024, 2, 16, 2, 64, 2048, 128, 64, 2, 1, _lib.NS_INT8, _lib.NS_INT8, 0), 15) == UNSUPPORTED
+    for op, count in ((_lib.rope_tables, 8), (_lib.rope_append, 32), (_lib.kv_values, 15), (_lib.ragged_paged_attn_q8, 34)):
+        assert op.words == count == len(_lib.SIGNATURES[op.name][1])
+
+
 def test_a_workspace_of_another_shape_is_refused():
     """Its counters lie elsewhere: they would be found non-zero."""
     from nanoserve_b200.kernels.paged_attention import AttnWorkspace, paged_attention_decode
