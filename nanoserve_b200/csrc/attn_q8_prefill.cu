@@ -21,7 +21,7 @@
 // when a row's reference has to move; A and B fill each other's gaps. Barriers are asked for ahead of the wait. Every mbarrier wait is
 // bounded: on expiry the CTA counts an error in the plan header (ns_collect_status), skips its stores, frees its tensor memory and
 // returns.
-// What bounds it (2,048 tokens on 6,001 keys, 28 / 4 heads of 128: 306 us, 674 TFLOP/s of the rows that exist; 256 items on 148 SMs
+// What bounds it (2,048 tokens on 6,001 keys, 28 / 4 heads of 128: 302 us, 682 TFLOP/s of the rows that exist; 256 items on 148 SMs
 // are two rounds, the second three quarters full, and seven of eight head slots are used): with
 // the softmax and the conversion cut out the same chain of waits and products takes 208 us, with the softmax alone cut out 239, with
 // the conversion alone cut out 298. Q is read again for every 64 keys, which makes 48 cycles of shared memory for 32 of arithmetic in Q.K
