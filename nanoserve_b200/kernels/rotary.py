@@ -67,7 +67,7 @@ def rope_tables(positions: torch.Tensor, inv_freq: torch.Tensor, factor: float =
     assert positions.dtype is torch.int64 and positions.dim() == 1 and positions.is_contiguous()
     assert inv_freq.dtype is torch.float32 and inv_freq.dim() == 1 and inv_freq.is_contiguous()
     t, half = positions.shape[0], inv_freq.shape[0]
-    cos = inv_freq.new_empty((t, half))
+    cos = inv_freq.new_empty(t, half)
     sin = torch.empty_like(cos)
     _lib.rope_tables(dev, positions.data_ptr(), inv_freq.data_ptr(), factor, cos.data_ptr(), sin.data_ptr(), t, half)
     return cos, sin
@@ -137,8 +137,8 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, n_heads
     assert cos.is_contiguous() and sin.is_contiguous() and 2 * half <= head_dim
     pool, n_slots, block_size, strides, code = _pool_args(dtype, n, n_kv_heads, head_dim, k_cache, v_cache, slots, k_scale, v_scale)
     dev = _lib.same_device(qkv, cos, sin, k_cache, v_cache, slots, k_scale, v_scale)
-    q = qkv.new_empty((n, n_heads, head_dim))
-    k = torch.empty((n, n_kv_heads, head_dim), device=qkv.device, dtype=dtype) if dense_kv else None
+    q = qkv.new_empty(n, n_heads, head_dim)
+    k = qkv.new_empty(n, n_kv_heads, head_dim) if dense_kv else None
     v = torch.empty_like(k) if dense_kv else None
     base, size = qkv.data_ptr(), 2 if dtype is torch.bfloat16 else 4
     base_k = base + n_heads * head_dim * size
@@ -170,7 +170,7 @@ def kv_values(pool: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torc
         raise NotImplementedError(f"kv_values reads int8 and float8_e4m3fn pools, not {pool.dtype}")
     assert pool.dim() == 4 and pool.stride(3) == 1
     strides = check_kv8_scales(pool, scale)
-    out = scale.new_empty(pool.shape) if dtype is torch.float32 else scale.new_empty(pool.shape, dtype=dtype)
+    out = scale.new_empty(*pool.shape) if dtype is torch.float32 else scale.new_empty(pool.shape, dtype=dtype)
     _lib.kv_values(dev, pool.data_ptr(), scale.data_ptr(), out.data_ptr(), *pool.shape, *pool.stride()[:3], *strides, _lib.dtype_code(dtype),
                    code)
     return out
