@@ -475,6 +475,12 @@ template <typename T, typename KV, int V> __device__ void append_large(const Rop
     const int head = cta % p.n_kv_heads, bs = p.block_size, mask = bs - 1;
     const int t0 = (cta / p.n_kv_heads) * p.chunk, n_tok = (int)p.n_tokens;
     auto hash = [](int b) -> int { return (int)(((uint32_t)b * 2654435761u) >> 16) & (kSlotsOfTable - 1); };
+    int64_t slot[8];                                                      // the first of all slots, asked for before anything else
+    auto request = [&](int base) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) slot[k] = base + k * kLargeThreads < n_tok ? p.slots[base + k * kLargeThreads] : -1;
+    };
+    request(tid);
     if (tid == 0) n_cand = 0, filter = 0;
     for (int i = tid; i < p.chunk * bs; i += blockDim.x) member[i] = -1;
     for (int i = tid; i < kSlotsOfTable; i += blockDim.x) key[i] = -1;
@@ -516,9 +522,7 @@ template <typename T, typename KV, int V> __device__ void append_large(const Rop
     // Every CTA looks at every slot, so a slot that is nobody's must cost little: bit (block & 31) of `seen` turns most of them away.
     const uint32_t seen = filter;
     for (int base = tid; base < n_tok; base += 8 * kLargeThreads) {       // eight slots in flight
-        int64_t slot[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) slot[k] = base + k * kLargeThreads < n_tok ? p.slots[base + k * kLargeThreads] : -1;
+        if (base != tid) request(base);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
             if (!((seen >> ((uint32_t)(slot[k] >> p.block_shift) & 31u)) & 1u)) continue;
