@@ -93,3 +93,47 @@ def test_split_captured_then_replayed_with_other_lengths():
         want = R.attend_fast(q, kv, vv, tables, torch.tensor([n]), cu, 0.125)
         tol = R.attend_tolerance(q, kv, vv, tables, torch.tensor([n]), 0.125, want, torch.bfloat16, 11)
         assert bool(((out.cpu().double() - want).abs() <= tol).all()), n
+
+
+@pytest.mark.parametrize("simple", [True, False])
+@pytest.mark.parametrize("lens,q_lens", [([5, 30], [40, 33]), ([600, 3, 1], [700, 16, 1])])
+def test_fewer_keys_than_tokens(lens, q_lens, simple):
+    """A chunk longer than its sequence: the first tokens see nothing and get zeros, the others what is left of the keys."""
+    from nanoserve_b200.kernels.paged_attention import ragged_paged_attention
+    q, k, v, ks, vs, tables, lens, cu = make_case(4, 2, 64, lens, torch.int8, torch.bfloat16, q_lens)
+    kv, vv = R.values(k, ks), R.values(v, vs)
+    want = R.attend_fast(q, kv, vv, tables, lens, cu, 0.125)
+    got = ragged_paged_attention(*[x.cuda() for x in (q, k, v, tables, lens, cu)], 0.125, k_scale=ks.cuda(), v_scale=vs.cuda(), simple=simple)
+    tol = R.attend_tolerance(q, kv, vv, tables, lens, 0.125, want, torch.bfloat16, None if simple else 11)
+    assert bool(((got.cpu().double() - want).abs() <= tol).all())
+    assert bool((got[:q_lens[0] - int(lens[0])] == 0).all())
+
+
+@pytest.mark.parametrize("simple", [True, False])
+@pytest.mark.parametrize("scale", [-0.125, 0.0])
+@pytest.mark.parametrize("lens,q_lens", [([300, 40, 9], [1, 1, 1]), ([700, 50], [90, 17])])
+def test_scales_of_the_scores_that_are_not_positive(lens, q_lens, scale, simple):
+    from nanoserve_b200.kernels.paged_attention import ragged_paged_attention
+    q, k, v, ks, vs, tables, lens, cu = make_case(14, 2, 64, lens, torch.float8_e4m3fn, torch.bfloat16, q_lens)
+    kv, vv = R.values(k, ks), R.values(v, vs)
+    want = R.attend_fast(q, kv, vv, tables, lens, cu, scale)
+    got = ragged_paged_attention(*[x.cuda() for x in (q, k, v, tables, lens, cu)], scale, k_scale=ks.cuda(), v_scale=vs.cuda(), simple=simple)
+    tol = R.attend_tolerance(q, kv, vv, tables, lens, abs(scale), want, torch.bfloat16, None if simple else 11)
+    assert bool(((got.cpu().double() - want).abs() <= tol).all())
+
+
+def test_calls_on_another_stream_than_the_default():
+    """Append and attention on a side stream, the plan included, while the default stream is busy with something else."""
+    from nanoserve_b200.kernels.paged_attention import ragged_paged_attention
+    case = make_case(14, 2, 64, [700, 1, 90], torch.int8, torch.bfloat16, [100, 1, 8])
+    want = attend(case, False)
+    q, k, v, ks, vs, tables, lens, cu = [t.cuda() for t in case]
+    torch.cuda.synchronize()
+    noise = torch.randn(2048, 2048, device="cuda")
+    side = torch.cuda.Stream()
+    for _ in range(5):
+        noise = (noise @ noise).clamp(-1, 1)
+        with torch.cuda.stream(side):
+            got = ragged_paged_attention(q, k, v, tables, lens, cu, 0.125, k_scale=ks, v_scale=vs)
+        side.synchronize()
+        assert torch.equal(got, want)
